@@ -166,6 +166,68 @@ int zt_attn_decode_step(const float *q, const float *k_new, const float *v_new, 
                         float *out, const int *pos, int B, int n_ctx, int n_heads, int n_kv_heads, int dim,
                         double theta, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- Paged KV cache (no reference counterpart) -------------------------
+ * A pool of pages shared by sequences of different lengths, for serving.
+ * k_pages/v_pages [n_pages, page_size, n_kv_heads*dim], page_size a power of two
+ * in [1, 1024], n_pages * page_size < 2^31.  table [B, table_stride] (DEVICE
+ * ints): row s of sequence b is row s % page_size of page table[b][s / page_size];
+ * entries past a sequence's last page are not read.  Sequences may share pages
+ * that are only read.  The kernels check every page number that they use: one
+ * outside [0, n_pages) is never followed, its rows are not written, and an
+ * output row that sees one comes out NaN.
+ * The batch is ragged.  q_start (HOST, B + 1 ints, not descending): the new tokens
+ * of sequence b are the packed rows q_start[b] .. q_start[b + 1] - 1 of q, out,
+ * k_new, v_new; rows outside [q_start[0], q_start[B]) are left as they are.
+ * n_rows (HOST, B ints): the rows of each sequence's cache WITH its new tokens,
+ * which are the last; a sequence may have no new tokens, or no rows.
+ * w [B, n_kv_heads, w_stride]: for each row and kv head the attention weight
+ * that it has drawn so far, by sequence (not by page).  Keys are stored after
+ * RoPE, so a row keeps its position when an eviction moves it.
+ * The host arrays are read during the call; a captured call replays with the
+ * lengths it was captured with.  Calls whose outputs do not overlap may run at the
+ * same time on different streams, each with a workspace of its own.
+ *
+ * zt_paged_append: q_out = RoPE(q), K row = RoPE(k_new), V row = v_new (as
+ * zt_rope_forward), w row = 0.  pos (HOST, B ints): the position of each
+ * sequence's first new token (after an eviction it is past the row).  q and q_out
+ * may both be null, or the same buffer; w may be null.  A page table must not name
+ * one page twice among the rows that a call writes. */
+int zt_paged_append(const float *q, const float *k_new, const float *v_new, float *q_out, float *k_pages, float *v_pages,
+                    const int *table, float *w, const int *q_start, const int *n_rows, const int *pos, int B, int n_pages,
+                    int page_size, int table_stride, int w_stride, int n_heads, int n_kv_heads, int dim, double theta,
+                    hipStream_t stream);
+
+/* Causal attention of the new tokens (one each: a decode step; all rows: a prompt) over
+ * their caches: token i of a sequence with L new ones sees rows 0 .. n_rows - L + i.
+ * lse [.., n_heads] (the natural log-sum-exp) may be null.  With w_in and w_out
+ * (both or neither; the same buffer or two that do not overlap) also
+ * w_out[b, j, s] = w_in[b, j, s] + the sum of row s's softmax weights over the new
+ * tokens and the query heads of kv head j, for s < n_rows[b]; later w_out are left
+ * as they are.  K and V rows that no token sees, and what they hold (inf, NaN), change
+ * no result.  `workspace`: zt_attn_paged_workspace(...) bytes for the same lengths,
+ * 16-byte aligned (null where that is 0). */
+size_t zt_attn_paged_workspace(const int *q_start, const int *n_rows, int B, int n_heads, int n_kv_heads, int dim,
+                               int weights);
+int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, float *out, float *lse,
+                  const float *w_in, float *w_out, const int *q_start, const int *n_rows, int B, int n_pages,
+                  int page_size, int table_stride, int w_stride, int n_heads, int n_kv_heads, int dim, void *workspace,
+                  size_t workspace_bytes, hipStream_t stream);
+
+/* Eviction by accumulated weight.  A sequence of more than `budget` rows keeps, in each kv
+ * head by itself, its first n_first rows, its last n_last, and of the others the budget -
+ * n_first - n_last with the largest w_in (equal weights: the lower row; NaN is
+ * less than everything).  The kept rows, in order of their row, become rows 0 .. budget - 1
+ * of table_out's pages, and their weights w_out's.  kept [B, n_kv_heads, budget]
+ * (device ints) receives the row that each was, -1 past a sequence's last.  A sequence within the
+ * budget keeps all rows.  The sequence's new n_rows is min(n_rows, budget).
+ * table_out is table (in place: the sequences' pages must not be shared) or
+ * another table of the same stride, none of whose pages is in table (a copy: table's
+ * pages, which may be shared, stay as they are); w_out is w_in or a buffer that
+ * does not overlap it. */
+int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *table_out, const float *w_in,
+                   float *w_out, int *kept, const int *n_rows, int B, int n_pages, int page_size, int table_stride,
+                   int w_stride, int n_kv_heads, int dim, int n_first, int n_last, int budget, hipStream_t stream);
+
 /* RMSNorm, src/norm.zig:18-47 on the device (the reference's src/cuda/norm.cu
  * kernel has no C entry point).  x/y [rows, cols], w [cols]; eps is
  * src/norm.zig:14's 1e-5 for the reference's behaviour.  rows == 0 launches

@@ -1,0 +1,466 @@
+"""The paged cache on the GPU against pagedref (64 bits): append, attention of one and more new tokens, accumulated
+weights, eviction, and a serving run of all of them."""
+import numpy as np
+import pytest
+
+import pagedref
+
+pytestmark = pytest.mark.gpu
+EPS = pagedref.EPS
+
+
+class Cache:
+    """Pools and tables of a ragged batch; pages dealt at random, entries behind a sequence's last name no page."""
+
+    def __init__(self, torch, rng, n_rows, page, Hkv, d, spare=1, garbage=None):
+        used = [-(-n // page) for n in n_rows]
+        self.n_rows, self.page, self.Hkv, self.d = list(n_rows), page, Hkv, d
+        self.n_pages = sum(used) + spare
+        order = rng.permutation(self.n_pages)
+        self.table_h = np.full((len(n_rows), max(max(used), 1)), -1, np.int32)
+        at = 0
+        for b, u in enumerate(used):
+            self.table_h[b, :u] = order[at:at + u]
+            at += u
+        shape = (self.n_pages * page, Hkv, d)
+        self.k_h, self.v_h = (rng.standard_normal(shape).astype(np.float32) for _ in range(2))
+        if garbage is not None:  # rows that are nobody's
+            mine = np.zeros(shape[0], bool)
+            for b, n in enumerate(n_rows):
+                mine[pagedref.places(self.table_h, b, n, page)] = True
+            self.k_h[~mine] = garbage
+            self.v_h[~mine] = garbage
+        self.k, self.v, self.table = (torch.from_numpy(x.copy()).cuda() for x in (self.k_h, self.v_h, self.table_h))
+
+
+def run_attend(gpu, zt, c, q_h, q_start, H, w_h=None, lse=True, stream=None):
+    """out, lse, w as numpy; buffers' rows that no token has, and the workspace, begin as NaN."""
+    q = gpu.from_numpy(np.ascontiguousarray(q_h, np.float32)).cuda()
+    out = gpu.full_like(q, float("nan"))
+    l = gpu.full(q.shape[:2], float("nan"), device="cuda") if lse else None
+    w_in = None if w_h is None else gpu.from_numpy(w_h.copy()).cuda()
+    w_out = None if w_h is None else gpu.full_like(w_in, -7.0)
+    need = zt.attn_paged_workspace_bytes(q_start, c.n_rows, H, c.Hkv, c.d, w_h is not None)
+    ws = gpu.full((need // 4,), float("nan"), device="cuda") if need else None
+    if stream is not None:
+        stream.wait_stream(gpu.cuda.current_stream())
+    zt.attn_paged(q, c.k, c.v, c.table, out, q_start, c.n_rows, c.page, H, c.Hkv, c.d, ws, l, w_in, w_out, stream)
+    gpu.cuda.synchronize()
+    return [None if t is None else t.cpu().numpy() for t in (out, l, w_out)]
+
+
+def grade(got, ref, q_start, n_rows, Hkv, w_h=None):
+    out, lse, w = got
+    r_out, r_lse, r_w, bound, w_bound = ref
+    rows = slice(q_start[0], q_start[-1])
+    assert np.all(np.abs(out[rows] - r_out[rows]) <= bound[rows])
+    assert np.all(np.isnan(out[:q_start[0]])) and np.all(np.isnan(out[q_start[-1]:]))
+    if lse is not None:
+        # The scores' error, the sum's (at most expm1(e) + n EPS, in `bound`'s terms) and the logarithm's.
+        top = (bound[rows] / np.maximum(np.abs(r_out[rows]), 1e-30)).min(-1)
+        assert np.all(np.abs(lse[rows] - r_lse[rows]) <= top + 4 * EPS * np.abs(r_lse[rows]) + 8 * EPS)
+        assert np.all(np.isnan(lse[:q_start[0]])) and np.all(np.isnan(lse[q_start[-1]:]))
+    if w_h is not None:
+        for b, n in enumerate(n_rows):
+            want = w_h[b, :, :n] + r_w[b, :, :n]
+            assert np.all(np.abs(w[b, :, :n] - want) <= w_bound[b, :, :n] + 2 * EPS * np.abs(want))
+            assert np.all(w[b, :, n:] == -7.0)
+
+
+SHAPES = [(4, 2, 32), (8, 8, 64), (6, 2, 64), (32, 8, 128), (8, 2, 96), (16, 4, 256), (5, 1, 128), (40, 2, 32), (2, 1, 160),
+          (4, 4, 34), (6, 3, 50), (9, 3, 250), (8, 2, 132), (4, 1, 192), (8, 4, 40)]
+# (rows with the new tokens, new tokens): one token, none, no rows, ends inside a 16-key tile and at it, prompts.
+BATCHES = {
+    "single_tokens": ([1, 2, 15, 16, 17, 33, 200], [1] * 7),
+    "ragged": ([40, 0, 7, 64, 129, 31, 5], [3, 0, 7, 0, 17, 31, 1]),
+    "long": ([700], [2]),
+    "chunk": ([333], [90]),
+}
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("page", [1, 8, 16, 64])
+@pytest.mark.parametrize("H,Hkv,d", SHAPES)
+def test_attention_and_weights(gpu, zt, H, Hkv, d, page, batch):
+    n_rows, q_len = BATCHES[batch]
+    rng = np.random.default_rng([H, Hkv, d, page, len(n_rows)])
+    c = Cache(gpu, rng, n_rows, page, Hkv, d, garbage=np.nan)
+    q_start = np.cumsum([2] + q_len).tolist()  # the packed tokens begin behind two that are not this call's
+    q = rng.standard_normal((q_start[-1] + 3, H, d)).astype(np.float32)
+    w = rng.random((len(n_rows), Hkv, max(n_rows) + 5), np.float32)
+    ref = pagedref.attend(q, c.k_h, c.v_h, c.table_h, q_start, n_rows, page, H, Hkv, d)
+    grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
+    plain = run_attend(gpu, zt, c, q, q_start, H, lse=False)
+    grade(plain, ref, q_start, n_rows, Hkv)
+    # In whole: the 2-norm of the difference, roundings adding up as independent ones, with a factor of four.
+    rows, n = slice(q_start[0], q_start[-1]), max(n_rows)
+    off = np.linalg.norm(plain[0][rows] - ref[0][rows]) / np.linalg.norm(ref[0][rows])
+    assert off <= 4 * EPS * (np.sqrt(d) + np.sqrt(n) + 16)
+
+
+def test_more_sequences_than_a_launch_takes(gpu, zt):
+    B, H, Hkv, d, page = 150, 4, 2, 32, 8
+    rng = np.random.default_rng(5)
+    n_rows = [int(x) for x in rng.integers(0, 60, B)]
+    n_rows[70] = 2500  # enough to be cut into chunks
+    q_len = [min(n, int(rng.integers(0, 12)) if i % 3 else 1) for i, n in enumerate(n_rows)]
+    c = Cache(gpu, rng, n_rows, page, Hkv, d, garbage=np.inf)
+    q_start = np.cumsum([0] + q_len).tolist()
+    q = rng.standard_normal((q_start[-1], H, d)).astype(np.float32)
+    w = rng.random((B, Hkv, max(n_rows)), np.float32)
+    ref = pagedref.attend(q, c.k_h, c.v_h, c.table_h, q_start, n_rows, page, H, Hkv, d)
+    grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
+
+
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("L,n", [(9, 40), (70, 130), (150, 150)])
+@pytest.mark.parametrize("H,Hkv,d", [(4, 2, 32), (8, 2, 128), (6, 2, 50), (4, 1, 256)])
+def test_what_a_token_does_not_see_changes_nothing(gpu, zt, H, Hkv, d, L, n, value):
+    """K and V of the last token's row not finite: tokens before it as without, bit for bit; it itself as 64 bits have it."""
+    rng = np.random.default_rng([H, d, L])
+    c = Cache(gpu, rng, [n], 16, Hkv, d)
+    q = rng.standard_normal((L, H, d)).astype(np.float32)
+    w = np.zeros((1, Hkv, n), np.float32)
+    out0, lse0, w0 = run_attend(gpu, zt, c, q, [0, L], H, w)
+    last = pagedref.places(c.table_h, 0, n, 16)[-1]
+    c.v[last, :, 3] = float(value)
+    out1, lse1, w1 = run_attend(gpu, zt, c, q, [0, L], H, w)
+    assert np.array_equal(out0[:-1], out1[:-1]) and np.array_equal(lse0, lse1) and np.array_equal(w0, w1)
+    keep = np.arange(d) != 3
+    assert np.array_equal(out0[-1][:, keep], out1[-1][:, keep])
+    assert np.all(np.isnan(out1[-1, :, 3]) if np.isnan(value) else out1[-1, :, 3] == value)
+    c.k[last] = float(value)
+    out2, lse2, w2 = run_attend(gpu, zt, c, q, [0, L], H, w)
+    assert np.array_equal(out0[:-1], out2[:-1]) and np.array_equal(lse0[:-1], lse2[:-1])
+    # inf * q over columns of both signs: NaN scores, and with them the token's whole row.
+    assert np.all(np.isnan(out2[-1])) and np.all(np.isnan(lse2[-1]))
+
+
+@pytest.mark.parametrize("bad", [-1, 10 ** 9, "n_pages"])
+@pytest.mark.parametrize("L", [6, 80])
+def test_a_page_of_no_pool_is_not_followed(gpu, zt, bad, L):
+    H, Hkv, d, page, n = 4, 2, 64, 8, 200
+    rng = np.random.default_rng(9)
+    c = Cache(gpu, rng, [n, n], page, Hkv, d)
+    q = rng.standard_normal((2 * L, H, d)).astype(np.float32)
+    q_start, w = [0, L, 2 * L], np.zeros((2, Hkv, n), np.float32)
+    good = run_attend(gpu, zt, c, q, q_start, H, w)
+    c.table[1, -1] = c.n_pages if bad == "n_pages" else bad  # sequence 1's last 8 rows
+    out, lse, w1 = run_attend(gpu, zt, c, q, q_start, H, w)
+    see = 2 * L - min(L, page)  # the first token that sees one of them
+    assert np.array_equal(out[:see], good[0][:see]) and np.array_equal(lse[:see], good[1][:see])
+    assert np.all(np.isnan(out[see:])) and np.all(np.isnan(lse[see:]))
+    assert np.array_equal(w1[0], good[2][0]) and np.all(np.isnan(w1[1]))
+
+
+@pytest.mark.parametrize("H,Hkv,d,page", [(4, 2, 32, 1), (32, 8, 128, 16), (6, 2, 50, 8), (16, 4, 256, 64), (3, 1, 34, 4)])
+@pytest.mark.parametrize("with_q", [True, False])
+def test_append(gpu, zt, H, Hkv, d, page, with_q):
+    rng = np.random.default_rng([H, d])
+    n_rows = [int(x) for x in rng.integers(0, 90, 80)]
+    q_len = [min(n, [0, 1, 3, 40][i % 4]) for i, n in enumerate(n_rows)]
+    pos = [n - l + 5000 * (i % 2) for i, (n, l) in enumerate(zip(n_rows, q_len))]
+    c = Cache(gpu, rng, n_rows, page, Hkv, d)
+    q_start = np.cumsum([3] + q_len).tolist()
+    N = q_start[-1] + 2
+    q, kn, vn = (rng.standard_normal((N, h, d)).astype(np.float32) for h in (H, Hkv, Hkv))
+    w = rng.random((80, Hkv, max(n_rows) + 1), np.float32)
+    dq, dk, dv, dw = (gpu.from_numpy(x).cuda() for x in (q, kn, vn, w))
+    q_out = gpu.full_like(dq, -7.0)
+    zt.paged_append(dq if with_q else None, dk, dv, q_out if with_q else None, c.k, c.v, c.table, q_start, n_rows, pos, page,
+                    H, Hkv, d, 10000.0, dw)
+    gpu.cuda.synchronize()
+    k, v, q_want = c.k_h.astype(np.float64), c.v_h.copy(), np.full(q.shape, -7.0)
+    for b, n in enumerate(n_rows):
+        t0, t1 = q_start[b], q_start[b + 1]
+        at = pagedref.places(c.table_h, b, n, page)[n - (t1 - t0):]
+        k[at], v[at] = pagedref.rotate(kn[t0:t1], pos[b], 10000.0), vn[t0:t1]
+        q_want[t0:t1] = pagedref.rotate(q[t0:t1], pos[b], 10000.0)
+        w[b, :, n - (t1 - t0):n] = 0
+    # One rounding to f32 of a value in 64 bits: half a step, and the 64-bit angle's own error (5000 radians x 2^-52).
+    assert np.all(np.abs(c.k.cpu().numpy() - k) <= EPS * np.abs(k) + 1e-11)
+    assert np.array_equal(c.v.cpu().numpy(), v) and np.array_equal(dw.cpu().numpy(), w)
+    if with_q:
+        assert np.all(np.abs(q_out.cpu().numpy() - q_want) <= EPS * np.abs(q_want) + 1e-11)
+        zt.paged_append(dq, dk, dv, dq, c.k, c.v, c.table, q_start, n_rows, pos, page, H, Hkv, d, 10000.0)  # in place
+        rows = slice(q_start[0], q_start[-1])
+        assert gpu.equal(dq[rows], q_out[rows])
+
+
+def test_append_rotates_as_the_contiguous_entry_does(gpu, zt):
+    """Bit for bit what zt_rope_qk_forward writes."""
+    T, H, Hkv, d = 37, 8, 2, 64
+    rng = np.random.default_rng(2)
+    c = Cache(gpu, rng, [T], 16, Hkv, d)
+    q, k, v = (gpu.randn(T, h, d, device="cuda") for h in (H, Hkv, Hkv))
+    q_out, q_rope, k_rope = gpu.empty_like(q), gpu.empty_like(q), gpu.empty_like(k)
+    zt.paged_append(q, k, v, q_out, c.k, c.v, c.table, [0, T], [T], [11], 16, H, Hkv, d)
+    zt.rope_qk(q, k, q_rope, k_rope, 1, T, H, Hkv, d, pos=11)
+    at = gpu.from_numpy(pagedref.places(c.table_h, 0, T, 16)).cuda()
+    assert gpu.equal(q_out, q_rope) and gpu.equal(c.k[at], k_rope)
+
+
+def test_append_writes_no_page_of_no_pool(gpu, zt):
+    H, Hkv, d, page = 2, 2, 32, 4
+    rng = np.random.default_rng(4)
+    c = Cache(gpu, rng, [12], page, Hkv, d, spare=3)
+    c.table[0, 1], c.table[0, 2] = -5, c.n_pages
+    before = c.k.clone(), c.v.clone()
+    k, v = gpu.randn(12, Hkv, d, device="cuda"), gpu.randn(12, Hkv, d, device="cuda")
+    zt.paged_append(None, k, v, None, c.k, c.v, c.table, [0, 12], [12], [0], page, H, Hkv, d)
+    first = gpu.from_numpy(pagedref.places(c.table_h, 0, 4, page)).cuda()
+    assert gpu.equal(c.v[first], v[:4])
+    before[0][first], before[1][first] = c.k[first], c.v[first]
+    assert gpu.equal(c.k, before[0]) and gpu.equal(c.v, before[1])
+
+
+def _weights(rng, B, Hkv, n, kind):
+    w = rng.random((B, Hkv, n), np.float32) ** 4 * 8
+    if kind == "ties":
+        w = np.floor(w)
+    elif kind == "equal":
+        w[:] = 0.25
+    elif kind == "odd":  # everything that f32 holds
+        w = rng.integers(0, 1 << 32, (B, Hkv, n), dtype=np.uint32).view(np.float32).copy()
+        w[rng.random(w.shape) < 0.2] = np.nan
+        w[rng.random(w.shape) < 0.1] = np.inf
+        w[rng.random(w.shape) < 0.1] = -0.0
+        w[rng.random(w.shape) < 0.1] = 0.0
+    return w
+
+
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "odd"])
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("n_rows,budget,first,last,Hkv,d,page", [
+    ([40, 7, 33, 0, 32], 32, 4, 8, 2, 32, 1), ([500, 130, 129], 128, 0, 0, 8, 128, 16), ([200, 90], 64, 32, 32, 3, 50, 8),
+    ([2100], 1, 0, 0, 1, 64, 16), ([2100], 1, 1, 0, 2, 34, 16), ([5000, 1500], 1300, 4, 64, 2, 96, 64),
+    ([300], 299, 0, 7, 4, 256, 4), ([90, 20], 200, 4, 4, 2, 32, 8), ([20000], 9000, 1, 1, 1, 32, 16)])
+def test_eviction(gpu, zt, n_rows, budget, first, last, Hkv, d, page, in_place, kind):
+    rng = np.random.default_rng([len(n_rows), budget, d])
+    B, stride = len(n_rows), max(n_rows) + 3
+    c = Cache(gpu, rng, n_rows + [budget] * B, page, Hkv, d)
+    table = c.table[:B].contiguous()
+    table_out = table if in_place else c.table[B:].contiguous()
+    out_h = c.table_h[:B] if in_place else c.table_h[B:]
+    w = _weights(rng, B, Hkv, stride, kind)
+    w_in = gpu.from_numpy(w).cuda()
+    w_out = w_in if in_place else gpu.full_like(w_in, -7.0)
+    kept = gpu.full((B, Hkv, budget), 12345, device="cuda", dtype=gpu.int32)
+    zt.paged_evict(c.k, c.v, table, table_out, w_in, w_out, kept, n_rows, page, Hkv, d, first, last, budget)
+    gpu.cuda.synchronize()
+    k, v = c.k_h.copy(), c.v_h.copy()
+    w_want = w.copy() if in_place else np.full_like(w, -7.0)
+    kept_want = np.full((B, Hkv, budget), -1)
+    for b, n in enumerate(n_rows):
+        src = pagedref.places(c.table_h, b, n, page)
+        dst = pagedref.places(out_h, b, min(n, budget), page)
+        for h in range(Hkv):
+            rows = pagedref.evict(w[b, h], n, budget, first, last)
+            kept_want[b, h, :len(rows)] = rows
+            k[dst, h], v[dst, h] = c.k_h[src[rows], h], c.v_h[src[rows], h]
+            w_want[b, h, :len(rows)] = w[b, h, rows]
+    assert np.array_equal(kept.cpu().numpy(), kept_want)
+    assert np.array_equal(c.k.cpu().numpy(), k) and np.array_equal(c.v.cpu().numpy(), v)
+    assert np.array_equal(w_out.cpu().numpy().view(np.uint32), w_want.view(np.uint32))
+
+
+def test_eviction_of_many_sequences(gpu, zt):
+    B, Hkv, d, page, budget = 130, 2, 32, 8, 24
+    rng = np.random.default_rng(6)
+    n_rows = [int(x) for x in rng.integers(0, 60, B)]
+    c = Cache(gpu, rng, n_rows, page, Hkv, d)
+    w = rng.random((B, Hkv, 60), np.float32)
+    w_dev = gpu.from_numpy(w).cuda()
+    kept = gpu.empty((B, Hkv, budget), device="cuda", dtype=gpu.int32)
+    zt.paged_evict(c.k, c.v, c.table, c.table, w_dev, w_dev, kept, n_rows, page, Hkv, d, 2, 5, budget)
+    kept, k = kept.cpu().numpy(), c.k.cpu().numpy()
+    for b, n in enumerate(n_rows):
+        at = pagedref.places(c.table_h, b, n, page)
+        for h in range(Hkv):
+            rows = pagedref.evict(w[b, h], n, budget, 2, 5)
+            assert np.array_equal(kept[b, h, :len(rows)], rows) and np.all(kept[b, h, len(rows):] == -1)
+            assert np.array_equal(k[at[:len(rows)], h], c.k_h[at[rows], h])
+
+
+def test_eviction_follows_no_page_of_no_pool(gpu, zt):
+    Hkv, d, page, budget = 2, 32, 4, 8
+    rng = np.random.default_rng(8)
+    for in_place in (True, False):
+        c = Cache(gpu, rng, [20, 8], page, Hkv, d)
+        w = gpu.rand(1, Hkv, 20, device="cuda")
+        table = c.table[:1].clone()
+        table[0, 3] = c.n_pages + 7
+        out = table if in_place else c.table[1:].clone()
+        kept = gpu.empty((1, Hkv, budget), device="cuda", dtype=gpu.int32)
+        zt.paged_evict(c.k, c.v, table, out, w, w.clone() if not in_place else w, kept, [20], page, Hkv, d, 1, 2, budget)
+        rows = kept.cpu().numpy()[0]
+        src = pagedref.places(c.table_h, 0, 20, page)
+        dst = src[:budget] if in_place else pagedref.places(c.table_h, 1, budget, page)
+        want = c.k_h.copy()
+        for h in range(Hkv):
+            ok = rows[h] // page != 3  # rows of the page that is none stay where they were
+            want[dst[ok], h] = c.k_h[src[rows[h][ok]], h]
+        assert np.array_equal(c.k.cpu().numpy(), want)
+
+
+def test_offsets_past_32_bits(gpu, zt):
+    """A pool of 4.3e9 floats: rows whose element offsets do not fit 32 bits."""
+    H, Hkv, d, page, n = 8, 8, 256, 64, 200
+    pool_rows = (1 << 32) // (Hkv * d) // page * page + 4 * page
+    rng = np.random.default_rng(12)
+    c = Cache(gpu, rng, [n], page, Hkv, d, spare=0)
+    k, v = (gpu.empty(pool_rows * Hkv * d, device="cuda") for _ in range(2))
+    far = pool_rows // page - c.n_pages  # the pool's last pages take the small pool's place
+    k[far * page * Hkv * d:], v[far * page * Hkv * d:] = c.k.view(-1), c.v.view(-1)
+    near = c.k, c.v, c.table
+    q = rng.standard_normal((3, H, d)).astype(np.float32)
+    w = rng.random((1, Hkv, n), np.float32)
+    want = run_attend(gpu, zt, c, q, [0, 3], H, w)
+    many = rng.standard_normal((150, H, d)).astype(np.float32)
+    want_many = run_attend(gpu, zt, c, many, [0, 150], H, w)
+    c.k, c.v, c.table = k, v, near[2] + far
+    got = run_attend(gpu, zt, c, q, [0, 3], H, w)
+    got_many = run_attend(gpu, zt, c, many, [0, 150], H, w)
+    for x, y in zip(want + want_many, got + got_many):
+        assert np.array_equal(x, y)
+    new = gpu.randn(2, Hkv * d, device="cuda")
+    for kk, vv, table in (near, (k, v, c.table)):
+        zt.paged_append(None, new, new, None, kk, vv, table, [0, 2], [n], [n - 2], page, H, Hkv, d)
+    kept = gpu.empty((1, Hkv, 50), device="cuda", dtype=gpu.int32)
+    for kk, vv, table in (near, (k, v, c.table)):
+        wd = gpu.from_numpy(w).cuda()
+        zt.paged_evict(kk, vv, table, table, wd, wd, kept, [n], page, Hkv, d, 1, 3, 50)
+    assert gpu.equal(k[far * page * Hkv * d:], near[0].view(-1)) and gpu.equal(v[far * page * Hkv * d:], near[1].view(-1))
+
+
+def test_other_streams_and_two_at_once(gpu, zt):
+    H, Hkv, d, page = 8, 2, 64, 16
+    rng = np.random.default_rng(14)
+    cs = [Cache(gpu, rng, [900, 300], page, Hkv, d) for _ in range(2)]
+    q = rng.standard_normal((5, H, d)).astype(np.float32)
+    w = rng.random((2, Hkv, 900), np.float32)
+    want = [run_attend(gpu, zt, c, q, [0, 1, 5], H, w) for c in cs]
+    streams = [gpu.cuda.Stream() for _ in range(2)]
+    got = [run_attend(gpu, zt, c, q, [0, 1, 5], H, w, stream=s) for c, s in zip(cs, streams)]
+    for x, y in zip(sum(want, []), sum(got, [])):
+        assert np.array_equal(x, y)
+    # Both in flight together, each with its own buffers.
+    dq = gpu.from_numpy(q).cuda()
+    need = zt.attn_paged_workspace_bytes([0, 1, 5], [900, 300], H, Hkv, d)
+    outs = [gpu.empty_like(dq) for _ in cs]
+    spaces = [gpu.empty(need + 16, device="cuda", dtype=gpu.uint8) for _ in cs]
+    gpu.cuda.synchronize()
+    for _ in range(20):
+        for c, s, o, ws in zip(cs, streams, outs, spaces):
+            zt.attn_paged(dq, c.k, c.v, c.table, o, [0, 1, 5], [900, 300], page, H, Hkv, d, ws, stream=s)
+    gpu.cuda.synchronize()
+    for o, x in zip(outs, want):
+        assert np.array_equal(o.cpu().numpy(), x[0])
+
+
+def test_captured_and_replayed(gpu, zt):
+    """A step (append, attend with weights, evict to other pages) as one graph: replays with new contents in the same
+    buffers give what eager calls give."""
+    H, Hkv, d, page, B, n, budget = 8, 2, 64, 16, 3, 400, 128
+    rng = np.random.default_rng(15)
+    c = Cache(gpu, rng, [n] * B + [budget] * B, page, Hkv, d)
+    table, table_out = c.table[:B].contiguous(), c.table[B:].contiguous()
+    q_start = list(range(B + 1))
+    need = zt.attn_paged_workspace_bytes(q_start, [n] * B, H, Hkv, d, True)
+    ws = gpu.empty(need + 16, device="cuda", dtype=gpu.uint8)
+    q, kn, vn = (gpu.empty(B, h, d, device="cuda") for h in (H, Hkv, Hkv))
+    q_out, out = gpu.empty_like(q), gpu.empty_like(q)
+    w, w_out, w_kept = (gpu.zeros(B, Hkv, n, device="cuda") for _ in range(3))
+    kept = gpu.empty(B, Hkv, budget, device="cuda", dtype=gpu.int32)
+
+    def step():
+        zt.paged_append(q, kn, vn, q_out, c.k, c.v, table, q_start, [n] * B, [n + 9] * B, page, H, Hkv, d, w=w)
+        zt.attn_paged(q_out, c.k, c.v, table, out, q_start, [n] * B, page, H, Hkv, d, ws, w_in=w, w_out=w_out)
+        zt.paged_evict(c.k, c.v, table, table_out, w_out, w_kept, kept, [n] * B, page, Hkv, d, 2, 16, budget)
+
+    def fill(seed):
+        gen = gpu.Generator(device="cuda").manual_seed(seed)
+        for t in (q, kn, vn, w):
+            t.normal_(generator=gen)
+
+    def state():
+        return [t.clone() for t in (q_out, out, w_out, w_kept, kept, c.k, c.v)]
+
+    fill(0)
+    step()  # loads the code objects
+    gpu.cuda.synchronize()
+    graph = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(graph):
+        step()
+    def clean():  # rows that no call writes keep what they hold: the same before both
+        for t in (q_out, out, w_out, w_kept):
+            t.fill_(-1.0)
+        kept.fill_(-9)
+        ws.fill_(255)
+
+    for seed in (1, 2, 3):
+        clean()
+        fill(seed)
+        step()
+        want = state()
+        clean()
+        fill(seed)
+        graph.replay()
+        gpu.cuda.synchronize()
+        for x, y in zip(want, state()):
+            assert gpu.equal(x, y)
+
+
+@pytest.mark.parametrize("H,Hkv,d,page", [(8, 2, 64, 16), (4, 2, 32, 4), (6, 1, 50, 8)])
+def test_a_serving_run(gpu, zt, H, Hkv, d, page):
+    """Prompts of two sequences, then tokens, with an eviction whenever the cache passes its limit: every output against
+    64-bit attention over the rows that each head has kept."""
+    rng = np.random.default_rng([H, d])
+    B, budget, limit, first, last, theta = 2, 48, 64, 2, 8, 10000.0
+    pages = limit // page
+    pool = Cache(gpu, rng, [limit] * B, page, Hkv, d)
+    w = gpu.zeros(B, Hkv, limit, device="cuda")
+    kept = gpu.empty(B, Hkv, budget, device="cuda", dtype=gpu.int32)
+    assert pool.table.shape[1] == pages
+    n, pos = [0, 0], [0, 0]
+    # What each head of each sequence holds, in 64 bits.
+    k_ref = [[np.zeros((0, d)) for _ in range(Hkv)] for _ in range(B)]
+    v_ref = [[np.zeros((0, d)) for _ in range(Hkv)] for _ in range(B)]
+    for step in range(30):
+        q_len = [37, 22] if step == 0 else [1, [0, 1, 3][step % 3]]
+        n = [x + l for x, l in zip(n, q_len)]
+        q_start = np.cumsum([0] + q_len).tolist()
+        N = q_start[-1]
+        q, kn, vn = (rng.standard_normal((N, h, d)).astype(np.float32) for h in (H, Hkv, Hkv))
+        dq, dk, dv = (gpu.from_numpy(x).cuda() for x in (q, kn, vn))
+        out = gpu.empty_like(dq)
+        zt.paged_append(dq, dk, dv, dq, pool.k, pool.v, pool.table, q_start, n, pos, page, H, Hkv, d, theta, w)
+        need = zt.attn_paged_workspace_bytes(q_start, n, H, Hkv, d, True)
+        ws = gpu.empty(need + 16, device="cuda", dtype=gpu.uint8)
+        zt.attn_paged(dq, pool.k, pool.v, pool.table, out, q_start, n, page, H, Hkv, d, ws, w_in=w, w_out=w)
+        got = out.cpu().numpy()
+        for b in range(B):
+            t0, t1 = q_start[b], q_start[b + 1]
+            if t1 == t0:
+                continue
+            qr, kr = pagedref.rotate(q[t0:t1], pos[b], theta), pagedref.rotate(kn[t0:t1], pos[b], theta)
+            k1, v1 = np.zeros((n[b], Hkv, d)), np.zeros((n[b], Hkv, d))
+            for h in range(Hkv):
+                k_ref[b][h] = np.concatenate((k_ref[b][h], kr[:, h]))
+                v_ref[b][h] = np.concatenate((v_ref[b][h], vn[t0:t1, h]))
+                k1[:, h], v1[:, h] = k_ref[b][h], v_ref[b][h]
+            want, _, _, bound, _ = pagedref.attend(qr, k1, v1, np.arange(n[b])[None], [0, t1 - t0], [n[b]], 1, H, Hkv, d)
+            # q and k are rounded once to f32 here: their part of a score's error is as large as one product's rounding each.
+            assert np.all(np.abs(got[t0:t1] - want) <= 2 * bound)
+        pos = [p + l for p, l in zip(pos, q_len)]
+        if max(n) + 3 > limit:
+            weights = w.cpu().numpy()
+            zt.paged_evict(pool.k, pool.v, pool.table, pool.table, w, w, kept, n, page, Hkv, d, first, last, budget)
+            rows = kept.cpu().numpy()
+            for b in range(B):
+                for h in range(Hkv):
+                    want = pagedref.evict(weights[b, h], n[b], budget, first, last)
+                    assert np.array_equal(rows[b, h][:len(want)], want)
+                    k_ref[b][h], v_ref[b][h] = k_ref[b][h][want], v_ref[b][h][want]
+            n = [min(x, budget) for x in n]
+    assert pos[0] > limit  # it did evict

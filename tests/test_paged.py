@@ -1,0 +1,114 @@
+"""The paged cache's entry points without a GPU: every refusal comes before any device call, with its reason, and a
+workspace's size follows from the lengths alone."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import pagedref
+
+N = ctypes.c_void_p(16)  # a pointer that no refused call follows
+
+
+def ints(*xs):
+    return (ctypes.c_int * len(xs))(*xs)
+
+
+def attend(L, q_start=(0, 1, 3), n_rows=(5, 9), B=2, n_pages=8, page=4, stride=4, w_stride=9, H=4, Hkv=2, d=32, q=N, k=N,
+           v=N, table=N, out=N, lse=None, w_in=None, w_out=None, ws=N, nbytes=1 << 40):
+    return L.zt_attn_paged(q, k, v, table, out, lse, w_in, w_out, ints(*q_start) if q_start else None,
+                           ints(*n_rows) if n_rows else None, B, n_pages, page, stride, w_stride, H, Hkv, d, ws, nbytes,
+                           None)
+
+
+def append(L, q_start=(0, 1, 3), n_rows=(5, 9), pos=(4, 7), B=2, n_pages=8, page=4, stride=4, w_stride=9, H=4, Hkv=2, d=32,
+           theta=1e4, q=N, k_new=N, v_new=N, q_out=N, k=N, v=N, table=N, w=None):
+    return L.zt_paged_append(q, k_new, v_new, q_out, k, v, table, w, ints(*q_start), ints(*n_rows),
+                             ints(*pos) if pos else None, B, n_pages, page, stride, w_stride, H, Hkv, d, theta, None)
+
+
+def evict(L, n_rows=(5, 9), B=2, n_pages=8, page=4, stride=4, w_stride=9, Hkv=2, d=32, first=1, last=2, budget=4, k=N, v=N,
+          table=N, table_out=N, w_in=N, w_out=N, kept=N):
+    return L.zt_paged_evict(k, v, table, table_out, w_in, w_out, kept, ints(*n_rows), B, n_pages, page, stride, w_stride,
+                            Hkv, d, first, last, budget, None)
+
+
+GEOMETRY = [(dict(B=0), "not launchable"), (dict(n_pages=0), "not launchable"), (dict(stride=0), "not launchable"),
+            (dict(page=0), "power of two"), (dict(page=3), "power of two"), (dict(page=2048), "power of two"),
+            (dict(page=-4), "power of two"), (dict(n_pages=1 << 21, page=1024), "2^31 - 1"),
+            (dict(n_rows=(5, 17)), "outside [0, 16]"), (dict(n_rows=(-1, 9)), "outside [0, 16]"),
+            (dict(d=33), "head_dim"), (dict(d=300), "head_dim"), (dict(Hkv=0), "not a group")]
+TOKENS = [(dict(q_start=(-1, 1, 3)), "q_start"), (dict(q_start=(0, 2, 1)), "new tokens"),
+          (dict(q_start=(0, 6, 7)), "new tokens"), (dict(H=3), "not a group"), (dict(H=1 << 17), "65535")]
+
+
+@pytest.mark.parametrize("bad,reason", GEOMETRY + TOKENS + [
+    (dict(n_rows=None), "n_rows"), (dict(q_start=None), "q_start"), (dict(q=None), "null"), (dict(k=None), "null"),
+    (dict(v=None), "null"), (dict(table=None), "null"), (dict(out=None), "null"), (dict(w_in=N), "together"),
+    (dict(w_out=N), "together"), (dict(w_in=N, w_out=N, w_stride=8), "accumulated weights"),
+    (dict(w_in=N, w_out=N, nbytes=64), "short of"), (dict(w_in=N, w_out=N, ws=None), "short of"),
+    (dict(w_in=N, w_out=N, ws=ctypes.c_void_p(24)), "16-byte"), (dict(q=ctypes.c_void_p(8)), "aligned"),
+    (dict(d=34, out=ctypes.c_void_p(4)), "aligned")])
+def test_attend_refuses(zt, capfd, bad, reason):
+    assert attend(zt.lib(), **bad) == 1
+    assert reason in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("bad,reason", GEOMETRY + TOKENS + [
+    (dict(pos=None), "pos"), (dict(pos=(-1, 0)), "position"), (dict(pos=(0, 2 ** 31 - 2)), "position"),
+    (dict(theta=0.0), "theta"), (dict(theta=float("nan")), "theta"), (dict(q=None), "null"), (dict(q_out=None), "null"),
+    (dict(k_new=None), "null"), (dict(v_new=None), "null"), (dict(k=None), "null"), (dict(table=None), "null"),
+    (dict(w=N, w_stride=8), "accumulated weights"), (dict(k=ctypes.c_void_p(8)), "aligned")])
+def test_append_refuses(zt, capfd, bad, reason):
+    assert append(zt.lib(), **bad) == 1
+    assert reason in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("bad,reason", GEOMETRY + [
+    (dict(budget=0), "budget"), (dict(first=-1), "budget"), (dict(last=-1), "budget"), (dict(first=3, last=2), "budget"),
+    (dict(first=2 ** 31 - 1, last=2 ** 31 - 1), "budget"), (dict(w_stride=8), "accumulated weights"),
+    (dict(k=None), "null"), (dict(v=None), "null"), (dict(table=None), "null"), (dict(table_out=None), "null"),
+    (dict(w_in=None), "null"), (dict(w_out=None), "null"), (dict(kept=None), "null"),
+    (dict(v=ctypes.c_void_p(20)), "aligned")])
+def test_evict_refuses(zt, capfd, bad, reason):
+    assert evict(zt.lib(), **bad) == 1
+    assert reason in capfd.readouterr().err
+
+
+def test_workspace_follows_the_lengths(zt):
+    L = zt.lib()
+
+    def need(q_start, n_rows, H=32, Hkv=8, d=128, weights=0):
+        return L.zt_attn_paged_workspace(ints(*q_start), ints(*n_rows), len(n_rows), H, Hkv, d, weights)
+
+    assert need((0, 1), (16,)) == 0  # one chunk: nothing to merge
+    long = need((0, 1), (1 << 20,))
+    assert long > 0 and need((0, 1), (1 << 20,), weights=1) > long
+    assert need((0, 1), (16,), d=33) == need((0, 2), (1,)) == need((0, 1), (-1,)) == need((0, 1), (16,), H=3) == 0
+    # Chunks are of one size whatever the sequence: a batch of short sequences needs no partials.
+    assert need(tuple(range(65)), (16,) * 64) == 0
+
+
+def test_the_reference_agrees_with_a_dense_softmax():
+    """pagedref against whole-matrix products, on a contiguous table."""
+    rng = np.random.default_rng(3)
+    n, L, H, Hkv, d, page = 23, 6, 6, 2, 32, 4
+    k, v = rng.standard_normal((24, Hkv, d)), rng.standard_normal((24, Hkv, d))
+    q = rng.standard_normal((L, H, d))
+    out, lse, w, bound, w_bound = pagedref.attend(q, k, v, np.arange(6)[None], [0, L], [n], page, H, Hkv, d)
+    for h in range(H):
+        s = q[:, h] @ k[:n, h // 3].T / np.sqrt(d)
+        s[np.arange(n)[None] > np.arange(n - L, n)[:, None]] = -np.inf
+        p = np.exp(s - np.log(np.exp(s).sum(1))[:, None])
+        assert np.allclose(p @ v[:n, h // 3], out[:, h], atol=1e-13)
+        assert np.allclose(np.log(np.exp(s).sum(1)), lse[:, h], atol=1e-13)
+        w[0, h // 3] -= p.sum(0)
+    assert np.abs(w).max() < 1e-12
+    assert 0 < bound.min() and bound.max() < 1e-3 and w_bound.max() < 1e-3
+
+
+def test_the_reference_keeps_ties_by_row_and_nan_last():
+    w = np.array([9, 1, 2, np.nan, 2, 2, -np.inf, 9, 9], np.float32)
+    assert pagedref.evict(w, 9, 5, 1, 2).tolist() == [0, 2, 4, 7, 8]
+    assert pagedref.evict(w, 9, 8, 1, 2).tolist() == [0, 1, 2, 4, 5, 6, 7, 8]
+    assert pagedref.evict(w, 9, 9, 1, 2).tolist() == list(range(9))

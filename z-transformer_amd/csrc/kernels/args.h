@@ -77,6 +77,80 @@ struct DecArgs {
     float scale_log2e;
 };
 
+// Sequences of a paged cache per launch (their lengths travel in the arguments).
+#define ZT_PAGED_MAXB 64
+
+// Pages of a cache: row s of a sequence is pool row (page << shift) + (s & mask), page the entry s >> shift of
+// its page table.
+struct PagePool {
+    float *k, *v;      // [n_pages, page_size, Hkv*dim]
+    const int *table;  // [B, table_stride] page numbers (device)
+    int n_pages, shift, table_stride;
+};
+
+// Attention over a paged cache.  Per sequence i of the launch and kv head, the rows
+// are its q_len[i] new tokens' query heads of that group, token-major: row r is
+// token r / G, head r % G of the group.
+struct PagedArgs {
+    PagePool pool;
+    const float *q;     // [N, H*dim]
+    float *out;         // [N, H*dim]
+    float *lse;         // [N, H] natural log-sum-exp, or null
+    float *part_acc;    // [slots, part_ld] partial outputs (sequences split into chunks)
+    float *part_ml;     // [slots, 2] their base (log2 units) and sum
+    float *stat;        // [N, H] log-sum-exp in log2 units, or null (no weights wanted)
+    float *scores;      // scaled scores (log2 units), or null: sequence i's at score0[i], [Hkv, rows, keys padded to 16]
+    int H, Hkv, G, dim;
+    int part_ld;        // dim rounded up to whole 16 bytes
+    int chunk;          // keys per workgroup
+    int ns;             // sequences
+    float scale_log2e;
+    int b[ZT_PAGED_MAXB];       // row of the page table
+    int q0[ZT_PAGED_MAXB];      // first token
+    int q_len[ZT_PAGED_MAXB];   // new tokens
+    int n_rows[ZT_PAGED_MAXB];  // rows of the cache, the new tokens' last
+    int first[ZT_PAGED_MAXB];   // first work item of the launch
+    int nch[ZT_PAGED_MAXB];     // key chunks; 1: the output is written at once
+    long long part0[ZT_PAGED_MAXB];   // first partial: slot (kvh * rows + row) * nch + chunk behind it
+    long long score0[ZT_PAGED_MAXB];
+};
+
+// Accumulated weights from stored scores: w_out = w_in + sum over the rows of exp2(score - stat).
+struct PagedWeightArgs {
+    const float *scores, *stat;
+    const float *w_in;  // [B, Hkv, w_stride]
+    float *w_out;
+    int H, Hkv, G, w_stride, ns;
+    int b[ZT_PAGED_MAXB], q0[ZT_PAGED_MAXB], q_len[ZT_PAGED_MAXB], n_rows[ZT_PAGED_MAXB], first[ZT_PAGED_MAXB];
+    long long score0[ZT_PAGED_MAXB];
+};
+
+// Append of new tokens to a paged cache, with RoPE on q and k.
+struct PagedAppendArgs {
+    PagePool pool;
+    const float *q, *k_new, *v_new;  // [N, H*dim], [N, Hkv*dim] (q null: none)
+    float *q_out;
+    float *w;                        // [B, Hkv, w_stride] accumulated weights, or null
+    int H, Hkv, dim, w_stride, ns;
+    int tokens, token0;  // of this launch, and the first of them
+    int slices;          // parts that a token group's heads are cut into
+    double theta;
+    int b[ZT_PAGED_MAXB], q0[ZT_PAGED_MAXB], row0[ZT_PAGED_MAXB], pos[ZT_PAGED_MAXB];
+};
+
+// Eviction from a paged cache.
+struct PagedEvictArgs {
+    PagePool pool;
+    const int *table_out;
+    const float *w_in;
+    float *w_out;
+    int *kept;           // [B, Hkv, budget]
+    int Hkv, dim, w_stride, n_first, n_last, budget;
+    int b0, ns;          // sequences b0 .. b0 + ns - 1
+    int slices;          // in place: column parts of a head's row
+    int n_rows[ZT_PAGED_MAXB];
+};
+
 struct NormArgs {
     const float *x, *w;
     float *y;

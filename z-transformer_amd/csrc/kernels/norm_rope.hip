@@ -22,6 +22,7 @@
 // parallel and reproducibly.
 #include "common.h"
 #include "args.h"
+#include "paged.h"
 
 
 DEVI double wave_sum_d(double v) {
@@ -200,6 +201,63 @@ extern "C" __global__ void __launch_bounds__(256) zt_rope_append(AppendArgs a) {
         const int c = j - n_rot;
         a.vc[((size_t)b * a.n_ctx + pos) * kld + c] = a.v[(size_t)b * kld + c];
     }
+}
+
+// Append of a ragged batch's new tokens to a paged cache: q and k rotated at the tokens'
+// positions, the rotated k and v written to the tokens' rows, those rows' accumulated
+// weights cleared.  A row whose page is none of the pool's is not written.
+// A workgroup takes a group of 256 / (d / 2) tokens, so that its threads compute one
+// (token, pair) angle each (as zt_rope_forward's, in f64) before they share them, and
+// one of a.slices parts of the tokens' heads: few tokens are cut into parts for more workgroups.
+extern "C" __global__ void __launch_bounds__(256) zt_rope_paged(PagedAppendArgs a) {
+    __shared__ double tab_c[256], tab_s[256];
+    __shared__ int row_of[16], seq_of[16], at_of[16];
+    const int half = a.dim / 2, per = min(16, 256 / half);
+    const int group = (int)blockIdx.x / a.slices, slice = (int)blockIdx.x % a.slices;
+    const int t0 = a.token0 + group * per, nt = min(per, a.token0 + a.tokens - t0);
+    for (int j = threadIdx.x; j < nt * half; j += 256) {
+        const int tl = j / half, i = j - tl * half, t = t0 + tl;
+        int sq = 0;  // the last sequence that does not begin past the token
+        for (int s = 1; s < a.ns; ++s) sq = a.q0[s] <= t ? s : sq;
+        rope_angle((double)a.pos[sq] + (t - a.q0[sq]), i, a.dim, a.theta, &tab_c[j], &tab_s[j]);
+        if (i == 0) {
+            const int row = a.row0[sq] + t - a.q0[sq];
+            row_of[tl] = pool_row(a.pool, a.pool.table + (size_t)a.b[sq] * a.pool.table_stride, row);
+            seq_of[tl] = a.b[sq];
+            at_of[tl] = row;
+        }
+    }
+    __syncthreads();
+    const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
+    // A token's tasks: its rotations, q's heads (if any) then k's, and the copies of v's pairs of values.
+    const int heads = (a.q ? a.H : 0) + a.Hkv, n_rot = heads * half, tasks = n_rot + a.Hkv * half;
+    const int per_slice = (tasks + a.slices - 1) / a.slices;
+    const int j0 = slice * per_slice, nj = min(per_slice, tasks - j0);
+    for (int e = threadIdx.x; e < nt * nj; e += 256) {
+        const int tl = e / nj, j = j0 + e - tl * nj;
+        const size_t t = (size_t)(t0 + tl);
+        const int row = row_of[tl];
+        if (j < n_rot) {
+            const int h = j / half, i = j - h * half, hk = h - (heads - a.Hkv);
+            const double c = tab_c[tl * half + i], s = tab_s[tl * half + i];
+            if (hk < 0) {
+                const size_t o = t * qld + (size_t)h * a.dim + i;
+                rope_rotate<false>(c, s, a.q + o, a.q_out + o, half);
+            } else if (row >= 0) {
+                const size_t col = (size_t)hk * a.dim + i;
+                rope_rotate<false>(c, s, a.k_new + t * kld + col, a.pool.k + (size_t)row * kld + col, half);
+            }
+        } else if (row >= 0) {
+            const size_t col = 2 * (size_t)(j - n_rot);
+            *reinterpret_cast<f2 *>(a.pool.v + (size_t)row * kld + col) =
+                *reinterpret_cast<const f2 *>(a.v_new + t * kld + col);
+        }
+    }
+    if (a.w && slice == 0)
+        for (int e = threadIdx.x; e < nt * a.Hkv; e += 256) {
+            const int tl = e / a.Hkv, hk = e - tl * a.Hkv;
+            a.w[((size_t)seq_of[tl] * a.Hkv + hk) * a.w_stride + at_of[tl]] = 0.f;
+        }
 }
 
 DEVI unsigned long long splitmix64(unsigned long long seed, unsigned long long ctr) {

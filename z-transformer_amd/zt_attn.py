@@ -27,6 +27,7 @@ ABI_SYMBOLS = [
     "zt_matmul", "zt_weight_grad", "zt_input_grad", "zt_attn_backward_train_workspace",
     "zt_attn_backward_train_ws", "zt_attn_forward_train_ws", "zt_attn_set_tuning", "zt_attn_get_tuning",
     "zt_calibrate_launch", "zt_attn_decode_noalloc", "zt_matmul_plan", "zt_product_plan",
+    "zt_attn_paged_workspace", "zt_attn_paged", "zt_paged_append", "zt_paged_evict",
 ]
 HOLDER_SYMBOLS = [
     "zt_bytes_for", "zt_to_cint", "zt_forward_bounds", "zt_holder_init", "zt_holder_deinit",
@@ -93,6 +94,10 @@ def load_library(path):
         "zt_input_grad": (I, [P, P, P, I, I, I, P]),
         "zt_matmul_plan": (I, [I, I, I, P, I]),
         "zt_product_plan": (I, [I, I, I, I, P, I]),
+        "zt_attn_paged_workspace": (Z, [P, P] + [I] * 5),
+        "zt_attn_paged": (I, [P] * 10 + [I] * 8 + [P, Z, P]),
+        "zt_paged_append": (I, [P] * 11 + [I] * 8 + [D, P]),
+        "zt_paged_evict": (I, [P] * 8 + [I] * 10 + [P]),
         "zt_calibrate": (I, [P, Z, P, Z, P, P, P]),
         "zt_calibrate_launch": (I, [ctypes.c_uint, ctypes.c_uint, I, P, P]),
         "zt_rope_forward": (I, [P, P, I, I, I, D, I, P]),
@@ -288,6 +293,69 @@ def decode_step(q, k_new, v_new, k_cache, v_cache, out, pos, B, n_ctx, n_heads, 
                                    B, n_ctx, n_heads, n_kv_heads, dim, theta, _ptr(workspace), nbytes,
                                    _stream(stream))
     _check(rc, "zt_attn_decode_step")
+
+
+def _i32_cuda(*ts):
+    import torch
+    for t in ts:
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise ValueError("page tables and row numbers must be contiguous int32 on the GPU")
+
+
+def _host_ints(xs, n):
+    if len(xs) != n:
+        raise ValueError(f"{len(xs)} lengths where {n} are needed")
+    return (ctypes.c_int * n)(*[int(x) for x in xs])
+
+
+def paged_append(q, k_new, v_new, q_out, k_pages, v_pages, table, q_start, n_rows, pos, page_size, n_heads, n_kv_heads,
+                 dim, theta=500000.0, w=None, stream=None):
+    """q_start (B + 1), n_rows, pos (B): host sequences; table [B, pages]; w [B, n_kv_heads, rows] or None.
+    q and q_out may both be None."""
+    _f32_cuda(k_new, v_new, k_pages, v_pages, *[t for t in (q, q_out, w) if t is not None])
+    _i32_cuda(table)
+    B, table_stride = table.shape
+    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    _check(lib().zt_paged_append(*map(_ptr, (q, k_new, v_new, q_out, k_pages, v_pages, table, w)),
+                                 _host_ints(q_start, B + 1), _host_ints(n_rows, B), _host_ints(pos, B), B, n_pages,
+                                 page_size, table_stride, 0 if w is None else w.shape[-1], n_heads, n_kv_heads, dim,
+                                 theta, _stream(stream)), "zt_paged_append")
+
+
+def attn_paged_workspace_bytes(q_start, n_rows, n_heads, n_kv_heads, dim, weights=False):
+    B = len(n_rows)
+    return lib().zt_attn_paged_workspace(_host_ints(q_start, B + 1), _host_ints(n_rows, B), B, n_heads, n_kv_heads,
+                                         dim, int(weights))
+
+
+def attn_paged(q, k_pages, v_pages, table, out, q_start, n_rows, page_size, n_heads, n_kv_heads, dim, workspace,
+               lse=None, w_in=None, w_out=None, stream=None):
+    """workspace: a tensor of attn_paged_workspace_bytes(...) bytes, or None where that is 0."""
+    _f32_cuda(q, k_pages, v_pages, out, *[t for t in (lse, w_in, w_out) if t is not None])
+    _i32_cuda(table)
+    if w_in is not None and w_out is not None and w_in.shape != w_out.shape:
+        raise ValueError("w_in and w_out have the same shape")
+    B, table_stride = table.shape
+    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().zt_attn_paged(*map(_ptr, (q, k_pages, v_pages, table, out, lse, w_in, w_out)),
+                               _host_ints(q_start, B + 1), _host_ints(n_rows, B), B, n_pages, page_size, table_stride,
+                               0 if w_out is None else w_out.shape[-1], n_heads, n_kv_heads, dim, _ptr(workspace),
+                               nbytes, _stream(stream)), "zt_attn_paged")
+
+
+def paged_evict(k_pages, v_pages, table, table_out, w_in, w_out, kept, n_rows, page_size, n_kv_heads, dim, n_first,
+                n_last, budget, stream=None):
+    """kept [B, n_kv_heads, budget] int32; table_out is table (in place) or a table of other pages."""
+    _f32_cuda(k_pages, v_pages, w_in, w_out)
+    _i32_cuda(table, table_out, kept)
+    B, table_stride = table.shape
+    if table_out.shape != table.shape or w_in.shape != w_out.shape or kept.numel() != B * n_kv_heads * budget:
+        raise ValueError("table and table_out, and w_in and w_out, have one shape; kept is [B, n_kv_heads, budget]")
+    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    _check(lib().zt_paged_evict(*map(_ptr, (k_pages, v_pages, table, table_out, w_in, w_out, kept)),
+                                _host_ints(n_rows, B), B, n_pages, page_size, table_stride, w_in.shape[-1], n_kv_heads,
+                                dim, n_first, n_last, budget, _stream(stream)), "zt_paged_evict")
 
 
 def rmsnorm(x, w, y, rows, cols, eps=1e-5, stream=None):
