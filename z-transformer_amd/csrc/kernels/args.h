@@ -98,7 +98,7 @@ struct PagedArgs {
     float *lse;         // [N, H] natural log-sum-exp, or null
     float *part_acc;    // [slots, part_ld] partial outputs (sequences split into chunks)
     float *part_ml;     // [slots, 2] their base (log2 units) and sum
-    float *stat;        // [N, H] log-sum-exp in log2 units, or null (no weights wanted)
+    float *stat;        // [N, H, 2] base m of each row and 1 / sum exp2(score - m), or null (no weights wanted)
     float *scores;      // scaled scores (log2 units), or null: sequence i's at score0[i], [Hkv, rows, keys padded to 16]
     int H, Hkv, G, dim;
     int part_ld;        // dim rounded up to whole 16 bytes
@@ -115,12 +115,17 @@ struct PagedArgs {
     long long score0[ZT_PAGED_MAXB];
 };
 
-// Accumulated weights from stored scores: w_out = w_in + sum over the rows of exp2(score - stat).
+// Accumulated weights: w_out = w_in + sum over the rows of exp2(score - m) / sum, from stored
+// scores (zt_paged_weights), or from q and k again, in parts of the rows (zt_paged_wparts_*) that zt_paged_wsum adds.
 struct PagedWeightArgs {
-    const float *scores, *stat;
+    PagePool pool;
+    const float *q, *scores, *stat;
     const float *w_in;  // [B, Hkv, w_stride]
     float *w_out;
-    int H, Hkv, G, w_stride, ns;
+    float *parts;       // sequence i's at score0[i]: [Hkv, parts, keys padded to 16]
+    int H, Hkv, G, dim, w_stride, ns;
+    int part_rows;      // rows of a part
+    float scale_log2e;
     int b[ZT_PAGED_MAXB], q0[ZT_PAGED_MAXB], q_len[ZT_PAGED_MAXB], n_rows[ZT_PAGED_MAXB], first[ZT_PAGED_MAXB];
     long long score0[ZT_PAGED_MAXB];
 };

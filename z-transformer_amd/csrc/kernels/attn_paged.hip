@@ -14,6 +14,7 @@
 #include "common.h"
 #include "args.h"
 #include "paged.h"
+#include "split.h"
 
 // N consecutive floats (2 or 4) of a row at column c; FULL: the row has DP aligned
 // columns; else columns past dim are 0 and rows may be 8-byte aligned only.
@@ -40,6 +41,12 @@ DEVI void load_cols(float *dst, const float *row, int c, int dim, bool vec4) {
         if (FULL || c < dim) x = __builtin_nontemporal_load(reinterpret_cast<const f2 *>(row + c));
         dst[0] = x.x; dst[1] = x.y;
     }
+}
+
+// A row's statistics: log-sum-exp in natural units, base and inverse sum for its weights.
+DEVI void put_stats(const PagedArgs &a, size_t row, float m, float l) {
+    if (a.lse) a.lse[row] = (m + log2f(l)) * 0.69314718055994531f;
+    if (a.stat) *reinterpret_cast<f2 *>(a.stat + 2 * row) = f2{m, 1.f / l};
 }
 
 // ---- Few rows: K and V stream through registers -----------------------------------
@@ -265,9 +272,7 @@ DEVI void paged_few(const PagedArgs &a) {
             const size_t row = (size_t)(a.q0[sq] + t);
             if (nch == 1) {
                 if (col == 0) {
-                    const float l2 = M + log2f(L);
-                    if (a.lse) a.lse[row * a.H + h] = l2 * 0.69314718055994531f;
-                    if (a.stat) a.stat[row * a.H + h] = l2;
+                    put_stats(a, row * a.H + h, M, L);
                 }
                 store4(a.out + row * qld + (size_t)h * a.dim, col, a.dim, vec4, A * (1.f / L));
             } else {
@@ -275,6 +280,426 @@ DEVI void paged_few(const PagedArgs &a) {
                 *reinterpret_cast<f4 *>(a.part_acc + slot * a.part_ld + col) = A;
                 if (col == 0) { a.part_ml[2 * slot] = M; a.part_ml[2 * slot + 1] = L; }
             }
+        }
+    }
+}
+
+// ---- Many rows: split operands -------------------------------------------------------
+//
+// The products on the bf16 matrix cores from three exact parts per operand (split.h).  A
+// workgroup takes one (sequence, kv head, chunk of keys, tile of 16 NQ NW rows); a wave holds 16 NQ of the
+// rows (Q's parts, O and the softmax state in registers), and the 32-key tiles of K and V pass through LDS,
+// split once for all waves: two buffers of each, and the second half of the waves runs half a step behind the
+// first, so that one half's softmax and splitting run beside the other's products.
+//   A step is phase A (S^T = K Q^T, softmax; the next K tile into LDS) and phase B (O^T += V^T P^T; the
+//   next V tile); tiles are loaded a whole step before they are written to LDS where registers allow (DEEP), else in that phase.
+//   * The pool rows that a thread stages are looked up in the page table one tile ahead of its loads.
+//   * The rows of V hold a value that is big (split.h), or that is not finite where a pair of the tile is
+//     hidden, as 0 in the split, and it is added from the full row to the rows that see it.
+//   * A key whose page is none of the pool's is staged as NaN: the scores it meets are NaN.
+template <int DP, int NW, int NQ>
+struct PagedMany {
+    static constexpr int NT = DP / 16, NKS = DP / 32, NTH = 64 * NW;
+    static constexpr int TILE = split_bytes(DP, 32);
+    static constexpr bool ALT = NW == 8 && 4 * TILE + 16 <= 160 * 1024;
+    static constexpr bool DEEP = NQ == 1 || DP <= 64;
+    static constexpr int FLAGS = (ALT ? 4 : 2) * TILE;
+    static constexpr int BYTES = FLAGS + 16;
+};
+
+template <int DP, int NW, int NQ, bool FULL>
+DEVI void paged_many(const PagedArgs &a) {
+    using P = PagedMany<DP, NW, NQ>;
+    constexpr int NT = P::NT, NKS = P::NKS, NTH = P::NTH;
+    constexpr bool ALT = P::ALT, DEEP = P::DEEP;
+    __shared__ __attribute__((aligned(16))) char smem[P::BYTES];
+    // The K (V) tile of step id, and the flag that holds id if V's tile has values to add.
+    auto ktile = [&](int id) { return smem + (ALT ? (id & 1) * 2 * P::TILE : 0); };
+    auto vtile = [&](int id) { return ktile(id) + P::TILE; };
+    int *const flags = reinterpret_cast<int *>(smem + P::FLAGS);
+    auto kflag = [&](int id) { return flags + (ALT ? (id & 1) * 2 : 0); };
+    auto vflag = [&](int id) { return kflag(id) + 1; };
+
+    const int tid = opaque((int)threadIdx.x), lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sq = paged_seq(a, blockIdx.x);
+    const int nch = a.nch[sq], q_len = a.q_len[sq], rows = q_len * a.G;
+    int item = (int)blockIdx.x - a.first[sq];
+    const int kvh = item % a.Hkv;
+    item /= a.Hkv;
+    const int c = item % nch;
+    constexpr int RT = 16 * NQ * NW;  // rows of a workgroup; the last tile, with most keys, first
+    const int wg_row0 = ((rows + RT - 1) / RT - 1 - item / nch) * RT, row0 = wg_row0 + 16 * NQ * w;
+    const int seen0 = a.n_rows[sq] - q_len;
+    const int kend_wg = seen0 + (min(rows, wg_row0 + RT) - 1) / a.G + 1;
+    const int kend_w = row0 < rows ? seen0 + (min(rows, row0 + 16 * NQ) - 1) / a.G + 1 : 0;
+    const int key0 = c * a.chunk, key1 = min(kend_wg, key0 + a.chunk);
+    if (key0 >= kend_wg) return;  // workgroup-uniform
+    const int edge0 = seen0 + wg_row0 / a.G;  // the workgroup's first row sees keys up to this one
+    const int *table = a.pool.table + (size_t)a.b[sq] * a.pool.table_stride;
+    const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
+    const float *kb = a.pool.k + (size_t)kvh * a.dim, *vb = a.pool.v + (size_t)kvh * a.dim;
+    const bool vec4 = (a.dim & 3) == 0;
+    if (tid < 4) flags[tid] = -1;
+
+    // Staging: thread tid takes the 8-column chunks e = tid + n NTH of a 32-key tile.
+    constexpr int CPR = DP / 8, CH = 32 * CPR, NP = (CH + NTH - 1) / NTH;
+    constexpr bool EVEN = CH % NTH == 0;
+    auto rows_of = [&](int (&r)[NP], int id) {  // pool rows of the chunks of step id; past the last key, that one's
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            r[n] = pool_row(a.pool, table, min(key0 + 32 * id + (tid + n * NTH) / CPR % 32, key1 - 1));
+    };
+    auto fetch = [&](float (&x)[NP][8], const float *base, const int (&r)[NP]) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int e = tid + n * NTH;
+            if (!EVEN && e >= CH) break;  // wave-uniform: CH is a multiple of 64
+            const float *p = base + (size_t)max(r[n], 0) * kld;
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                load_cols<4, FULL>(y, p, e % CPR * 8 + i, a.dim, vec4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[n][i + k] = y[k];
+            }
+        }
+    };
+    auto put = [&](const float (&x)[NP][8], char *t, int *flag, int id, bool odd_too, auto split) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int e = tid + n * NTH;
+            if (!EVEN && e >= CH) break;
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[n][i];
+            bool take = any_big(max_abs(y));
+            if (odd_too) {
+                bool nan = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) nan |= y[i] != y[i];
+                take |= __builtin_amdgcn_ballot_w64(nan) != 0;
+            }
+            if (take) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = odd_too && y[i] != y[i] ? 0.f : small_part(y[i]);
+                if (lane == 0) *flag = id;
+            }
+            put_tri<DP>(t, 32, e / CPR, e % CPR * 8, split(y));
+        }
+    };
+
+    // Q: the B operand of the score product, lane l16 = row, k slot = column.  Rows past the last take its values.
+    Tri q[NKS][NQ];
+    int last[NQ];
+    float qmax = 0.f;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = min(row0 + 16 * n + l16, rows - 1), t = r / a.G;
+        last[n] = seen0 + t;
+        const float *row = a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                float z[4];
+                load_cols<4, FULL>(z, row, 32 * ks + 8 * grp + i, a.dim, vec4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[i + k] = z[k] * a.scale_log2e;
+            }
+            const float mx = max_abs(y);
+            qmax = vmax(qmax, mx);
+            if (any_big(mx)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = small_part(y[i]);
+            }
+            q[ks][n] = split8_as_is(y);
+        }
+    }
+    const bool qbig = any_big(qmax);
+    f4 o[NT][NQ];
+    float m[NQ], lsum[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[i][n] = zero4();
+        m[n] = -INFINITY;
+        lsum[n] = 0.f;
+    }
+
+    f4 s[2 * NQ];  // s[j NQ + n]: keys k0 + 16 j + 4 grp + r of row block n
+    auto softmax = [&](const int k0) {
+        if (k0 + 31 > seen0 + row0 / a.G || k0 + 32 > key1) {  // wave-uniform
+#pragma unroll
+            for (int i = 0; i < 2 * NQ; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = k0 + 16 * (i / NQ) + 4 * grp + r;
+                    if (key > last[i % NQ] || key >= key1) s[i][r] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = s[(i / 4) * NQ + n][i % 4];
+            const float mt = max4grp(vmax_n(y));
+            if (mt > m[n] + 8.f) {  // the base is raised only when a score passes it by 2^8
+                const float mnew = vmax(m[n], mt), corr = fast_exp2(m[n] - mnew);
+                m[n] = mnew;
+                lsum[n] *= corr;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) o[i][n] *= corr;
+            }
+            const float mb = m[n] == -INFINITY ? 0.f : m[n];  // nothing seen yet
+            float ps = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = fast_exp2(y[i] - mb);
+                s[(i / 4) * NQ + n][i % 4] = y[i];
+                ps = i == 0 ? y[0] : ps + y[i];
+            }
+            lsum[n] += ps;
+        }
+    };
+
+    const int nsteps = (key1 - key0 + 31) >> 5;
+    float px[NP][8], py[DEEP ? NP : 1][8];
+    int rk[NP], rv[NP], rn[NP];  // pool rows of the next K fetch, of the next V fetch, and of the tile after
+    const auto as_is = [](const float (&y)[8]) { return split8_as_is(y); };
+    const auto scaled = [](const float (&y)[8]) { return split8(y); };
+    auto copy_rows = [](int (&to)[NP], const int (&from)[NP]) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) to[n] = from[n];
+    };
+    bool none[NP];  // of the K tile in px: its page is none of the pool's
+    auto fetch_k = [&](int id) {  // then the rows of the tile after it
+        copy_rows(rk, rn);
+        fetch(px, kb, rk);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) none[n] = rk[n] < 0;
+        rows_of(rn, min(id + 1, nsteps - 1));
+    };
+    auto stage_k = [&](int id) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            if (none[n]) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) px[n][i] = __builtin_nanf("");
+            }
+        put(px, ktile(id), kflag(id), id, false, as_is);
+    };
+    auto fetch_v = [&](int id) {
+        if constexpr (DEEP) fetch(py, vb, rv);
+        else fetch(px, vb, rv);
+    };
+    auto stage_v = [&](int id) {
+        const bool edge = key0 + 32 * id + 31 > edge0 || key0 + 32 * id + 32 > key1;
+        if constexpr (DEEP) put(py, vtile(id), vflag(id), id, edge, scaled);
+        else put(px, vtile(id), vflag(id), id, edge, scaled);
+    };
+    // Rows: K of tile i is fetched before V of tile i, which takes the rows that K's fetch used.
+    __syncthreads();  // the flags
+    rows_of(rn, 0);
+    fetch_k(0);
+    copy_rows(rv, rk);
+    stage_k(0);
+    fetch_v(0);
+    if constexpr (ALT) {
+        stage_v(0);
+        if constexpr (DEEP) {
+            fetch_k(min(1, nsteps - 1));
+            copy_rows(rv, rk);
+            fetch_v(min(1, nsteps - 1));
+        }
+    } else if constexpr (DEEP) {
+        fetch_k(min(1, nsteps - 1));
+    }
+    __syncthreads();
+    // Half a step behind: the second half's waves meet one barrier more here, the first half's one more at the end.
+    if (ALT && w >= NW / 2) __syncthreads();
+    for (int id = 0; id < nsteps; ++id) {
+        const int k0 = key0 + 32 * id;
+        const int n1 = min(id + 1, nsteps - 1), n2 = min(id + 2, nsteps - 1);  // (the last loads itself again, unused)
+        const bool active = k0 < kend_w;  // wave-uniform
+        const char *const Ks = ktile(id), *const Vs = vtile(id);
+        // Phase A: scores and weights; the next K (without ALT: this V) into LDS.
+        if constexpr (!DEEP) {
+            if constexpr (ALT) {
+                fetch_k(n1);
+                copy_rows(rv, rk);
+            } else {
+                fetch_v(id);
+            }
+        }
+        if (active) {
+#pragma unroll
+            for (int i = 0; i < 2 * NQ; ++i) s[i] = zero4();
+            stream_parts<2 * NKS, 3>(
+                [&](int i, int part) {
+                    return get_row<DP>(Ks, 32, 16 * (i / NKS), 32 * (i % NKS), l16, grp, part);
+                },
+                [&](int i, auto part, u4 x) {
+                    f4 t[NQ];
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) t[n] = s[(i / NKS) * NQ + n];
+                    mfma_parts<part>(t, x, [&](int n) -> const Tri & { return q[i % NKS][n]; });
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) s[(i / NKS) * NQ + n] = t[n];
+                });
+            const bool kbig = __builtin_amdgcn_readfirstlane(*kflag(id)) == id;
+            if (kbig || qbig) {
+                // Products with a big operand, from the full values; of both sides, the whole product in f32.
+                if (kbig && qbig) {
+#pragma unroll
+                    for (int i = 0; i < 2 * NQ; ++i) s[i] = zero4();
+                }
+                const int ll = opaque(lane), lrow = ll & 15, lgrp = ll >> 4;
+                const float *krow[2], *qrow[NQ];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int r = pool_row(a.pool, table, min(k0 + 16 * j + lrow, key1 - 1));
+                    krow[j] = kb + (size_t)max(r, 0) * kld;
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const int r = min(row0 + 16 * n + lrow, rows - 1), t = r / a.G;
+                    qrow[n] = a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+                }
+#pragma unroll 1
+                for (int cc = 0; cc < 8 * NKS; ++cc) {
+                    const int col = 32 * (cc >> 3) + 8 * lgrp + (cc & 7);
+                    float kv[2], qv[NQ];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        kv[j] = col < a.dim ? krow[j][col] : 0.f;
+                        if (!qbig) kv[j] = big_part(kv[j]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        qv[n] = col < a.dim ? qrow[n][col] * a.scale_log2e : 0.f;
+                        if (!kbig) qv[n] = big_part(qv[n]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2 * NQ; ++i) s[i] = mfma16(kv[i / NQ], qv[i % NQ], s[i]);
+                }
+            }
+            softmax(k0);
+        }
+        if constexpr (ALT) {
+            stage_k(id + 1);
+            if constexpr (DEEP) fetch_k(n2);
+        } else {
+            stage_v(id);
+            if constexpr (DEEP) {
+                copy_rows(rv, rk);
+                fetch_v(n1);
+            }
+        }
+        __syncthreads();
+
+        // Phase B: the output product; the next V (without ALT: K) into LDS.
+        if constexpr (!DEEP) {
+            if constexpr (ALT) {
+                fetch_v(n1);
+            } else {
+                fetch_k(n1);
+                copy_rows(rv, rk);
+            }
+        }
+        if (active) {
+            Tri p[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = s[(i / 4) * NQ + n][i % 4];
+                p[n] = split8_as_is(y);
+            }
+            f4 t[NQ];
+            stream_parts<NT, 3>(
+                [&](int i, int part) { return get_col<DP>(Vs, 32, 0, 16 * i, lane, part); },
+                [&](int i, auto part, u4 x) {
+                    if constexpr (part == 0) {
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) t[n] = zero4();
+                    }
+                    mfma_parts<part>(t, x, [&](int n) -> const Tri & { return p[n]; });
+                    if constexpr (part == 2) {
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) o[i][n] += t[n] * kUnscale1;
+                    }
+                });
+            if (__builtin_amdgcn_readfirstlane(*vflag(id)) == id) {
+                // V's big and odd values, from the full rows, to the rows that see them.
+                const int ll = opaque(lane), lrow = ll & 15, lgrp = ll >> 4;
+                const bool edge = k0 + 31 > edge0 || k0 + 32 > key1;
+#pragma unroll 1
+                for (int key = 0; key < 32; ++key) {
+                    if (k0 + key >= key1) break;
+                    const int r = pool_row(a.pool, table, k0 + key);
+                    const float *vr = vb + (size_t)max(r, 0) * kld;
+                    const int slot = 4 * (key >> 4) + (key & 3);  // of the lane group (key >> 2) & 3
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        unsigned ph = p[n].h.x, pm = p[n].m.x, pl = p[n].l.x;
+#pragma unroll
+                        for (int e = 1; e < 4; ++e) {
+                            ph = slot >> 1 == e ? p[n].h[e] : ph;
+                            pm = slot >> 1 == e ? p[n].m[e] : pm;
+                            pl = slot >> 1 == e ? p[n].l[e] : pl;
+                        }
+                        const float pk = __shfl(join_bf16(ph, pm, pl, slot & 1), 16 * ((key >> 2) & 3) + lrow, 64);
+                        const bool sees = k0 + key <= last[n];
+#pragma unroll
+                        for (int i = 0; i < NT; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int col = 16 * i + 4 * lgrp + k;
+                                if (!sees || col >= a.dim) continue;
+                                const float x = vr[col];
+                                if (__builtin_fabsf(x) >= kBig || (edge && x != x)) o[i][n][k] += pk * x;
+                            }
+                    }
+                }
+            }
+        }
+        if constexpr (ALT) {
+            stage_v(id + 1);
+            if constexpr (DEEP) {
+                copy_rows(rv, rk);
+                fetch_v(n2);
+            }
+        } else {
+            stage_k(id + 1);
+            if constexpr (DEEP) fetch_k(n2);
+        }
+        __syncthreads();
+    }
+    if (ALT && w < NW / 2) __syncthreads();
+
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int el = opaque(lane), egrp = el >> 4;
+        const int r = row0 + 16 * n + (el & 15);
+        const float l = sum4grp(lsum[n]);
+        if (r >= rows) continue;
+        const int t = r / a.G, h = kvh * a.G + r - t * a.G;
+        const size_t row = (size_t)(a.q0[sq] + t);
+        if (nch == 1) {
+            const float inv = 1.f / l;
+            if (egrp == 0) put_stats(a, row * a.H + h, m[n], l);
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                store4(a.out + row * qld + (size_t)h * a.dim, 16 * i + 4 * egrp, a.dim, vec4, o[i][n] * inv);
+        } else {
+            const size_t slot = (size_t)a.part0[sq] + ((size_t)kvh * rows + r) * nch + c;
+            if (egrp == 0) { a.part_ml[2 * slot] = m[n]; a.part_ml[2 * slot + 1] = l; }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                if (16 * i + 4 * egrp < a.dim)
+                    *reinterpret_cast<f4 *>(a.part_acc + slot * a.part_ld + 16 * i + 4 * egrp) = o[i][n];
         }
     }
 }
@@ -344,17 +769,16 @@ DEVI void paged_merge(const PagedArgs &a) {
     if (g != 0 || !ok) return;
     const size_t row = (size_t)(a.q0[sq] + t);
     if (col == 0) {
-        const float l2 = M + log2f(L);
-        if (a.lse) a.lse[row * a.H + h] = l2 * 0.69314718055994531f;
-        if (a.stat) a.stat[row * a.H + h] = l2;
+        put_stats(a, row * a.H + h, M, L);
     }
     store4(a.out + row * a.H * a.dim + (size_t)h * a.dim, col, a.dim, (a.dim & 3) == 0, A * (1.f / L));
 }
 
-// ---- Accumulated weights from stored scores ------------------------------------------
+// ---- Accumulated weights ---------------------------------------------------------------
 //
-// A thread takes four keys of one (sequence, kv head) and adds the weights of all rows,
-// rows in order.  Sequences without new tokens copy their weights.
+// Few rows: from the scores that the attention stored.  A thread takes four keys of one
+// (sequence, kv head) and adds the weights of all rows, rows in order.  Sequences without
+// new tokens copy their weights.
 extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightArgs a) {
     const int sq = paged_seq(a, blockIdx.x);
     const int n = a.n_rows[sq], kpad = (n + 15) & ~15, rows = a.q_len[sq] * a.G;
@@ -363,16 +787,16 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
     const int kvh = item / per_head, key = (item % per_head) * 1024 + 4 * (int)threadIdx.x;
     if (key >= n) return;
     const float *sp = a.scores + a.score0[sq] + (size_t)kvh * rows * kpad + key;
-    const float *st = a.stat + (size_t)a.q0[sq] * a.H + kvh * a.G;
+    const float *st = a.stat + 2 * ((size_t)a.q0[sq] * a.H + kvh * a.G);
     const int seen0 = n - a.q_len[sq];
     f4 sum = zero4();
     int t = 0, g = 0;
     for (int r = 0; r < rows; ++r) {
         if (key <= seen0 + t) {  // else none of the four keys is seen (and the score may not be written)
             const f4 s = *reinterpret_cast<const f4 *>(sp + (size_t)r * kpad);
-            const float l2 = st[(size_t)t * a.H + g];
+            const f2 ml = *reinterpret_cast<const f2 *>(st + 2 * ((size_t)t * a.H + g));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += key + e <= seen0 + t ? fast_exp2(s[e] - l2) : 0.f;
+            for (int e = 0; e < 4; ++e) sum[e] += key + e <= seen0 + t ? fast_exp2(s[e] - ml.x) * ml.y : 0.f;
         }
         if (++g == a.G) { g = 0; ++t; }
     }
@@ -382,12 +806,233 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
         if (key + e < n) a.w_out[at + e] = a.w_in[at + e] + sum[e];
 }
 
+// Many rows: the scores again, on split operands.  A workgroup takes one (sequence, kv
+// head, tile of 16 NK NW keys, part of the rows); a wave holds 16 NK keys (K's parts in registers), and Q
+// passes through LDS in 32-row tiles, split once for all waves, two buffers, beside the rows'
+// statistics.  S = Q K^T has a key per lane and four rows, so that the sum over rows
+// stays in the lane until the end.
+template <int DP, int NW, int NK, bool FULL>
+DEVI void paged_wparts(const PagedWeightArgs &a) {
+    constexpr int NKS = DP / 32, NTH = 64 * NW, TILE = split_bytes(DP, 32), KT = 16 * NK * NW;
+    __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+    __shared__ __attribute__((aligned(16))) float row_m[2][32], row_inv[2][32];
+    __shared__ __attribute__((aligned(16))) int row_last[2][32];
+    __shared__ int flags[2];
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sq = paged_seq(a, blockIdx.x);
+    const int n = a.n_rows[sq], q_len = a.q_len[sq], rows = q_len * a.G, seen0 = n - q_len;
+    const int nparts = (rows + a.part_rows - 1) / a.part_rows;
+    int item = (int)blockIdx.x - a.first[sq];
+    const int kvh = item % a.Hkv;
+    item /= a.Hkv;
+    const int part = item % nparts, kt0 = item / nparts * KT;
+    // Rows of the part that see the tile's first key.
+    const int r0 = max(part * a.part_rows, max(0, kt0 - seen0) * a.G) & ~31, r1 = min(rows, (part + 1) * a.part_rows);
+    if (r0 >= r1) return;  // workgroup-uniform; zt_paged_wsum does not read it
+    const int *table = a.pool.table + (size_t)a.b[sq] * a.pool.table_stride;
+    const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
+    const float *kb = a.pool.k + (size_t)kvh * a.dim;
+    const bool vec4 = (a.dim & 3) == 0;
+    if (tid < 2) flags[tid] = -1;
+
+    const int k0 = kt0 + 16 * NK * w;  // the wave's first key
+    Tri k[NKS][NK];
+    float acc[NK], kmax = 0.f;
+    const float *krow[NK];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+        acc[i] = 0.f;
+        const int r = pool_row(a.pool, table, min(k0 + 16 * i + l16, n - 1));
+        krow[i] = kb + (size_t)max(r, 0) * kld;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            float y[8];
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                float z[4];
+                load_cols<4, FULL>(z, krow[i], 32 * ks + 8 * grp + h, a.dim, vec4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[h + e] = r < 0 ? __builtin_nanf("") : z[e];
+            }
+            const float mx = max_abs(y);
+            kmax = vmax(kmax, mx);
+            if (any_big(mx)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = small_part(y[e]);
+            }
+            k[ks][i] = split8_as_is(y);
+        }
+    }
+    const bool kbig = any_big(kmax);
+
+    constexpr int CPR = DP / 8, CH = 32 * CPR, NP = (CH + NTH - 1) / NTH;
+    constexpr bool EVEN = CH % NTH == 0;
+    auto q_row = [&](int r) {  // of row r, or the part's last
+        r = min(r, r1 - 1);
+        const int t = r / a.G;
+        return a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+    };
+    float px[NP][8], sm = 0.f, si = 0.f;
+    int sl = 0;
+    auto fetch = [&](int rt) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int e = tid + i * NTH;
+            if (!EVEN && e >= CH) break;  // wave-uniform
+            const float *p = q_row(rt + e / CPR);
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                float z[4];
+                load_cols<4, FULL>(z, p, e % CPR * 8 + h, a.dim, vec4);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) px[i][h + x] = z[x] * a.scale_log2e;
+            }
+        }
+        if (tid < 32) {
+            const int r = min(rt + tid, r1 - 1), t = r / a.G;
+            const f2 ml = *reinterpret_cast<const f2 *>(a.stat + 2 * ((size_t)(a.q0[sq] + t) * a.H + kvh * a.G + r - t * a.G));
+            sm = ml.x;
+            si = ml.y;
+            sl = rt + tid < r1 ? seen0 + t : -1;  // a row past the part's last sees nothing
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int e = tid + i * NTH;
+            if (!EVEN && e >= CH) break;
+            float y[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) y[x] = px[i][x];
+            if (any_big(max_abs(y))) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) y[x] = small_part(y[x]);
+                if (lane == 0) flags[buf & 1] = buf;
+            }
+            put_tri<DP>(smem + (buf & 1) * TILE, 32, e / CPR, e % CPR * 8, split8_as_is(y));
+        }
+        if (tid < 32) {
+            row_m[buf & 1][tid] = sm;
+            row_inv[buf & 1][tid] = si;
+            row_last[buf & 1][tid] = sl;
+        }
+    };
+    const int nsteps = (r1 - r0 + 31) >> 5;
+    fetch(r0);
+    __syncthreads();  // the flags
+    put(0);
+    if (nsteps > 1) fetch(r0 + 32);
+    __syncthreads();
+    for (int id = 0; id < nsteps; ++id) {
+        const char *const Qs = smem + (id & 1) * TILE;
+        const int rt = r0 + 32 * id;
+        f4 s[2 * NK];  // s[j NK + i]: rows rt + 16 j + 4 grp + x, key k0 + 16 i + l16
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i) s[i] = zero4();
+        stream_parts<2 * NKS, 3>(
+            [&](int i, int p) { return get_row<DP>(Qs, 32, 16 * (i / NKS), 32 * (i % NKS), l16, grp, p); },
+            [&](int i, auto p, u4 x) {
+                f4 t[NK];
+#pragma unroll
+                for (int j = 0; j < NK; ++j) t[j] = s[(i / NKS) * NK + j];
+                mfma_parts<p>(t, x, [&](int j) -> const Tri & { return k[i % NKS][j]; });
+#pragma unroll
+                for (int j = 0; j < NK; ++j) s[(i / NKS) * NK + j] = t[j];
+            });
+        const bool qbig = __builtin_amdgcn_readfirstlane(flags[id & 1]) == id;
+        if (kbig || qbig) {  // products with a big operand, from the full values; of both sides, all in f32
+            if (kbig && qbig) {
+#pragma unroll
+                for (int i = 0; i < 2 * NK; ++i) s[i] = zero4();
+            }
+            const int ll = opaque(lane), lrow = ll & 15, lgrp = ll >> 4;
+            const float *qrow[2] = {q_row(rt + lrow), q_row(rt + 16 + lrow)};
+#pragma unroll 1
+            for (int cc = 0; cc < 8 * NKS; ++cc) {
+                const int col = 32 * (cc >> 3) + 8 * lgrp + (cc & 7);
+                float kv[NK], qv[2];
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    kv[i] = col < a.dim ? krow[i][col] : 0.f;
+                    if (!qbig) kv[i] = big_part(kv[i]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    qv[j] = col < a.dim ? qrow[j][col] * a.scale_log2e : 0.f;
+                    if (!kbig) qv[j] = big_part(qv[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * NK; ++i) s[i] = mfma16(qv[i / NK], kv[i % NK], s[i]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int at = 16 * j + 4 * grp;
+            const f4 m4 = *reinterpret_cast<const f4 *>(&row_m[id & 1][at]);
+            const f4 i4 = *reinterpret_cast<const f4 *>(&row_inv[id & 1][at]);
+            int last[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) last[x] = row_last[id & 1][at + x];
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                const int key = k0 + 16 * i + l16;
+                float sum = 0.f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float p = fast_exp2(s[j * NK + i][x] - m4[x]) * i4[x];
+                    sum += key <= last[x] ? p : 0.f;
+                }
+                acc[i] += sum;
+            }
+        }
+        if (id + 1 < nsteps) {
+            put(id + 1);
+            if (id + 2 < nsteps) fetch(rt + 64);
+        }
+        __syncthreads();
+    }
+    const int kpad = (n + 15) & ~15;
+    float *out = a.parts + a.score0[sq] + ((size_t)kvh * nparts + part) * kpad;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+        const float sum = sum4grp(acc[i]);
+        const int key = k0 + 16 * i + l16;
+        if (grp == 0 && key < n) out[key] = sum;
+    }
+}
+
+// The parts of the rows, added in order.
+template <int KT>
+DEVI void paged_wsum(const PagedWeightArgs &a) {
+    const int sq = paged_seq(a, blockIdx.x);
+    const int n = a.n_rows[sq], q_len = a.q_len[sq], rows = q_len * a.G, kpad = (n + 15) & ~15;
+    const int nparts = (rows + a.part_rows - 1) / a.part_rows;
+    const int per_head = (n + 255) / 256;
+    const int item = (int)blockIdx.x - a.first[sq];
+    const int kvh = item / per_head, key = (item % per_head) * 256 + (int)threadIdx.x;
+    if (key >= n) return;
+    const int from = max(0, key / KT * KT - (n - q_len)) * a.G / a.part_rows;  // the first part that saw the tile
+    const float *p = a.parts + a.score0[sq] + (size_t)kvh * nparts * kpad + key;
+    float sum = 0.f;
+    for (int i = from; i < nparts; ++i) sum += p[(size_t)i * kpad];
+    const size_t at = ((size_t)a.b[sq] * a.Hkv + kvh) * a.w_stride + key;
+    a.w_out[at] = a.w_in[at] + sum;
+}
+
 #define ZT_PAGED_FEW(DP, NQ)                                                                        \
     extern "C" __global__ void __launch_bounds__(256, 2) zt_paged_few_d##DP##_n##NQ(PagedArgs a) {   \
         paged_few<DP, NQ, true>(a);                                                                 \
     }                                                                                               \
     extern "C" __global__ void __launch_bounds__(256, 2) zt_paged_few_d##DP##_n##NQ##_any(PagedArgs a) { \
         paged_few<DP, NQ, false>(a);                                                                \
+    }
+#define ZT_PAGED_MANY(DP, NW, NQ)                                                                   \
+    extern "C" __global__ void __launch_bounds__(64 * NW, 2) zt_paged_many_d##DP##_##NW##NQ(PagedArgs a) { \
+        paged_many<DP, NW, NQ, true>(a);                                                            \
+    }                                                                                               \
+    extern "C" __global__ void __launch_bounds__(64 * NW, 2) zt_paged_many_d##DP##_##NW##NQ##_any(PagedArgs a) { \
+        paged_many<DP, NW, NQ, false>(a);                                                           \
     }
 #define ZT_PAGED(DP)                                                                                \
     ZT_PAGED_FEW(DP, 1) ZT_PAGED_FEW(DP, 2)                                                         \
@@ -398,3 +1043,24 @@ ZT_PAGED(96)
 ZT_PAGED(128)
 ZT_PAGED(192)
 ZT_PAGED(256)
+ZT_PAGED_MANY(32, 8, 2)
+ZT_PAGED_MANY(64, 8, 2)
+ZT_PAGED_MANY(96, 8, 2)
+ZT_PAGED_MANY(128, 8, 2)
+ZT_PAGED_MANY(192, 8, 1)
+ZT_PAGED_MANY(256, 8, 1)
+#define ZT_PAGED_WPARTS(DP, NK)                                                                     \
+    extern "C" __global__ void __launch_bounds__(512, 2) zt_paged_wparts_d##DP(PagedWeightArgs a) {  \
+        paged_wparts<DP, 8, NK, true>(a);                                                           \
+    }                                                                                               \
+    extern "C" __global__ void __launch_bounds__(512, 2) zt_paged_wparts_d##DP##_any(PagedWeightArgs a) { \
+        paged_wparts<DP, 8, NK, false>(a);                                                          \
+    }
+ZT_PAGED_WPARTS(32, 2)
+ZT_PAGED_WPARTS(64, 2)
+ZT_PAGED_WPARTS(96, 2)
+ZT_PAGED_WPARTS(128, 2)
+ZT_PAGED_WPARTS(192, 1)
+ZT_PAGED_WPARTS(256, 1)
+extern "C" __global__ void __launch_bounds__(256) zt_paged_wsum_256(PagedWeightArgs a) { paged_wsum<256>(a); }
+extern "C" __global__ void __launch_bounds__(256) zt_paged_wsum_128(PagedWeightArgs a) { paged_wsum<128>(a); }

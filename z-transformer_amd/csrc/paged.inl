@@ -78,31 +78,55 @@ static int paged_dp(int dim) {
 
 namespace {
 
-// The 16-row blocks of a tile of the streaming kernel.
-int paged_blocks(int rows) { return rows <= 16 ? 1 : 2; }
+// Which kernel takes a sequence, by its rows per kv head (new tokens x heads of the group): the streaming
+// kernel with one or two 16-row blocks, or the split-operand one.
+enum class PagedKind { None, Few1, Few2, Many };
+constexpr PagedKind kPagedKinds[] = {PagedKind::Few1, PagedKind::Few2, PagedKind::Many};
 
 // What a call does for each sequence.
 struct PagedPlan {
     const int *q_start, *n_rows;
-    int B, H, Hkv, G, dim, part_ld, chunk;
+    int B, H, Hkv, G, dim, dp, part_ld;
+    int chunk_few, chunk_many;  // keys of a workgroup
+    int part_rows;              // rows of a part of the weights' sums (Many)
 
     int q_len(int b) const { return q_start[b + 1] - q_start[b]; }
     int rows(int b) const { return q_len(b) * G; }
-    int tile(int b) const { return 16 * paged_blocks(rows(b)); }
-    int tiles(int b) const { return (rows(b) + tile(b) - 1) / tile(b); }
-    int chunks(int b) const { return q_len(b) ? (n_rows[b] + chunk - 1) / chunk : 0; }
+    PagedKind kind(int b) const {
+        const int r = rows(b);
+        return r == 0 ? PagedKind::None : r <= 16 ? PagedKind::Few1 : r <= 32 ? PagedKind::Few2 : PagedKind::Many;
+    }
+    bool many(int b) const { return kind(b) == PagedKind::Many; }
+    int many_rows() const { return dp <= 128 ? 256 : 128; }     // of a workgroup
+    int weight_keys() const { return dp <= 128 ? 256 : 128; }   // of a workgroup of the weights' sums
+    int tiles(int b) const { return many(b) ? (rows(b) + many_rows() - 1) / many_rows() : 1; }
+    int chunk(int b) const { return many(b) ? chunk_many : chunk_few; }
+    int chunks(int b) const { return q_len(b) ? (n_rows[b] + chunk(b) - 1) / chunk(b) : 0; }
     long long items(int b) const { return (long long)tiles(b) * chunks(b) * Hkv; }
     long long slots(int b) const { return chunks(b) > 1 ? (long long)q_len(b) * H * chunks(b) : 0; }
-    long long scores(int b) const { return (long long)q_len(b) * H * ((n_rows[b] + 15) / 16 * 16); }
+    int kpad(int b) const { return (n_rows[b] + 15) / 16 * 16; }
+    int parts(int b) const { return (rows(b) + part_rows - 1) / part_rows; }
+    // Floats that the weights need: every row's scores, or the parts' sums.
+    long long scores(int b) const { return (long long)kpad(b) * (many(b) ? (long long)Hkv * parts(b) : (long long)q_len(b) * H); }
 };
 
 PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
-    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, (dim + 3) / 4 * 4, 0};
-    long long tiles = 0;  // (16 keys x row tile) steps
-    for (int b = 0; b < B; ++b) tiles += (long long)p.tiles(b) * Hkv * ((n_rows[b] + 15) / 16);
-    long long per = (tiles + 1023) / 1024;
-    per = std::max(8LL, (per + 3) / 4 * 4);  // whole rounds of four waves
-    p.chunk = (int)std::min(16 * per, 1LL << 30);
+    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, 0, 0, 0};
+    long long few = 0, many = 0, most = 0, sums = 0;  // steps of 16 and of 32 keys; row tiles x key tiles
+    for (int b = 0; b < B; ++b) {
+        if (p.many(b)) {
+            many += (long long)p.tiles(b) * Hkv * ((n_rows[b] + 31) / 32);
+            most = std::max(most, (long long)(n_rows[b] + 31) / 32);
+            sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
+        } else if (p.q_len(b)) {
+            few += (long long)Hkv * ((n_rows[b] + 15) / 16);
+        }
+    }
+    const long long f = std::max(8LL, (few + 1023) / 1024);
+    p.chunk_few = (int)std::min(16 * ((f + 3) / 4 * 4), 1LL << 30);  // whole rounds of four waves
+    const long long m = std::max(8LL, (many + 255) / 256);
+    p.chunk_many = (int)std::min(32 * m, 1LL << 30);
+    p.part_rows = (int)std::min(std::max(256LL, (sums / 512 + 31) / 32 * 32), 1LL << 30);
     return p;
 }
 
@@ -119,7 +143,7 @@ PagedSpace paged_space(const PagedPlan &p, bool weights) {
     PagedSpace s{};
     s.ml = align256((size_t)slots * p.part_ld * sizeof(float));
     s.stat = s.ml + align256((size_t)slots * 2 * sizeof(float));
-    s.scores = s.stat + (weights ? align256((size_t)p.q_start[p.B] * p.H * sizeof(float)) : 0);
+    s.scores = s.stat + (weights ? align256((size_t)p.q_start[p.B] * p.H * 2 * sizeof(float)) : 0);
     s.bytes = s.scores + (weights ? (size_t)scores * sizeof(float) : 0);
     return s;
 }
@@ -177,72 +201,90 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     a.part_acc = reinterpret_cast<float *>(ws);
     a.part_ml = reinterpret_cast<float *>(ws + space.ml);
     a.stat = weights ? reinterpret_cast<float *>(ws + space.stat) : nullptr;
-    a.scores = weights ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
     a.H = n_heads; a.Hkv = n_kv_heads; a.G = p.G; a.dim = dim;
-    a.part_ld = p.part_ld; a.chunk = p.chunk;
+    a.part_ld = p.part_ld;
     a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)dim));
     // Whole 16-byte chunks throughout a row.
-    const bool full = dim == dp && dim % 4 == 0;
+    const char *const any = dim == dp ? "" : "_any";
 
-    // Launches of up to ZT_PAGED_MAXB sequences of those that `take` has work items for.
-    const auto each = [&](const char *name, unsigned threads, unsigned per_wg, auto take) -> int {
-        long long part0 = 0, score0 = 0, blocks = 0;
-        a.ns = 0;
+    // Launches `name` for the sequences that `items` has work items for, up to ZT_PAGED_MAXB at a time; per_wg items
+    // to a workgroup.  `each` fills in argument block x's entry i for sequence b.
+    const auto launch_for = [&](const char *name, unsigned threads, unsigned per_wg, auto &x, auto items, auto each) -> int {
+        long long blocks = 0;
+        x.ns = 0;
         const auto flush = [&]() -> int {
-            if (!a.ns) return 0;
             const unsigned long long wgs = ((unsigned long long)blocks + per_wg - 1) / per_wg;
-            if (!grid_ok(wgs, threads) || launch(st, name, (unsigned)wgs, a, stream, threads)) return 1;
-            a.ns = 0;
+            const bool bad = x.ns && (!grid_ok(wgs, threads) || launch(st, name, (unsigned)wgs, x, stream, threads));
+            x.ns = 0;
             blocks = 0;
-            return 0;
+            return bad;
         };
         for (int b = 0; b < B; ++b) {
-            const long long items = take(b);
-            if (items > 0) {
-                if (a.ns == ZT_PAGED_MAXB || blocks + items > INT32_MAX)
-                    if (flush()) return 1;
-                if (items > INT32_MAX) return grid_ok(0) ? 0 : 1;
-                const int i = a.ns++;
-                a.b[i] = b; a.q0[i] = q_start[b]; a.q_len[i] = p.q_len(b); a.n_rows[i] = n_rows[b];
-                a.first[i] = (int)blocks;
-                a.nch[i] = p.chunks(b);
-                a.part0[i] = part0;
-                a.score0[i] = score0;
-                blocks += items;
+            const long long n = items(b);
+            if (n > 0) {
+                if ((x.ns == ZT_PAGED_MAXB || blocks + n > INT32_MAX) && flush()) return 1;
+                if (n > INT32_MAX) {
+                    grid_ok((unsigned long long)n, threads);  // says why
+                    return 1;
+                }
+                const int i = x.ns++;
+                x.b[i] = b; x.q0[i] = q_start[b]; x.q_len[i] = p.q_len(b); x.n_rows[i] = n_rows[b];
+                x.first[i] = (int)blocks;
+                each(i, b);
+                blocks += n;
             }
-            part0 += p.slots(b);
-            score0 += p.scores(b);
+            each(-1, b);  // after it
         }
         return flush();
     };
     char name[64];
-    for (int nq : {1, 2}) {
-        snprintf(name, sizeof name, full ? "zt_paged_few_d%d_n%d" : "zt_paged_few_d%d_n%d_any", dp, nq);
-        if (each(name, kThreads, 1, [&](int b) { return paged_blocks(p.rows(b)) == nq ? p.items(b) : 0LL; })) return 1;
+    for (const PagedKind kind : kPagedKinds) {
+        const bool many = kind == PagedKind::Many;
+        a.chunk = many ? p.chunk_many : p.chunk_few;
+        a.scores = weights && !many ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
+        long long part0 = 0, score0 = 0;
+        const auto fill = [&](int i, int b) {
+            if (i < 0) {
+                part0 += p.slots(b);
+                score0 += p.scores(b);
+                return;
+            }
+            a.nch[i] = p.chunks(b);
+            a.part0[i] = part0;
+            a.score0[i] = score0;
+        };
+        const auto mine = [&](int b) { return p.kind(b) == kind; };
+        if (many) snprintf(name, sizeof name, "zt_paged_many_d%d_8%d%s", dp, dp <= 128 ? 2 : 1, any);
+        else snprintf(name, sizeof name, "zt_paged_few_d%d_n%d%s", dp, kind == PagedKind::Few1 ? 1 : 2, any);
+        if (launch_for(name, many ? 512u : 256u, 1, a, [&](int b) { return mine(b) ? p.items(b) : 0LL; }, fill)) return 1;
+        // Same stream: the merge reads the chunks' partials.
+        part0 = score0 = 0;
+        snprintf(name, sizeof name, "zt_paged_merge_d%d", dp);
+        const auto merged = [&](int b) { return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads : 0LL; };
+        if (launch_for(name, 256u, 4, a, merged, fill)) return 1;
     }
-    // Same stream: the merge reads the chunks' partials, the weights the rows' statistics.
-    snprintf(name, sizeof name, "zt_paged_merge_d%d", dp);
-    if (each(name, kThreads, 4, [&](int b) { return p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads : 0LL; })) return 1;
     if (!weights) return 0;
+    // ... and these the rows' statistics.
     PagedWeightArgs g{};
-    g.scores = a.scores; g.stat = a.stat; g.w_in = w_in; g.w_out = w_out;
-    g.H = n_heads; g.Hkv = n_kv_heads; g.G = p.G; g.w_stride = w_stride;
+    g.pool = a.pool; g.q = q; g.stat = a.stat; g.w_in = w_in; g.w_out = w_out;
+    g.scores = g.parts = reinterpret_cast<float *>(ws + space.scores);
+    g.H = n_heads; g.Hkv = n_kv_heads; g.G = p.G; g.dim = dim; g.w_stride = w_stride;
+    g.part_rows = p.part_rows;
+    g.scale_log2e = a.scale_log2e;
     long long score0 = 0;
-    for (int b0 = 0; b0 < B; b0 += ZT_PAGED_MAXB) {
-        g.ns = std::min(B - b0, ZT_PAGED_MAXB);
-        long long blocks = 0;
-        for (int i = 0; i < g.ns; ++i) {
-            const int b = b0 + i;
-            g.b[i] = b; g.q0[i] = q_start[b]; g.q_len[i] = p.q_len(b); g.n_rows[i] = n_rows[b];
-            g.first[i] = (int)blocks;
-            g.score0[i] = score0;
-            blocks += (long long)((n_rows[b] + 1023) / 1024) * n_kv_heads;
-            score0 += p.scores(b);
-        }
-        if (blocks == 0) continue;
-        if (!grid_ok((unsigned long long)blocks) || launch(st, "zt_paged_weights", (unsigned)blocks, g, stream)) return 1;
-    }
-    return 0;
+    const auto fill = [&](int i, int b) {
+        if (i < 0) score0 += p.scores(b);
+        else g.score0[i] = score0;
+    };
+    const auto per_head = [&](int b, int keys) { return (long long)((n_rows[b] + keys - 1) / keys) * n_kv_heads; };
+    if (launch_for("zt_paged_weights", 256u, 1, g, [&](int b) { return p.many(b) ? 0LL : per_head(b, 1024); }, fill)) return 1;
+    score0 = 0;
+    snprintf(name, sizeof name, "zt_paged_wparts_d%d%s", dp, any);
+    const auto parts = [&](int b) { return p.many(b) ? per_head(b, p.weight_keys()) * p.parts(b) : 0LL; };
+    if (launch_for(name, 512u, 1, g, parts, fill)) return 1;
+    score0 = 0;
+    snprintf(name, sizeof name, "zt_paged_wsum_%d", p.weight_keys());
+    return launch_for(name, 256u, 1, g, [&](int b) { return p.many(b) ? per_head(b, 256) : 0LL; }, fill);
 }
 
 int zt_paged_append(const float *q, const float *k_new, const float *v_new, float *q_out, float *k_pages, float *v_pages,
