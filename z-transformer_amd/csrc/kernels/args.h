@@ -88,6 +88,20 @@ struct PagePool {
     int n_pages, shift, table_stride;
 };
 
+// The sequences of a launch, an array per field: a wave reads them all at once, a
+// lane per sequence, and takes the one that its work item belongs to (paged.h).
+struct PagedSeqs {
+    int n;
+    int first[ZT_PAGED_MAXB];   // first work item of the launch
+    int b[ZT_PAGED_MAXB];       // row of the page table
+    int q0[ZT_PAGED_MAXB];      // first token
+    int q_len[ZT_PAGED_MAXB];   // new tokens
+    int n_rows[ZT_PAGED_MAXB];  // rows of the cache, the new tokens' last
+    int nch[ZT_PAGED_MAXB];     // key chunks; 1: the output is written at once
+    int chunk[ZT_PAGED_MAXB];   // keys of one
+    long long at0[ZT_PAGED_MAXB];
+};
+
 // Attention over a paged cache.  Per sequence i of the launch and kv head, the rows
 // are its q_len[i] new tokens' query heads of that group, token-major: row r is
 // token r / G, head r % G of the group.
@@ -102,16 +116,8 @@ struct PagedArgs {
     float *scores;      // scaled scores (log2 units), or null: sequence i's at score0[i], [Hkv, rows, keys padded to 16]
     int H, Hkv, G, dim;
     int part_ld;        // dim rounded up to whole 16 bytes
-    int chunk;          // keys per workgroup
-    int ns;             // sequences
     float scale_log2e;
-    int b[ZT_PAGED_MAXB];       // row of the page table
-    int q0[ZT_PAGED_MAXB];      // first token
-    int q_len[ZT_PAGED_MAXB];   // new tokens
-    int n_rows[ZT_PAGED_MAXB];  // rows of the cache, the new tokens' last
-    int first[ZT_PAGED_MAXB];   // first work item of the launch
-    int nch[ZT_PAGED_MAXB];     // key chunks; 1: the output is written at once
-    long long part0[ZT_PAGED_MAXB];   // first partial: slot (kvh * rows + row) * nch + chunk behind it
+    PagedSeqs seq;      // at0: the first partial, slot (kvh * rows + row) * nch + chunk behind it
     long long score0[ZT_PAGED_MAXB];
 };
 
@@ -122,12 +128,11 @@ struct PagedWeightArgs {
     const float *q, *scores, *stat;
     const float *w_in;  // [B, Hkv, w_stride]
     float *w_out;
-    float *parts;       // sequence i's at score0[i]: [Hkv, parts, keys padded to 16]
-    int H, Hkv, G, dim, w_stride, ns;
+    float *parts;       // [Hkv, parts, keys padded to 16]
+    int H, Hkv, G, dim, w_stride;
     int part_rows;      // rows of a part
     float scale_log2e;
-    int b[ZT_PAGED_MAXB], q0[ZT_PAGED_MAXB], q_len[ZT_PAGED_MAXB], n_rows[ZT_PAGED_MAXB], first[ZT_PAGED_MAXB];
-    long long score0[ZT_PAGED_MAXB];
+    PagedSeqs seq;      // at0: the sequence's scores or parts
 };
 
 // Append of new tokens to a paged cache, with RoPE on q and k.

@@ -68,17 +68,17 @@ DEVI void paged_few(const PagedArgs &a) {
     __shared__ float Wm[NW][16], Wl[NW][16];
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int sq = paged_seq(a, blockIdx.x);
-    const int nch = a.nch[sq], q_len = a.q_len[sq], rows = q_len * a.G;
-    int item = (int)blockIdx.x - a.first[sq];
-    const int kvh = item % a.Hkv;
-    item /= a.Hkv;
-    const int c = item % nch, row0 = item / nch * 16 * NQ;
-    const int seen0 = a.n_rows[sq] - q_len;  // the cache row of token 0, the last it sees
+    const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
+    const int nch = sq.nch, q_len = sq.q_len, rows = q_len * a.G;
+    int item = (int)blockIdx.x - sq.first;
+    const int c = item % nch;
+    item /= nch;
+    const int kvh = item % a.Hkv, row0 = item / a.Hkv * 16 * NQ;
+    const int seen0 = sq.n_rows - q_len;  // the cache row of token 0, the last it sees
     const int kend = seen0 + (min(rows, row0 + 16 * NQ) - 1) / a.G + 1;
-    const int key0 = c * a.chunk, key1 = min(kend, key0 + a.chunk);
+    const int key0 = c * sq.chunk, key1 = min(kend, key0 + sq.chunk);
     if (key0 >= kend) return;  // workgroup-uniform
-    const int *table = a.pool.table + (size_t)a.b[sq] * a.pool.table_stride;
+    const int *table = a.pool.table + (size_t)sq.b * a.pool.table_stride;
     const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
     const bool vec4 = (a.dim & 3) == 0;
     const float *kb = a.pool.k + (size_t)kvh * a.dim, *vb = a.pool.v + (size_t)kvh * a.dim;
@@ -90,7 +90,7 @@ DEVI void paged_few(const PagedArgs &a) {
     for (int n = 0; n < NQ; ++n) {
         const int r = min(row0 + 16 * n + l16, rows - 1), t = r / a.G;
         last[n] = seen0 + t;
-        const float *row = a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+        const float *row = a.q + (size_t)(sq.q0 + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             load_cols<4, FULL>(q[n][j], row, 16 * j + 4 * grp, a.dim, vec4);
@@ -162,8 +162,8 @@ DEVI void paged_few(const PagedArgs &a) {
                 if (edge && (key > last[n] || key >= key1)) s[n][r] = -INFINITY;
             }
         if (a.scores) {
-            const int kpad = (a.n_rows[sq] + 15) & ~15;
-            float *sp = a.scores + a.score0[sq] + (size_t)kvh * rows * kpad + k0 + 4 * grp;
+            const int kpad = (sq.n_rows + 15) & ~15;
+            float *sp = a.scores + a.score0[sq.i] + (size_t)kvh * rows * kpad + k0 + 4 * grp;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 const int r = row0 + 16 * n + l16;
@@ -269,14 +269,14 @@ DEVI void paged_few(const PagedArgs &a) {
                 A += *reinterpret_cast<const f4 *>(&Wacc[x][i][col]) * f;
             }
             const int t = r / a.G, h = kvh * a.G + r - t * a.G;
-            const size_t row = (size_t)(a.q0[sq] + t);
+            const size_t row = (size_t)(sq.q0 + t);
             if (nch == 1) {
                 if (col == 0) {
                     put_stats(a, row * a.H + h, M, L);
                 }
                 store4(a.out + row * qld + (size_t)h * a.dim, col, a.dim, vec4, A * (1.f / L));
             } else {
-                const size_t slot = (size_t)a.part0[sq] + ((size_t)kvh * rows + r) * nch + c;
+                const size_t slot = (size_t)sq.at0 + ((size_t)kvh * rows + r) * nch + c;
                 *reinterpret_cast<f4 *>(a.part_acc + slot * a.part_ld + col) = A;
                 if (col == 0) { a.part_ml[2 * slot] = M; a.part_ml[2 * slot + 1] = L; }
             }
@@ -322,21 +322,24 @@ DEVI void paged_many(const PagedArgs &a) {
 
     const int tid = opaque((int)threadIdx.x), lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int sq = paged_seq(a, blockIdx.x);
-    const int nch = a.nch[sq], q_len = a.q_len[sq], rows = q_len * a.G;
-    int item = (int)blockIdx.x - a.first[sq];
+    const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
+    const int nch = sq.nch, q_len = sq.q_len, rows = q_len * a.G;
+    int item = (int)blockIdx.x - sq.first;
     const int kvh = item % a.Hkv;
     item /= a.Hkv;
-    const int c = item % nch;
-    constexpr int RT = 16 * NQ * NW;  // rows of a workgroup; the last tile, with most keys, first
-    const int wg_row0 = ((rows + RT - 1) / RT - 1 - item / nch) * RT, row0 = wg_row0 + 16 * NQ * w;
-    const int seen0 = a.n_rows[sq] - q_len;
+    // Chunk by chunk, in each the last row tile, with most keys, first: neighbours are of like length (workgroups
+    // go to the XCDs and their shader engines in turn, so that a pattern of long and short ones would
+    // pile up the long ones: a 2048-row prompt cut in two took 327 us with a tile's chunks side by side).
+    constexpr int RT = 16 * NQ * NW;  // rows of a workgroup
+    const int ntiles = (rows + RT - 1) / RT, c = item / ntiles;
+    const int wg_row0 = (ntiles - 1 - item % ntiles) * RT, row0 = wg_row0 + 16 * NQ * w;
+    const int seen0 = sq.n_rows - q_len;
     const int kend_wg = seen0 + (min(rows, wg_row0 + RT) - 1) / a.G + 1;
     const int kend_w = row0 < rows ? seen0 + (min(rows, row0 + 16 * NQ) - 1) / a.G + 1 : 0;
-    const int key0 = c * a.chunk, key1 = min(kend_wg, key0 + a.chunk);
+    const int key0 = c * sq.chunk, key1 = min(kend_wg, key0 + sq.chunk);
     if (key0 >= kend_wg) return;  // workgroup-uniform
     const int edge0 = seen0 + wg_row0 / a.G;  // the workgroup's first row sees keys up to this one
-    const int *table = a.pool.table + (size_t)a.b[sq] * a.pool.table_stride;
+    const int *table = a.pool.table + (size_t)sq.b * a.pool.table_stride;
     const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
     const float *kb = a.pool.k + (size_t)kvh * a.dim, *vb = a.pool.v + (size_t)kvh * a.dim;
     const bool vec4 = (a.dim & 3) == 0;
@@ -397,7 +400,7 @@ DEVI void paged_many(const PagedArgs &a) {
     for (int n = 0; n < NQ; ++n) {
         const int r = min(row0 + 16 * n + l16, rows - 1), t = r / a.G;
         last[n] = seen0 + t;
-        const float *row = a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+        const float *row = a.q + (size_t)(sq.q0 + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
             float y[8];
@@ -565,7 +568,7 @@ DEVI void paged_many(const PagedArgs &a) {
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
                     const int r = min(row0 + 16 * n + lrow, rows - 1), t = r / a.G;
-                    qrow[n] = a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+                    qrow[n] = a.q + (size_t)(sq.q0 + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
                 }
 #pragma unroll 1
                 for (int cc = 0; cc < 8 * NKS; ++cc) {
@@ -686,7 +689,7 @@ DEVI void paged_many(const PagedArgs &a) {
         const float l = sum4grp(lsum[n]);
         if (r >= rows) continue;
         const int t = r / a.G, h = kvh * a.G + r - t * a.G;
-        const size_t row = (size_t)(a.q0[sq] + t);
+        const size_t row = (size_t)(sq.q0 + t);
         if (nch == 1) {
             const float inv = 1.f / l;
             if (egrp == 0) put_stats(a, row * a.H + h, m[n], l);
@@ -694,7 +697,7 @@ DEVI void paged_many(const PagedArgs &a) {
             for (int i = 0; i < NT; ++i)
                 store4(a.out + row * qld + (size_t)h * a.dim, 16 * i + 4 * egrp, a.dim, vec4, o[i][n] * inv);
         } else {
-            const size_t slot = (size_t)a.part0[sq] + ((size_t)kvh * rows + r) * nch + c;
+            const size_t slot = (size_t)sq.at0 + ((size_t)kvh * rows + r) * nch + c;
             if (egrp == 0) { a.part_ml[2 * slot] = m[n]; a.part_ml[2 * slot + 1] = l; }
 #pragma unroll
             for (int i = 0; i < NT; ++i)
@@ -706,71 +709,81 @@ DEVI void paged_many(const PagedArgs &a) {
 
 // ---- Merge of the key chunks --------------------------------------------------------
 //
-// A wave takes one (token, head): M = max_c m_c, out = sum_c acc_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).
-// LPR lanes cover a partial row with 16-byte loads, 64 / LPR chunks at a time, eight such
-// loads in flight; each lane group folds its chunks, then the groups are merged in a fixed order.
-template <int DP>
+// Of one (token, head): M = max_c m_c, out = sum_c acc_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).
+// LPR lanes cover a partial row with 16-byte loads.  ROWS false, for few rows of many
+// chunks: a wave takes a row, its lane groups 64 / LPR chunks at a time, and the groups are
+// merged in a fixed order; true, for many rows of few chunks: each lane group takes a row
+// (65536 rows of 3 chunks at d = 128: 43 us with a wave to a row).
+template <int DP, bool ROWS>
 DEVI void paged_merge(const PagedArgs &a) {
-    constexpr int LPR = DP <= 32 ? 8 : DP <= 64 ? 16 : DP <= 128 ? 32 : 64, GR = 64 / LPR;
-    const int lane = lane_id(), w = threadIdx.x >> 6;
-    const int item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + w);
-    const int sq = paged_seq(a, item);
-    const int q_len = a.q_len[sq], rows = q_len * a.G, nslots = a.nch[sq];
-    const int i = item - a.first[sq];
-    if (i >= q_len * a.H) return;  // the last sequence's end
-    const int t = i / a.H, h = i % a.H, kvh = h / a.G, r = t * a.G + h % a.G;
-    const int nch = (a.n_rows[sq] - q_len + t) / a.chunk + 1;  // chunks that hold a key the token sees
-    const size_t slot0 = (size_t)a.part0[sq] + ((size_t)kvh * rows + r) * nslots;
-    const int g = lane / LPR, col = 4 * (lane % LPR);
+    constexpr int LPR = DP <= 32 ? 8 : DP <= 64 ? 16 : DP <= 128 ? 32 : 64, GR = ROWS ? 1 : 64 / LPR;
+    constexpr int U = ROWS ? 4 : 8;  // chunks of a lane group in flight
+    const int lane = lane_id(), g = ROWS ? 0 : lane / LPR, col = 4 * (lane % LPR);
+    const int per_wg = ROWS ? 256 / LPR : 4;
+    const int item0 = (int)blockIdx.x * per_wg;
+    int item = item0 + (int)threadIdx.x / (256 / per_wg);
+    const PagedSeq sq = paged_seq(a.seq, item0);
+    // The workgroup's rows, if they are all of one sequence; else each lane group's own.
+    int q_len = sq.q_len, n_rows = sq.n_rows, nslots = sq.nch, chunk = sq.chunk, q0 = sq.q0, i = item - sq.first;
+    long long at0 = sq.at0;
+    int k = sq.i;
+    while (i >= q_len * a.H) {  // of a sequence behind it, or past the last's end
+        if (++k == a.seq.n) return;
+        i = item - a.seq.first[k];
+        q_len = a.seq.q_len[k]; n_rows = a.seq.n_rows[k]; nslots = a.seq.nch[k]; chunk = a.seq.chunk[k]; q0 = a.seq.q0[k];
+        at0 = a.seq.at0[k];
+    }
+    const int rows = q_len * a.G, t = i / a.H, h = i % a.H, kvh = h / a.G, r = t * a.G + h % a.G;
+    const int nch = (n_rows - q_len + t) / chunk + 1;  // chunks that hold a key the token sees
+    const size_t slot0 = (size_t)at0 + ((size_t)kvh * rows + r) * nslots;
     const bool ok = col < a.dim;
     const float *acc = a.part_acc + slot0 * a.part_ld + col;
     const float *ml = a.part_ml + 2 * slot0;
     float M = -INFINITY, L = 0.f;
     f4 A = zero4();
-    for (int c0 = g; c0 < nch; c0 += 8 * GR) {
-        float e[8], l[8];
-        f4 x[8];
+    for (int c0 = g; c0 < nch; c0 += U * GR) {
+        f2 e[U];
+        f4 x[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < U; ++j) {
             const int c = c0 + j * GR;
             const bool in = c < nch;
-            e[j] = in ? ml[2 * c] : -INFINITY;
-            l[j] = in ? ml[2 * c + 1] : 0.f;
+            e[j] = in ? *reinterpret_cast<const f2 *>(ml + 2 * c) : f2{-INFINITY, 0.f};
             x[j] = in && ok ? *reinterpret_cast<const f4 *>(acc + (size_t)c * a.part_ld) : zero4();
         }
         float mb = M;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mb = fmaxf(mb, e[j]);
+        for (int j = 0; j < U; ++j) mb = fmaxf(mb, e[j].x);
         const float f0 = M == -INFINITY ? 0.f : fast_exp2(M - mb);
         L *= f0;
         A *= f0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float f = e[j] == -INFINITY ? 0.f : fast_exp2(e[j] - mb);
-            L += l[j] * f;
+        for (int j = 0; j < U; ++j) {
+            const float f = e[j].x == -INFINITY ? 0.f : fast_exp2(e[j].x - mb);
+            L += e[j].y * f;
             A += x[j] * f;
         }
         M = mb;
     }
+    if constexpr (!ROWS) {
 #pragma unroll
-    for (int d = LPR; d < 64; d <<= 1) {  // both sides of an exchange form the same sums
-        const float M2 = wave_xor(M, d), mb = fmaxf(M, M2);
-        const float f1 = M == -INFINITY ? 0.f : fast_exp2(M - mb), f2v = M2 == -INFINITY ? 0.f : fast_exp2(M2 - mb);
-        const bool up = lane & d;
-        const float la = L * f1, lb = wave_xor(L, d) * f2v;
-        L = up ? lb + la : la + lb;
+        for (int d = LPR; d < 64; d <<= 1) {  // both sides of an exchange form the same sums
+            const float M2 = wave_xor(M, d), mb = fmaxf(M, M2);
+            const float f1 = M == -INFINITY ? 0.f : fast_exp2(M - mb), f2v = M2 == -INFINITY ? 0.f : fast_exp2(M2 - mb);
+            const bool up = lane & d;
+            const float la = L * f1, lb = wave_xor(L, d) * f2v;
+            L = up ? lb + la : la + lb;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float xa = A[k] * f1, xb = wave_xor(A[k], d) * f2v;
-            A[k] = up ? xb + xa : xa + xb;
+            for (int k2 = 0; k2 < 4; ++k2) {
+                const float xa = A[k2] * f1, xb = wave_xor(A[k2], d) * f2v;
+                A[k2] = up ? xb + xa : xa + xb;
+            }
+            M = mb;
         }
-        M = mb;
     }
     if (g != 0 || !ok) return;
-    const size_t row = (size_t)(a.q0[sq] + t);
-    if (col == 0) {
-        put_stats(a, row * a.H + h, M, L);
-    }
+    const size_t row = (size_t)(q0 + t);
+    if (col == 0) put_stats(a, row * a.H + h, M, L);
     store4(a.out + row * a.H * a.dim + (size_t)h * a.dim, col, a.dim, (a.dim & 3) == 0, A * (1.f / L));
 }
 
@@ -780,15 +793,15 @@ DEVI void paged_merge(const PagedArgs &a) {
 // (sequence, kv head) and adds the weights of all rows, rows in order.  Sequences without
 // new tokens copy their weights.
 extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightArgs a) {
-    const int sq = paged_seq(a, blockIdx.x);
-    const int n = a.n_rows[sq], kpad = (n + 15) & ~15, rows = a.q_len[sq] * a.G;
+    const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
+    const int n = sq.n_rows, kpad = (n + 15) & ~15, rows = sq.q_len * a.G;
     const int per_head = (n + 1023) / 1024;
-    const int item = (int)blockIdx.x - a.first[sq];
+    const int item = (int)blockIdx.x - sq.first;
     const int kvh = item / per_head, key = (item % per_head) * 1024 + 4 * (int)threadIdx.x;
     if (key >= n) return;
-    const float *sp = a.scores + a.score0[sq] + (size_t)kvh * rows * kpad + key;
-    const float *st = a.stat + 2 * ((size_t)a.q0[sq] * a.H + kvh * a.G);
-    const int seen0 = n - a.q_len[sq];
+    const float *sp = a.scores + sq.at0 + (size_t)kvh * rows * kpad + key;
+    const float *st = a.stat + 2 * ((size_t)sq.q0 * a.H + kvh * a.G);
+    const int seen0 = n - sq.q_len;
     f4 sum = zero4();
     int t = 0, g = 0;
     for (int r = 0; r < rows; ++r) {
@@ -800,7 +813,7 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
         }
         if (++g == a.G) { g = 0; ++t; }
     }
-    const size_t at = ((size_t)a.b[sq] * a.Hkv + kvh) * a.w_stride + key;
+    const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (key + e < n) a.w_out[at + e] = a.w_in[at + e] + sum[e];
@@ -820,17 +833,18 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
     __shared__ int flags[2];
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int sq = paged_seq(a, blockIdx.x);
-    const int n = a.n_rows[sq], q_len = a.q_len[sq], rows = q_len * a.G, seen0 = n - q_len;
+    const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
+    const int n = sq.n_rows, q_len = sq.q_len, rows = q_len * a.G, seen0 = n - q_len;
     const int nparts = (rows + a.part_rows - 1) / a.part_rows;
-    int item = (int)blockIdx.x - a.first[sq];
+    int item = (int)blockIdx.x - sq.first;
     const int kvh = item % a.Hkv;
     item /= a.Hkv;
-    const int part = item % nparts, kt0 = item / nparts * KT;
+    // Part by part, the last, which all keys of a prompt have rows in, first (neighbours of like length, as in paged_many).
+    const int ntiles = (n + KT - 1) / KT, part = nparts - 1 - item / ntiles, kt0 = item % ntiles * KT;
     // Rows of the part that see the tile's first key.
     const int r0 = max(part * a.part_rows, max(0, kt0 - seen0) * a.G) & ~31, r1 = min(rows, (part + 1) * a.part_rows);
     if (r0 >= r1) return;  // workgroup-uniform; zt_paged_wsum does not read it
-    const int *table = a.pool.table + (size_t)a.b[sq] * a.pool.table_stride;
+    const int *table = a.pool.table + (size_t)sq.b * a.pool.table_stride;
     const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
     const float *kb = a.pool.k + (size_t)kvh * a.dim;
     const bool vec4 = (a.dim & 3) == 0;
@@ -871,7 +885,7 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
     auto q_row = [&](int r) {  // of row r, or the part's last
         r = min(r, r1 - 1);
         const int t = r / a.G;
-        return a.q + (size_t)(a.q0[sq] + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
+        return a.q + (size_t)(sq.q0 + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
     };
     float px[NP][8], sm = 0.f, si = 0.f;
     int sl = 0;
@@ -891,7 +905,7 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
         }
         if (tid < 32) {
             const int r = min(rt + tid, r1 - 1), t = r / a.G;
-            const f2 ml = *reinterpret_cast<const f2 *>(a.stat + 2 * ((size_t)(a.q0[sq] + t) * a.H + kvh * a.G + r - t * a.G));
+            const f2 ml = *reinterpret_cast<const f2 *>(a.stat + 2 * ((size_t)(sq.q0 + t) * a.H + kvh * a.G + r - t * a.G));
             sm = ml.x;
             si = ml.y;
             sl = rt + tid < r1 ? seen0 + t : -1;  // a row past the part's last sees nothing
@@ -993,7 +1007,7 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
         __syncthreads();
     }
     const int kpad = (n + 15) & ~15;
-    float *out = a.parts + a.score0[sq] + ((size_t)kvh * nparts + part) * kpad;
+    float *out = a.parts + sq.at0 + ((size_t)kvh * nparts + part) * kpad;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
         const float sum = sum4grp(acc[i]);
@@ -1005,18 +1019,18 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
 // The parts of the rows, added in order.
 template <int KT>
 DEVI void paged_wsum(const PagedWeightArgs &a) {
-    const int sq = paged_seq(a, blockIdx.x);
-    const int n = a.n_rows[sq], q_len = a.q_len[sq], rows = q_len * a.G, kpad = (n + 15) & ~15;
+    const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
+    const int n = sq.n_rows, q_len = sq.q_len, rows = q_len * a.G, kpad = (n + 15) & ~15;
     const int nparts = (rows + a.part_rows - 1) / a.part_rows;
     const int per_head = (n + 255) / 256;
-    const int item = (int)blockIdx.x - a.first[sq];
+    const int item = (int)blockIdx.x - sq.first;
     const int kvh = item / per_head, key = (item % per_head) * 256 + (int)threadIdx.x;
     if (key >= n) return;
     const int from = max(0, key / KT * KT - (n - q_len)) * a.G / a.part_rows;  // the first part that saw the tile
-    const float *p = a.parts + a.score0[sq] + (size_t)kvh * nparts * kpad + key;
+    const float *p = a.parts + sq.at0 + (size_t)kvh * nparts * kpad + key;
     float sum = 0.f;
     for (int i = from; i < nparts; ++i) sum += p[(size_t)i * kpad];
-    const size_t at = ((size_t)a.b[sq] * a.Hkv + kvh) * a.w_stride + key;
+    const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;
     a.w_out[at] = a.w_in[at] + sum;
 }
 
@@ -1036,31 +1050,36 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
     }
 #define ZT_PAGED(DP)                                                                                \
     ZT_PAGED_FEW(DP, 1) ZT_PAGED_FEW(DP, 2)                                                         \
-    extern "C" __global__ void __launch_bounds__(256) zt_paged_merge_d##DP(PagedArgs a) { paged_merge<DP>(a); }
+    extern "C" __global__ void __launch_bounds__(256) zt_paged_merge_d##DP(PagedArgs a) {     \
+        paged_merge<DP, false>(a);                                                                  \
+    }                                                                                               \
+    extern "C" __global__ void __launch_bounds__(256) zt_paged_merge_rows_d##DP(PagedArgs a) {       \
+        paged_merge<DP, true>(a);                                                                   \
+    }
 ZT_PAGED(32)
 ZT_PAGED(64)
 ZT_PAGED(96)
 ZT_PAGED(128)
 ZT_PAGED(192)
 ZT_PAGED(256)
-ZT_PAGED_MANY(32, 8, 2)
-ZT_PAGED_MANY(64, 8, 2)
-ZT_PAGED_MANY(96, 8, 2)
-ZT_PAGED_MANY(128, 8, 2)
-ZT_PAGED_MANY(192, 8, 1)
-ZT_PAGED_MANY(256, 8, 1)
-#define ZT_PAGED_WPARTS(DP, NK)                                                                     \
-    extern "C" __global__ void __launch_bounds__(512, 2) zt_paged_wparts_d##DP(PagedWeightArgs a) {  \
-        paged_wparts<DP, 8, NK, true>(a);                                                           \
+ZT_PAGED_MANY(32, 4, 1) ZT_PAGED_MANY(32, 4, 2) ZT_PAGED_MANY(32, 8, 2)
+ZT_PAGED_MANY(64, 4, 1) ZT_PAGED_MANY(64, 4, 2) ZT_PAGED_MANY(64, 8, 2)
+ZT_PAGED_MANY(96, 4, 1) ZT_PAGED_MANY(96, 4, 2) ZT_PAGED_MANY(96, 8, 2)
+ZT_PAGED_MANY(128, 4, 1) ZT_PAGED_MANY(128, 4, 2) ZT_PAGED_MANY(128, 8, 2)
+ZT_PAGED_MANY(192, 4, 1) ZT_PAGED_MANY(192, 8, 1)
+ZT_PAGED_MANY(256, 4, 1) ZT_PAGED_MANY(256, 8, 1)
+#define ZT_PAGED_WPARTS(DP, NW, NK)                                                                 \
+    extern "C" __global__ void __launch_bounds__(64 * NW, 2) zt_paged_wparts_d##DP(PagedWeightArgs a) { \
+        paged_wparts<DP, NW, NK, true>(a);                                                          \
     }                                                                                               \
-    extern "C" __global__ void __launch_bounds__(512, 2) zt_paged_wparts_d##DP##_any(PagedWeightArgs a) { \
-        paged_wparts<DP, 8, NK, false>(a);                                                          \
+    extern "C" __global__ void __launch_bounds__(64 * NW, 2) zt_paged_wparts_d##DP##_any(PagedWeightArgs a) { \
+        paged_wparts<DP, NW, NK, false>(a);                                                         \
     }
-ZT_PAGED_WPARTS(32, 2)
-ZT_PAGED_WPARTS(64, 2)
-ZT_PAGED_WPARTS(96, 2)
-ZT_PAGED_WPARTS(128, 2)
-ZT_PAGED_WPARTS(192, 1)
-ZT_PAGED_WPARTS(256, 1)
-extern "C" __global__ void __launch_bounds__(256) zt_paged_wsum_256(PagedWeightArgs a) { paged_wsum<256>(a); }
+ZT_PAGED_WPARTS(32, 4, 2)
+ZT_PAGED_WPARTS(64, 4, 2)
+ZT_PAGED_WPARTS(96, 4, 2)
+ZT_PAGED_WPARTS(128, 4, 2)
+ZT_PAGED_WPARTS(192, 4, 1)
+ZT_PAGED_WPARTS(256, 8, 1)
 extern "C" __global__ void __launch_bounds__(256) zt_paged_wsum_128(PagedWeightArgs a) { paged_wsum<128>(a); }
+extern "C" __global__ void __launch_bounds__(256) zt_paged_wsum_64(PagedWeightArgs a) { paged_wsum<64>(a); }

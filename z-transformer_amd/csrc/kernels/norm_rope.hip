@@ -209,28 +209,36 @@ extern "C" __global__ void __launch_bounds__(256) zt_rope_append(AppendArgs a) {
 // A workgroup takes a group of 256 / (d / 2) tokens, so that its threads compute one
 // (token, pair) angle each (as zt_rope_forward's, in f64) before they share them, and
 // one of a.slices parts of the tokens' heads: few tokens are cut into parts for more workgroups.
-extern "C" __global__ void __launch_bounds__(256) zt_rope_paged(PagedAppendArgs a) {
+// A thread then takes VW pairs of a head, two loads and two stores of 4 VW bytes.  Bound: HBM.
+template <int VW>
+DEVI void rope_paged(const PagedAppendArgs &a) {
+    typedef float vec __attribute__((ext_vector_type(VW)));
+    constexpr int VV = VW == 1 ? 2 : VW;  // of v's copies (rows hold an even number of floats)
+    typedef float vvec __attribute__((ext_vector_type(VV)));
     __shared__ double tab_c[256], tab_s[256];
     __shared__ int row_of[16], seq_of[16], at_of[16];
     const int half = a.dim / 2, per = min(16, 256 / half);
     const int group = (int)blockIdx.x / a.slices, slice = (int)blockIdx.x % a.slices;
     const int t0 = a.token0 + group * per, nt = min(per, a.token0 + a.tokens - t0);
-    for (int j = threadIdx.x; j < nt * half; j += 256) {
-        const int tl = j / half, i = j - tl * half, t = t0 + tl;
+    const int lane = threadIdx.x & 63;
+    const int q0 = a.q0[lane], b = a.b[lane], row0 = a.row0[lane], pos = a.pos[lane];
+    for (int j = threadIdx.x; j < (nt * half + 63 & ~63); j += 256) {  // whole waves
+        const int tl = min(j / half, nt - 1), i = j - tl * half, t = t0 + tl;
         int sq = 0;  // the last sequence that does not begin past the token
-        for (int s = 1; s < a.ns; ++s) sq = a.q0[s] <= t ? s : sq;
-        rope_angle((double)a.pos[sq] + (t - a.q0[sq]), i, a.dim, a.theta, &tab_c[j], &tab_s[j]);
+        for (int s = 1; s < a.ns; ++s) sq = __builtin_amdgcn_readlane(q0, s) <= t ? s : sq;
+        const int at = t - __shfl(q0, sq, 64), p = __shfl(pos, sq, 64), r0 = __shfl(row0, sq, 64), bs = __shfl(b, sq, 64);
+        if (j >= nt * half) continue;
         if (i == 0) {
-            const int row = a.row0[sq] + t - a.q0[sq];
-            row_of[tl] = pool_row(a.pool, a.pool.table + (size_t)a.b[sq] * a.pool.table_stride, row);
-            seq_of[tl] = a.b[sq];
-            at_of[tl] = row;
+            row_of[tl] = pool_row(a.pool, a.pool.table + (size_t)bs * a.pool.table_stride, r0 + at);
+            seq_of[tl] = bs;
+            at_of[tl] = r0 + at;
         }
+        rope_angle((double)p + at, i, a.dim, a.theta, &tab_c[j], &tab_s[j]);
     }
     __syncthreads();
     const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
-    // A token's tasks: its rotations, q's heads (if any) then k's, and the copies of v's pairs of values.
-    const int heads = (a.q ? a.H : 0) + a.Hkv, n_rot = heads * half, tasks = n_rot + a.Hkv * half;
+    // A token's tasks: its rotations, q's heads (if any) then k's, and the copies of v.
+    const int heads = (a.q ? a.H : 0) + a.Hkv, hv = half / VW, n_rot = heads * hv, tasks = n_rot + a.Hkv * (a.dim / VV);
     const int per_slice = (tasks + a.slices - 1) / a.slices;
     const int j0 = slice * per_slice, nj = min(per_slice, tasks - j0);
     for (int e = threadIdx.x; e < nt * nj; e += 256) {
@@ -238,19 +246,28 @@ extern "C" __global__ void __launch_bounds__(256) zt_rope_paged(PagedAppendArgs 
         const size_t t = (size_t)(t0 + tl);
         const int row = row_of[tl];
         if (j < n_rot) {
-            const int h = j / half, i = j - h * half, hk = h - (heads - a.Hkv);
-            const double c = tab_c[tl * half + i], s = tab_s[tl * half + i];
-            if (hk < 0) {
-                const size_t o = t * qld + (size_t)h * a.dim + i;
-                rope_rotate<false>(c, s, a.q + o, a.q_out + o, half);
-            } else if (row >= 0) {
-                const size_t col = (size_t)hk * a.dim + i;
-                rope_rotate<false>(c, s, a.k_new + t * kld + col, a.pool.k + (size_t)row * kld + col, half);
+            const int h = j / hv, i = (j - h * hv) * VW, hk = h - (heads - a.Hkv);
+            if (hk >= 0 && row < 0) continue;
+            const size_t from = t * (hk < 0 ? qld : kld) + (size_t)(hk < 0 ? h : hk) * a.dim + i;
+            const float *x = (hk < 0 ? a.q : a.k_new) + from;
+            float *y = hk < 0 ? a.q_out + from : a.pool.k + (size_t)row * kld + (size_t)hk * a.dim + i;
+            const vec lo = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x));
+            const vec hi = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + half));
+            vec ylo, yhi;
+#pragma unroll
+            for (int v = 0; v < VW; ++v) {
+                const float in[2] = {lo[v], hi[v]};
+                float out[2];
+                rope_rotate<false>(tab_c[tl * half + i + v], tab_s[tl * half + i + v], in, out, 1);
+                ylo[v] = out[0];
+                yhi[v] = out[1];
             }
+            *reinterpret_cast<vec *>(y) = ylo;
+            *reinterpret_cast<vec *>(y + half) = yhi;
         } else if (row >= 0) {
-            const size_t col = 2 * (size_t)(j - n_rot);
-            *reinterpret_cast<f2 *>(a.pool.v + (size_t)row * kld + col) =
-                *reinterpret_cast<const f2 *>(a.v_new + t * kld + col);
+            const size_t col = (size_t)VV * (j - n_rot);
+            *reinterpret_cast<vvec *>(a.pool.v + (size_t)row * kld + col) =
+                __builtin_nontemporal_load(reinterpret_cast<const vvec *>(a.v_new + t * kld + col));
         }
     }
     if (a.w && slice == 0)
@@ -259,6 +276,9 @@ extern "C" __global__ void __launch_bounds__(256) zt_rope_paged(PagedAppendArgs 
             a.w[((size_t)seq_of[tl] * a.Hkv + hk) * a.w_stride + at_of[tl]] = 0.f;
         }
 }
+extern "C" __global__ void __launch_bounds__(256) zt_rope_paged_4(PagedAppendArgs a) { rope_paged<4>(a); }
+extern "C" __global__ void __launch_bounds__(256) zt_rope_paged_2(PagedAppendArgs a) { rope_paged<2>(a); }
+extern "C" __global__ void __launch_bounds__(256) zt_rope_paged_1(PagedAppendArgs a) { rope_paged<1>(a); }
 
 DEVI unsigned long long splitmix64(unsigned long long seed, unsigned long long ctr) {
     unsigned long long z = seed + (ctr + 1ull) * 0x9E3779B97F4A7C15ull;

@@ -15,45 +15,56 @@ DEVI unsigned weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of a wave-uniform count over the workgroup's waves; every thread gets it.
-template <int NW>
-DEVI int block_count(int mine, int *red) {
-    __syncthreads();  // the last reduction's reads
-    if (lane_id() == 0) red[threadIdx.x >> 6] = mine;
-    __syncthreads();
-    int s = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) s += red[i];
-    return s;
+// Lane i of a row of 16 ends with the sum of the row's lanes 0 .. i (VALU only).
+DEVI int row_scan(int v) {
+    v += __builtin_amdgcn_mov_dpp(v, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8; 0 comes in
+    v += __builtin_amdgcn_mov_dpp(v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x118, 0xf, 0xf, true);
+    return v;
 }
-
-// Sums of the waves before this one, and of all.
+// From each wave's entry of red: the sum of those before wave w, and of all.
 template <int NW>
-DEVI int block_before(int mine, int *red, int *all) {
-    __syncthreads();
-    const int w = threadIdx.x >> 6;
+DEVI int waves_before(const int *red, int w, int *all) {
+    const int i = lane_id() & 15;
+    const int v = row_scan(i < NW ? red[i] : 0);
+    *all = __builtin_amdgcn_readlane(v, 15);
+    return w ? __builtin_amdgcn_readlane(v, w - 1) : 0;
+}
+// The same, the wave's own number first put there.
+template <int NW>
+DEVI int block_before(int mine, int w, int *red, int *all) {
+    __syncthreads();  // the last use's reads
     if (lane_id() == 0) red[w] = mine;
     __syncthreads();
-    int before = 0, s = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-        before += i < w ? red[i] : 0;
-        s += red[i];
-    }
-    *all = s;
-    return before;
+    return waves_before<NW>(red, w, all);
 }
 
-// Which rows stay: one workgroup of 16 waves per (sequence, kv head).  The threshold, the
-// largest key T that at least `need` candidates reach, is found bit by bit from the
-// highest; then the rows are walked in order, 1024 at a time, with running counts of those kept and
-// of those that equal T.  w may be compacted in place: a block's rows are read before any
-// is written, and a row never moves up.
-template <int KPT>
+// Lane i ends with the sum of the wave's lanes 0 .. i.
+DEVI int wave_scan(int v) {
+    v = row_scan(v);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+    return v;
+}
+
+// Which rows stay: one workgroup of NW waves per (sequence, kv head).  With the candidates'
+// weights as ordered numbers, T is the largest key that at least `need` of them reach, found by
+// digits of 11, 11 and 10 bits: a histogram (LDS) of the digit among those that share the digits
+// before it, summed from the top, says in which bin the need-th lies.  It ends early
+// where a bin holds exactly as many as are wanted.  Those past T stay and, of those that equal
+// it, the lowest rows that are still wanted.
+//   KPT > 0, up to 64 NW KPT rows: a wave holds a run of 64 KPT rows in registers, so that w is read once, and
+// two sums over the waves place every row.
+//   KPT 0, any number: w is read again for every digit, and rows are placed 64 NW at a time, in order.
+// w may be compacted in place: what a step overwrites has been read, since a row never moves up.
+// Latency: 8192 rows take 72 us by single bits that read w again, 39 by two bits, counted by ballots, from registers.
+template <int NW, int KPT>
 DEVI void evict_select(const PagedEvictArgs &a) {
-    constexpr int NW = 16;
-    __shared__ int red[NW];
-    const int tid = threadIdx.x, lane = lane_id();
+    constexpr int NTH = 64 * NW, BINS = 2048, BPT = BINS / NTH;
+    __shared__ __attribute__((aligned(16))) int hist[BINS];
+    __shared__ int red[2][NW], found[3];
+    const int tid = threadIdx.x, lane = lane_id(), wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sl = (int)blockIdx.x / a.Hkv, h = (int)blockIdx.x % a.Hkv, b = a.b0 + sl;
     const int n = a.n_rows[sl];
     const size_t head = (size_t)b * a.Hkv + h;
@@ -61,68 +72,141 @@ DEVI void evict_select(const PagedEvictArgs &a) {
     float *wo = a.w_out + head * a.w_stride;
     int *kept = a.kept + head * a.budget;
     if (n <= a.budget) {  // all stay
-        for (int i = tid; i < a.budget; i += 64 * NW) kept[i] = i < n ? i : -1;
+        for (int i = tid; i < a.budget; i += NTH) kept[i] = i < n ? i : -1;
         if (wo != w)
-            for (int i = tid; i < n; i += 64 * NW) wo[i] = w[i];
+            for (int i = tid; i < n; i += NTH) wo[i] = w[i];
         return;
     }
     const int lo = a.n_first, hi = n - a.n_last, need = a.budget - a.n_first - a.n_last;
-    unsigned T = 0;
-    int above = 0;  // candidates past T
-    unsigned key[KPT];
+    const int run0 = wv * 64 * KPT + lane;  // KPT > 0: the thread's rows are run0 + 64 k
+    float x[KPT > 0 ? KPT : 1];
+    unsigned key[KPT > 0 ? KPT : 1];
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
-        const int i = lo + k * 64 * NW + tid;
-        key[k] = KPT > 1 && i < hi ? weight_key(w[i]) : 0;
+        const int i = run0 + 64 * k;
+        x[k] = i < n ? w[i] : 0.f;
+        key[k] = weight_key(x[k]);
     }
-    auto count = [&](unsigned at) {  // candidates whose key is at least `at` (> 0)
-        int c = 0;
-        if constexpr (KPT > 1) {
+    unsigned T = 0xffffffffu;  // that none reaches: a NaN's key is 0, +inf's less than this
+    int equal = 0;             // rows wanted of those that equal T
+    if (need > 0) {
+        T = 0;
+        equal = need;
+        int left = 32;  // bits not looked at yet
+        while (left > 0) {
+            const int bits = left > 10 ? 11 : 10, shift = left - bits;
 #pragma unroll
-            for (int k = 0; k < KPT; ++k) c += __popcll(__builtin_amdgcn_ballot_w64(key[k] >= at));
-        } else {
-            for (int i0 = lo; i0 < hi; i0 += 64 * NW) {
-                const int i = i0 + tid;
-                c += __popcll(__builtin_amdgcn_ballot_w64(i < hi && weight_key(w[i]) >= at));
+            for (int j = 0; j < BPT; ++j) hist[j * NTH + tid] = 0;
+            __syncthreads();
+            auto put = [&](unsigned ki) {  // a candidate; those that share the digits so far count
+                if (left == 32 || ki >> left == T >> left) atomicAdd(&hist[ki >> shift & ((1 << bits) - 1)], 1);
+            };
+            if constexpr (KPT > 0) {
+#pragma unroll
+                for (int k = 0; k < KPT; ++k) {
+                    const int i = run0 + 64 * k;
+                    if (i >= lo && i < hi) put(key[k]);
+                }
+            } else {
+                for (int i = lo + tid; i < hi; i += NTH) put(weight_key(w[i]));
+            }
+            __syncthreads();
+            // From the top: thread t has bins BINS - 1 - BPT t and below.
+            int c[BPT], sum = 0;
+#pragma unroll
+            for (int j = 0; j < BPT; ++j) {
+                c[j] = hist[BINS - 1 - (BPT * tid + j)];
+                sum += c[j];
+            }
+            const int upto = wave_scan(sum);
+            if (lane == 63) red[0][wv] = upto;
+            __syncthreads();
+            int all;
+            int above = waves_before<NW>(red[0], wv, &all) + upto - sum;
+#pragma unroll
+            for (int j = 0; j < BPT; ++j) {
+                if (above < equal && above + c[j] >= equal) {  // one thread's one bin
+                    found[0] = BINS - 1 - (BPT * tid + j);
+                    found[1] = above;
+                    found[2] = c[j];
+                }
+                above += c[j];
+            }
+            __syncthreads();
+            T |= (unsigned)found[0] << shift;
+            equal -= found[1];
+            left = shift;
+            if (found[2] == equal) {  // all that reach T stay, whatever the bits behind it
+                if (T == 0) break;    // (every candidate, NaN among them: those equal to 0 by row are all)
+                --T;
+                equal = 0;
+                break;
             }
         }
-        return block_count<NW>(c, red);
-    };
-    if (need > 0) {
-        for (int bit = 31; bit >= 0; --bit) {
-            const unsigned trial = T | 1u << bit;
-            const int c = count(trial);
-            if (c >= need) T = trial;
-            else above = c;
+    }
+    const unsigned long long below = (1ull << lane) - 1;
+    if constexpr (KPT > 0) {
+        int eq = 0, all = 0;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+            const int i = run0 + 64 * k;
+            eq += __popcll(__builtin_amdgcn_ballot_w64(i >= lo && i < hi && key[k] == T));
+        }
+        int eq_at = block_before<NW>(eq, wv, red[0], &all);
+        unsigned long long stay[KPT];
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+            const int i = run0 + 64 * k;
+            const bool cand = i >= lo && i < hi;
+            const unsigned long long e = __builtin_amdgcn_ballot_w64(cand && key[k] == T);
+            stay[k] = __builtin_amdgcn_ballot_w64(
+                i < n && (!cand || key[k] > T || (key[k] == T && eq_at + __popcll(e & below) < equal)));
+            eq_at += __popcll(e);
+            mine += __popcll(stay[k]);
+        }
+        int at = block_before<NW>(mine, wv, red[1], &all);
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+            if (stay[k] >> lane & 1) {
+                const int to = at + __popcll(stay[k] & below);
+                kept[to] = run0 + 64 * k;
+                wo[to] = x[k];
+            }
+            at += __popcll(stay[k]);
         }
     } else {
-        T = 0xffffffffu;  // (a NaN's key is 0 and +inf's is less than this: none reaches it)
-    }
-    const int equal = need - above;  // so many of those that equal T, the lowest rows
-    int n_kept = 0, n_equal = 0;
-    for (int i0 = 0; i0 < n; i0 += 64 * NW) {
-        const int i = i0 + tid;
-        const float wi = i < n ? w[i] : 0.f;
-        const bool cand = i >= lo && i < hi;
-        const unsigned ki = weight_key(wi);
-        const unsigned long long eq = __builtin_amdgcn_ballot_w64(cand && ki == T);
-        int all_eq = 0;
-        const int eq_before = block_before<NW>(__popcll(eq), red, &all_eq) + n_equal;
-        const unsigned long long below = (1ull << lane) - 1;
-        const bool stay = i < n && (!cand || ki > T || (ki == T && eq_before + __popcll(eq & below) < equal));
-        const unsigned long long st = __builtin_amdgcn_ballot_w64(stay);
-        int all = 0;
-        const int at = block_before<NW>(__popcll(st), red, &all) + n_kept + __popcll(st & below);
-        if (stay) {
-            kept[at] = i;
-            wo[at] = wi;
+        int n_kept = 0, n_equal = 0;
+        for (int i0 = 0; i0 < n; i0 += NTH) {
+            const int i = i0 + tid;
+            const float wi = i < n ? w[i] : 0.f;
+            const bool cand = i >= lo && i < hi;
+            const unsigned ki = weight_key(wi);
+            const unsigned long long eq = __builtin_amdgcn_ballot_w64(cand && ki == T);
+            int all_eq = 0;
+            const int eq_before = block_before<NW>(__popcll(eq), wv, red[0], &all_eq) + n_equal;
+            const bool keep = i < n && (!cand || ki > T || (ki == T && eq_before + __popcll(eq & below) < equal));
+            const unsigned long long st = __builtin_amdgcn_ballot_w64(keep);
+            int all = 0;
+            const int at = block_before<NW>(__popcll(st), wv, red[1], &all) + n_kept + __popcll(st & below);
+            if (keep) {
+                kept[at] = i;
+                wo[at] = wi;
+            }
+            n_kept += all;
+            n_equal += all_eq;
         }
-        n_kept += all;
-        n_equal += all_eq;
     }
 }
 
-extern "C" __global__ void __launch_bounds__(1024) zt_evict_select(PagedEvictArgs a) { evict_select<1>(a); }
+#define ZT_EVICT_SELECT(NAME, NW, KPT)                                                              \
+    extern "C" __global__ void __launch_bounds__(64 * NW) zt_evict_select_##NAME(PagedEvictArgs a) { \
+        evict_select<NW, KPT>(a);                                                                   \
+    }
+ZT_EVICT_SELECT(1024, 4, 4)
+ZT_EVICT_SELECT(4096, 8, 8)
+ZT_EVICT_SELECT(16384, 16, 16)
+ZT_EVICT_SELECT(any, 16, 0)
 
 // Rows to other pages: a thread takes 16 (VEC) or 8 bytes of K and V of (row, column).
 template <int N>

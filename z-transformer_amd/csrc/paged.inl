@@ -78,55 +78,137 @@ static int paged_dp(int dim) {
 
 namespace {
 
-// Which kernel takes a sequence, by its rows per kv head (new tokens x heads of the group): the streaming
-// kernel with one or two 16-row blocks, or the split-operand one.
-enum class PagedKind { None, Few1, Few2, Many };
-constexpr PagedKind kPagedKinds[] = {PagedKind::Few1, PagedKind::Few2, PagedKind::Many};
+// Which kernel takes a sequence, by its rows per kv head (new tokens x heads of the group): the streaming kernel
+// with one or two 16-row blocks, or the split-operand one with 64, 128 or 256 rows in a workgroup.
+enum PagedKind { kFew1, kFew2, kMany64, kMany128, kMany256, kPagedKinds };
+constexpr bool paged_few(PagedKind k) { return k <= kFew2; }
+// Waves and 16-row blocks per wave of the split-operand kernel.
+struct PagedShape {
+    int nw, nq;
+};
+constexpr PagedShape paged_shape(PagedKind k, int dp) {
+    return k == kMany64 ? PagedShape{4, 1} : k == kMany256 ? PagedShape{8, 2} : dp <= 128 ? PagedShape{4, 2} : PagedShape{8, 1};
+}
 
 // What a call does for each sequence.
 struct PagedPlan {
     const int *q_start, *n_rows;
     int B, H, Hkv, G, dim, dp, part_ld;
-    int chunk_few, chunk_many;  // keys of a workgroup
-    int part_rows;              // rows of a part of the weights' sums (Many)
+    int most[kPagedKinds];  // units of keys (unit()) of a workgroup at most
+    int part_rows;          // rows of a part of the weights' sums
 
     int q_len(int b) const { return q_start[b + 1] - q_start[b]; }
     int rows(int b) const { return q_len(b) * G; }
+    bool any(int b) const { return q_len(b) > 0; }
     PagedKind kind(int b) const {
         const int r = rows(b);
-        return r == 0 ? PagedKind::None : r <= 16 ? PagedKind::Few1 : r <= 32 ? PagedKind::Few2 : PagedKind::Many;
+        return r <= 16 ? kFew1 : r <= 32 ? kFew2 : r <= 64 ? kMany64 : r <= 128 || dp > 128 ? kMany128 : kMany256;
     }
-    bool many(int b) const { return kind(b) == PagedKind::Many; }
-    int many_rows() const { return dp <= 128 ? 256 : 128; }     // of a workgroup
-    int weight_keys() const { return dp <= 128 ? 256 : 128; }   // of a workgroup of the weights' sums
-    int tiles(int b) const { return many(b) ? (rows(b) + many_rows() - 1) / many_rows() : 1; }
-    int chunk(int b) const { return many(b) ? chunk_many : chunk_few; }
-    int chunks(int b) const { return q_len(b) ? (n_rows[b] + chunk(b) - 1) / chunk(b) : 0; }
+    bool many(int b) const { return any(b) && !paged_few(kind(b)); }
+    // Rows of a workgroup, and the keys of its steps: a 16-key tile for each of four waves, or 32.
+    int tile_rows(PagedKind k) const { return k == kFew1 ? 16 : k == kFew2 ? 32 : 16 * paged_shape(k, dp).nw * paged_shape(k, dp).nq; }
+    static int unit(PagedKind k) { return paged_few(k) ? 64 : 32; }
+    int tiles(int b) const { return (rows(b) + tile_rows(kind(b)) - 1) / tile_rows(kind(b)); }
+    // Keys of a chunk: as few chunks as the limit allows, of one length.
+    static int chunk_of(int n_rows, int unit, int most) {
+        const int steps = (n_rows + unit - 1) / unit, n = (steps + most - 1) / most;
+        return (n > 1 ? (steps + n - 1) / n : steps) * unit;
+    }
+    int chunk(int b) const { return chunk_of(n_rows[b], unit(kind(b)), most[kind(b)]); }
+    int chunks(int b) const { return any(b) ? (n_rows[b] + chunk(b) - 1) / chunk(b) : 0; }
     long long items(int b) const { return (long long)tiles(b) * chunks(b) * Hkv; }
     long long slots(int b) const { return chunks(b) > 1 ? (long long)q_len(b) * H * chunks(b) : 0; }
     int kpad(int b) const { return (n_rows[b] + 15) / 16 * 16; }
+    // The weights' sums: waves of a workgroup (four, two workgroups to a CU, while LDS has room), and its keys.
+    int weight_waves() const { return dp <= 192 ? 4 : 8; }
+    int weight_keys() const { return 16 * weight_waves() * (dp <= 128 ? 2 : 1); }
     int parts(int b) const { return (rows(b) + part_rows - 1) / part_rows; }
     // Floats that the weights need: every row's scores, or the parts' sums.
     long long scores(int b) const { return (long long)kpad(b) * (many(b) ? (long long)Hkv * parts(b) : (long long)q_len(b) * H); }
 };
 
-PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
-    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, 0, 0, 0};
-    long long few = 0, many = 0, most = 0, sums = 0;  // steps of 16 and of 32 keys; row tiles x key tiles
-    for (int b = 0; b < B; ++b) {
-        if (p.many(b)) {
-            many += (long long)p.tiles(b) * Hkv * ((n_rows[b] + 31) / 32);
-            most = std::max(most, (long long)(n_rows[b] + 31) / 32);
-            sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
-        } else if (p.q_len(b)) {
-            few += (long long)Hkv * ((n_rows[b] + 15) / 16);
+// When the last workgroup of kind k ends, in steps, were `limit` the most steps of one: the kernel's order of
+// items, each to whichever of the device's places (`slots` workgroups) is free first, a workgroup's own
+// start and end counted as `extra` steps.  A kv head's items are alike, so that one head's stand for all
+// on its share of the places.  *items: how many, all heads.
+double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double extra, long long *items) {
+    const int unit = p.unit(k);
+    double busy[512] = {};  // when each place is free, as a heap
+    const int places = std::max(1, std::min(512, slots / p.Hkv));
+    double end = 0;
+    *items = 0;
+    for (int b = 0; b < p.B; ++b) {
+        if (!p.any(b) || p.kind(b) != k) continue;
+        const int c = p.chunk_of(p.n_rows[b], unit, limit) / unit, nt = p.tiles(b);
+        const int chunks = ((p.n_rows[b] + unit - 1) / unit + c - 1) / c;
+        for (int ci = 0; ci < chunks; ++ci) {
+            for (int t = nt - 1; t >= 0; --t) {
+                const int keys = p.n_rows[b] - p.q_len(b) + (std::min(p.rows(b), (t + 1) * p.tile_rows(k)) - 1) / p.G + 1;
+                const int left = (keys + unit - 1) / unit - ci * c;
+                if (left <= 0) break;  // nor have the tiles before it
+                const double at = busy[0] + std::min(left, c) + extra;
+                end = std::max(end, at);
+                *items += p.Hkv;
+                int i = 0;  // the first place takes it and sinks to where it belongs
+                for (int j = 1; j < places; j = 2 * i + 1) {
+                    if (j + 1 < places && busy[j + 1] < busy[j]) ++j;
+                    if (busy[j] >= at) break;
+                    busy[i] = busy[j];
+                    i = j;
+                }
+                busy[i] = at;
+            }
         }
     }
-    const long long f = std::max(8LL, (few + 1023) / 1024);
-    p.chunk_few = (int)std::min(16 * ((f + 3) / 4 * 4), 1LL << 30);  // whole rounds of four waves
-    const long long m = std::max(8LL, (many + 255) / 256);
-    p.chunk_many = (int)std::min(32 * m, 1LL << 30);
-    p.part_rows = (int)std::min(std::max(256LL, (sums / 512 + 31) / 32 * 32), 1LL << 30);
+    return end;
+}
+
+// Steps of a workgroup at most.  Keys are cut where whole row tiles would leave CUs idle or end unevenly: of
+// the whole and some cuts the one of the least estimated time (paged_span, and the partial sums' way to
+// memory and back: of the split-operand kernel 0.011 steps each, a step being RT x 32 keys at 216 TFLOP/s against 4.7
+// TB/s; of the streaming kernel's few rows next to nothing).  Measured on MI355X (us,
+// chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8 heads at d = 128 139 / 91, three chunks of
+// 501 on 1850 to 2980 rows at d = 96 470 / 240.
+int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
+    const int slots = k == kMany256 || (p.dp > 128 && k == kMany128) ? 256 : 512;  // two workgroups of four waves per CU
+    const double extra = paged_few(k) ? 1 : 3, way = paged_few(k) ? 0.0005 : 0.011;
+    const int least = paged_few(k) ? 2 : 4;
+    int best = longest;
+    long long items = 0;
+    double time = paged_span(p, k, longest, slots, extra, &items);
+    if (items >= 4 * slots) return best;
+    int last = longest;
+    for (const int cut : {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256}) {
+        const int limit = (longest + cut - 1) / cut;
+        if (limit < least || items > 4 * slots) break;
+        if (limit == last) continue;
+        last = limit;
+        const double t = paged_span(p, k, limit, slots, extra, &items) + 1 + way * items;
+        if (t < 0.98 * time) {
+            time = t;
+            best = limit;
+        }
+    }
+    return best;
+}
+
+PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
+    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0};
+    int longest[kPagedKinds] = {};
+    long long few = 0, sums = 0;
+    for (int b = 0; b < B; ++b) {
+        if (!p.any(b)) continue;
+        const PagedKind k = p.kind(b);
+        longest[k] = std::max(longest[k], (n_rows[b] + p.unit(k) - 1) / p.unit(k));
+        if (paged_few(k)) few += (long long)Hkv * ((n_rows[b] + 63) / 64);
+        else sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
+    }
+    const int wgs = tuned(kTunePagedWgs, 0);
+    for (int k = 0; k < kPagedKinds; ++k)
+        p.most[k] = !longest[k] ? 1
+                    : paged_few((PagedKind)k) && wgs ? (int)std::min<long long>(std::max(1LL, (few + wgs - 1) / wgs), 1 << 24)
+                                                     : paged_limit(p, (PagedKind)k, longest[k]);
+    p.part_rows = (int)std::min(std::max(256LL, (sums / 2048 + 31) / 32 * 32), 1LL << 30);
     return p;
 }
 
@@ -208,28 +290,31 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     const char *const any = dim == dp ? "" : "_any";
 
     // Launches `name` for the sequences that `items` has work items for, up to ZT_PAGED_MAXB at a time; per_wg items
-    // to a workgroup.  `each` fills in argument block x's entry i for sequence b.
+    // to a workgroup.  `each(i, b)` fills in what else argument block x needs for its entry i, sequence b; each(-1, b)
+    // comes behind every sequence.
     const auto launch_for = [&](const char *name, unsigned threads, unsigned per_wg, auto &x, auto items, auto each) -> int {
         long long blocks = 0;
-        x.ns = 0;
+        PagedSeqs &s = x.seq;
+        s.n = 0;
         const auto flush = [&]() -> int {
             const unsigned long long wgs = ((unsigned long long)blocks + per_wg - 1) / per_wg;
-            const bool bad = x.ns && (!grid_ok(wgs, threads) || launch(st, name, (unsigned)wgs, x, stream, threads));
-            x.ns = 0;
+            const bool bad = s.n && (!grid_ok(wgs, threads) || launch(st, name, (unsigned)wgs, x, stream, threads));
+            s.n = 0;
             blocks = 0;
             return bad;
         };
         for (int b = 0; b < B; ++b) {
             const long long n = items(b);
             if (n > 0) {
-                if ((x.ns == ZT_PAGED_MAXB || blocks + n > INT32_MAX) && flush()) return 1;
+                if ((s.n == ZT_PAGED_MAXB || blocks + n > INT32_MAX) && flush()) return 1;
                 if (n > INT32_MAX) {
                     grid_ok((unsigned long long)n, threads);  // says why
                     return 1;
                 }
-                const int i = x.ns++;
-                x.b[i] = b; x.q0[i] = q_start[b]; x.q_len[i] = p.q_len(b); x.n_rows[i] = n_rows[b];
-                x.first[i] = (int)blocks;
+                const int i = s.n++;
+                s.b[i] = b; s.q0[i] = q_start[b]; s.q_len[i] = p.q_len(b); s.n_rows[i] = n_rows[b];
+                s.first[i] = (int)blocks;
+                s.nch[i] = p.chunks(b); s.chunk[i] = p.chunk(b);
                 each(i, b);
                 blocks += n;
             }
@@ -238,10 +323,11 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         return flush();
     };
     char name[64];
-    for (const PagedKind kind : kPagedKinds) {
-        const bool many = kind == PagedKind::Many;
-        a.chunk = many ? p.chunk_many : p.chunk_few;
-        a.scores = weights && !many ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
+    for (int ki = 0; ki < kPagedKinds; ++ki) {
+        const PagedKind kind = (PagedKind)ki;
+        const bool few = paged_few(kind);
+        const PagedShape shape = paged_shape(kind, dp);
+        a.scores = weights && few ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
         long long part0 = 0, score0 = 0;
         const auto fill = [&](int i, int b) {
             if (i < 0) {
@@ -249,19 +335,20 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
                 score0 += p.scores(b);
                 return;
             }
-            a.nch[i] = p.chunks(b);
-            a.part0[i] = part0;
+            a.seq.at0[i] = part0;
             a.score0[i] = score0;
         };
-        const auto mine = [&](int b) { return p.kind(b) == kind; };
-        if (many) snprintf(name, sizeof name, "zt_paged_many_d%d_8%d%s", dp, dp <= 128 ? 2 : 1, any);
-        else snprintf(name, sizeof name, "zt_paged_few_d%d_n%d%s", dp, kind == PagedKind::Few1 ? 1 : 2, any);
-        if (launch_for(name, many ? 512u : 256u, 1, a, [&](int b) { return mine(b) ? p.items(b) : 0LL; }, fill)) return 1;
+        const auto mine = [&](int b) { return p.any(b) && p.kind(b) == kind; };
+        if (few) snprintf(name, sizeof name, "zt_paged_few_d%d_n%d%s", dp, kind == kFew1 ? 1 : 2, any);
+        else snprintf(name, sizeof name, "zt_paged_many_d%d_%d%d%s", dp, shape.nw, shape.nq, any);
+        const auto items = [&](int b) { return mine(b) ? p.items(b) : 0LL; };
+        if (launch_for(name, few ? 256u : 64u * shape.nw, 1, a, items, fill)) return 1;
         // Same stream: the merge reads the chunks' partials.
         part0 = score0 = 0;
-        snprintf(name, sizeof name, "zt_paged_merge_d%d", dp);
+        // Few rows of many chunks: a wave to a row; many rows of few: a lane group (256 threads hold 1024 floats).
+        snprintf(name, sizeof name, few ? "zt_paged_merge_d%d" : "zt_paged_merge_rows_d%d", dp);
         const auto merged = [&](int b) { return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads : 0LL; };
-        if (launch_for(name, 256u, 4, a, merged, fill)) return 1;
+        if (launch_for(name, 256u, few ? 4 : dp <= 32 ? 32 : dp <= 64 ? 16 : dp <= 128 ? 8 : 4, a, merged, fill)) return 1;
     }
     if (!weights) return 0;
     // ... and these the rows' statistics.
@@ -274,14 +361,14 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     long long score0 = 0;
     const auto fill = [&](int i, int b) {
         if (i < 0) score0 += p.scores(b);
-        else g.score0[i] = score0;
+        else g.seq.at0[i] = score0;
     };
     const auto per_head = [&](int b, int keys) { return (long long)((n_rows[b] + keys - 1) / keys) * n_kv_heads; };
     if (launch_for("zt_paged_weights", 256u, 1, g, [&](int b) { return p.many(b) ? 0LL : per_head(b, 1024); }, fill)) return 1;
     score0 = 0;
     snprintf(name, sizeof name, "zt_paged_wparts_d%d%s", dp, any);
     const auto parts = [&](int b) { return p.many(b) ? per_head(b, p.weight_keys()) * p.parts(b) : 0LL; };
-    if (launch_for(name, 512u, 1, g, parts, fill)) return 1;
+    if (launch_for(name, 64u * p.weight_waves(), 1, g, parts, fill)) return 1;
     score0 = 0;
     snprintf(name, sizeof name, "zt_paged_wsum_%d", p.weight_keys());
     return launch_for(name, 256u, 1, g, [&](int b) { return p.many(b) ? per_head(b, 256) : 0LL; }, fill);
@@ -323,7 +410,10 @@ int zt_paged_append(const float *q, const float *k_new, const float *v_new, floa
     a.q = q; a.k_new = k_new; a.v_new = v_new; a.q_out = q_out; a.w = w;
     a.H = n_heads; a.Hkv = n_kv_heads; a.dim = dim; a.w_stride = w_stride; a.theta = theta;
     const int per = std::min(16, 256 / (dim / 2));  // tokens of a workgroup
-    const long long tasks = ((q ? n_heads : 0) + 2LL * n_kv_heads) * (dim / 2);
+    const int vw = dim % 8 == 0 ? 4 : dim % 4 == 0 ? 2 : 1;  // pairs of a thread: both halves of a head in whole chunks of that
+    const long long tasks = ((q ? n_heads : 0) + 2LL * n_kv_heads) * (dim / 2) / vw;
+    char name[64];
+    snprintf(name, sizeof name, "zt_rope_paged_%d", vw);
     for (int b = 0; b < B;) {
         a.ns = 0;
         a.token0 = q_start[b];
@@ -338,7 +428,7 @@ int zt_paged_append(const float *q, const float *k_new, const float *v_new, floa
         const long long groups = (a.tokens + per - 1) / per;
         a.slices = (int)std::max(1LL, std::min(512 / groups, (std::min(a.tokens, per) * tasks + kThreads - 1) / kThreads));
         if (!grid_ok((unsigned long long)groups * a.slices)) return 1;
-        if (launch(st, "zt_rope_paged", (unsigned)(groups * a.slices), a, stream)) return 1;
+        if (launch(st, name, (unsigned)(groups * a.slices), a, stream)) return 1;
     }
     return 0;
 }
@@ -376,8 +466,12 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
             a.n_rows[i] = n_rows[b0 + i];
             most = std::max(most, a.n_rows[i]);
         }
-        if (!grid_ok((unsigned long long)a.ns * n_kv_heads, 1024)) return 1;
-        if (launch(st, "zt_evict_select", (unsigned)(a.ns * n_kv_heads), a, stream, 1024)) return 1;
+        // By the rows that a workgroup's registers hold.
+        const char *select = most <= 1024 ? "zt_evict_select_1024" : most <= 4096 ? "zt_evict_select_4096"
+                             : most <= 16384 ? "zt_evict_select_16384" : "zt_evict_select_any";
+        const unsigned threads = most <= 1024 ? 256 : most <= 4096 ? 512 : 1024;
+        if (!grid_ok((unsigned long long)a.ns * n_kv_heads, threads)) return 1;
+        if (launch(st, select, (unsigned)(a.ns * n_kv_heads), a, stream, threads)) return 1;
         // Same stream: the rows move as `kept` says.
         if (table_out == table) {
             if (most <= budget) continue;
