@@ -98,6 +98,23 @@ def test_attention_and_weights(gpu, zt, H, Hkv, d, page, batch):
     assert off <= 4 * EPS * (np.sqrt(d) + np.sqrt(n) + 16)
 
 
+@pytest.mark.parametrize("settings", [{"ZT_PAGED_SCORES": 0}, {"ZT_PAGED_SCORES": 1}, {"ZT_PAGED_WGS": 256},
+                                      {"ZT_PAGED_WGS": 32768}])
+@pytest.mark.parametrize("H,Hkv,d", [(4, 2, 32), (8, 8, 64), (8, 2, 96), (32, 8, 128), (6, 2, 50), (4, 1, 192), (8, 2, 256),
+                                     (3, 1, 250)])
+def test_forced_variants(gpu, zt, tune, settings, H, Hkv, d):
+    """Weights from kept scores and from scores formed again, and other splits of the keys."""
+    n_rows, q_len, page = [600, 90, 1300, 333], [300, 9, 1, 41], 16
+    rng = np.random.default_rng([H, d])
+    c = Cache(gpu, rng, n_rows, page, Hkv, d, garbage=np.nan)
+    q_start = np.cumsum([0] + q_len).tolist()
+    q = rng.standard_normal((q_start[-1], H, d)).astype(np.float32)
+    w = rng.random((4, Hkv, max(n_rows) + 5), np.float32)
+    ref = pagedref.attend(q, c.k_h, c.v_h, c.table_h, q_start, n_rows, page, H, Hkv, d)
+    tune(settings)
+    grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
+
+
 def test_more_sequences_than_a_launch_takes(gpu, zt):
     B, H, Hkv, d, page = 150, 4, 2, 32, 8
     rng = np.random.default_rng(5)

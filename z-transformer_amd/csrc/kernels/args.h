@@ -113,7 +113,8 @@ struct PagedArgs {
     float *part_acc;    // [slots, part_ld] partial outputs (sequences split into chunks)
     float *part_ml;     // [slots, 2] their base (log2 units) and sum
     float *stat;        // [N, H, 2] base m of each row and 1 / sum exp2(score - m), or null (no weights wanted)
-    float *scores;      // scaled scores (log2 units), or null: sequence i's at score0[i], [Hkv, rows, keys padded to 16]
+    float *scores;      // scaled scores (log2 units), or null: sequence i's at score0[i], the streaming kernel's
+                        // [Hkv, rows, keys padded to 16], the split-operand one's in 16 x 16 tiles [Hkv, row tile, key tile]
     int H, Hkv, G, dim;
     int part_ld;        // dim rounded up to whole 16 bytes
     float scale_log2e;
@@ -121,18 +122,20 @@ struct PagedArgs {
     long long score0[ZT_PAGED_MAXB];
 };
 
-// Accumulated weights: w_out = w_in + sum over the rows of exp2(score - m) / sum, from stored
-// scores (zt_paged_weights), or from q and k again, in parts of the rows (zt_paged_wparts_*) that zt_paged_wsum adds.
+// Accumulated weights: w_out = w_in + sum over the rows of exp2(score - m) / sum, from stored scores at once
+// (zt_paged_weights), or in parts of the rows from stored scores (zt_paged_wcols) or from q and k again
+// (zt_paged_wparts_*), which zt_paged_wsum_* adds.
 struct PagedWeightArgs {
     PagePool pool;
     const float *q, *scores, *stat;
     const float *w_in;  // [B, Hkv, w_stride]
     float *w_out;
-    float *parts;       // [Hkv, parts, keys padded to 16]
+    float *parts;       // sequence i's at parts0[i]: [Hkv, parts, keys padded to 16]
     int H, Hkv, G, dim, w_stride;
     int part_rows;      // rows of a part
     float scale_log2e;
-    PagedSeqs seq;      // at0: the sequence's scores or parts
+    PagedSeqs seq;      // at0: the sequence's scores
+    long long parts0[ZT_PAGED_MAXB];
 };
 
 // Append of new tokens to a paged cache, with RoPE on q and k.

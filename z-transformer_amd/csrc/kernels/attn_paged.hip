@@ -442,6 +442,15 @@ DEVI void paged_many(const PagedArgs &a) {
                     if (key > last[i % NQ] || key >= key1) s[i][r] = -INFINITY;
                 }
         }
+        if (a.scores) {  // kept for the weights: 16 x 16 tiles as the lanes hold them, 1 KB a store
+            const int ktiles = (sq.n_rows + 15) >> 4;
+            float *sp = a.scores + a.score0[sq.i] + 4 * lane +
+                        (((size_t)kvh * ((rows + 15) >> 4) + (row0 >> 4)) * ktiles + (k0 >> 4)) * 256;
+#pragma unroll
+            for (int i = 0; i < 2 * NQ; ++i)
+                if (row0 + 16 * (i % NQ) < rows && k0 + 16 * (i / NQ) < key1)  // wave-uniform
+                    __builtin_nontemporal_store(s[i], reinterpret_cast<f4 *>(sp + ((size_t)(i % NQ) * ktiles + i / NQ) * 256));
+        }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             float y[8];
@@ -790,8 +799,8 @@ DEVI void paged_merge(const PagedArgs &a) {
 // ---- Accumulated weights ---------------------------------------------------------------
 //
 // Few rows: from the scores that the attention stored.  A thread takes four keys of one
-// (sequence, kv head) and adds the weights of all rows, rows in order.  Sequences without
-// new tokens copy their weights.
+// (sequence, kv head) and adds the weights of all rows, in order.  Rows that do not see the keys are skipped
+// (their scores may not be written).  Sequences without new tokens copy their weights.
 extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightArgs a) {
     const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
     const int n = sq.n_rows, kpad = (n + 15) & ~15, rows = sq.q_len * a.G;
@@ -805,7 +814,7 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
     f4 sum = zero4();
     int t = 0, g = 0;
     for (int r = 0; r < rows; ++r) {
-        if (key <= seen0 + t) {  // else none of the four keys is seen (and the score may not be written)
+        if (key <= seen0 + t) {  // else none of the four keys is seen
             const f4 s = *reinterpret_cast<const f4 *>(sp + (size_t)r * kpad);
             const f2 ml = *reinterpret_cast<const f2 *>(st + 2 * ((size_t)t * a.H + g));
 #pragma unroll
@@ -819,7 +828,70 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
         if (key + e < n) a.w_out[at + e] = a.w_in[at + e] + sum[e];
 }
 
-// Many rows: the scores again, on split operands.  A workgroup takes one (sequence, kv
+// Many rows: from the tiles that the attention stored.  A workgroup takes 128 keys of one
+// (sequence, kv head) and a part of the rows; a wave two neighbouring key tiles, 2 KB a row tile, four row tiles in flight:
+// lane (l16, grp) adds row l16's weights of keys 4 grp .. 4 grp + 3 over the row tiles, and the 16 rows' lanes are added
+// at the end.  Bound: HBM, the scores read once.
+extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs a) {
+    const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
+    const int n = sq.n_rows, rows = sq.q_len * a.G, seen0 = n - sq.q_len, ktiles = (n + 15) >> 4;
+    const int nparts = (rows + a.part_rows - 1) / a.part_rows, ntiles = (n + 127) / 128;
+    int item = (int)blockIdx.x - sq.first;
+    const int kvh = item % a.Hkv;
+    item /= a.Hkv;
+    const int part = nparts - 1 - item / ntiles, kt0 = item % ntiles * 128;
+    if (max(0, kt0 - seen0) * a.G >= (part + 1) * a.part_rows) return;  // no row sees the keys; zt_paged_wsum does not read it
+    const int lane = lane_id(), l16 = lane & 15, grp = lane >> 4;
+    const int k0 = kt0 + 32 * __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (k0 >= n) return;
+    const int rt0 = max(part * a.part_rows, max(0, k0 - seen0) * a.G) >> 4, rt1 = (min(rows, (part + 1) * a.part_rows) + 15) >> 4;
+    const bool two = k0 + 16 < n;
+    const float *sp = a.scores + sq.at0 + 4 * lane + ((size_t)kvh * ((rows + 15) >> 4) * ktiles + (k0 >> 4)) * 256;
+    const float *st = a.stat + 2 * ((size_t)sq.q0 * a.H + kvh * a.G);
+    f4 sum[2] = {zero4(), zero4()};
+    for (int rt = rt0; rt < rt1; rt += 4) {
+        f4 s[4][2];
+        f2 ml[4];
+        int last[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = 16 * (rt + j) + l16, t = r / a.G;
+            const bool in = r < rows && rt + j < rt1;
+            last[j] = in ? seen0 + t : -1;
+            ml[j] = f2{0.f, 0.f};
+            if (in) ml[j] = *reinterpret_cast<const f2 *>(st + 2 * ((size_t)t * a.H + r - t * a.G));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                s[j][i] = zero4();
+                // Tiles that none of their rows sees are not written.
+                if (rt + j < rt1 && (i == 0 || two) && k0 + 16 * i <= seen0 + min(rows - 1, 16 * (rt + j) + 15) / a.G)
+                    s[j][i] = __builtin_nontemporal_load(
+                        reinterpret_cast<const f4 *>(sp + ((size_t)(rt + j) * ktiles + i) * 256));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int key = k0 + 16 * i + 4 * grp;
+            f4 four = zero4();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) four[e] += key + e <= last[j] ? fast_exp2(s[j][i][e] - ml[j].x) * ml[j].y : 0.f;
+            sum[i] += four;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[i][e] += wave_xor(sum[i][e], m);
+    if (l16 > 1 || (l16 == 1 && !two)) return;
+    *reinterpret_cast<f4 *>(a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * 16 * ktiles + k0 + 16 * l16 + 4 * grp) =
+        l16 ? sum[1] : sum[0];
+}
+
+// Many rows whose scores would take too much room: the scores again, on split operands.  A workgroup takes one (sequence, kv
 // head, tile of 16 NK NW keys, part of the rows); a wave holds 16 NK keys (K's parts in registers), and Q
 // passes through LDS in 32-row tiles, split once for all waves, two buffers, beside the rows'
 // statistics.  S = Q K^T has a key per lane and four rows, so that the sum over rows
@@ -1007,7 +1079,7 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
         __syncthreads();
     }
     const int kpad = (n + 15) & ~15;
-    float *out = a.parts + sq.at0 + ((size_t)kvh * nparts + part) * kpad;
+    float *out = a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * kpad;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
         const float sum = sum4grp(acc[i]);
@@ -1027,7 +1099,7 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
     const int kvh = item / per_head, key = (item % per_head) * 256 + (int)threadIdx.x;
     if (key >= n) return;
     const int from = max(0, key / KT * KT - (n - q_len)) * a.G / a.part_rows;  // the first part that saw the tile
-    const float *p = a.parts + sq.at0 + (size_t)kvh * nparts * kpad + key;
+    const float *p = a.parts + a.parts0[sq.i] + (size_t)kvh * nparts * kpad + key;
     float sum = 0.f;
     for (int i = from; i < nparts; ++i) sum += p[(size_t)i * kpad];
     const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;

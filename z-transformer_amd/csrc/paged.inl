@@ -96,6 +96,7 @@ struct PagedPlan {
     int B, H, Hkv, G, dim, dp, part_ld;
     int most[kPagedKinds];  // units of keys (unit()) of a workgroup at most
     int part_rows;          // rows of a part of the weights' sums
+    bool keep;              // the split-operand kernel stores its scores for the weights
 
     int q_len(int b) const { return q_start[b + 1] - q_start[b]; }
     int rows(int b) const { return q_len(b) * G; }
@@ -119,12 +120,16 @@ struct PagedPlan {
     long long items(int b) const { return (long long)tiles(b) * chunks(b) * Hkv; }
     long long slots(int b) const { return chunks(b) > 1 ? (long long)q_len(b) * H * chunks(b) : 0; }
     int kpad(int b) const { return (n_rows[b] + 15) / 16 * 16; }
-    // The weights' sums: waves of a workgroup (four, two workgroups to a CU, while LDS has room), and its keys.
+    // The weights' sums from scores formed again: waves of a workgroup (four, two workgroups to a CU, while LDS has
+    // room); and the keys of a workgroup, also of that which reads them.
     int weight_waves() const { return dp <= 192 ? 4 : 8; }
-    int weight_keys() const { return 16 * weight_waves() * (dp <= 128 ? 2 : 1); }
+    int weight_keys() const { return keep ? 128 : 16 * weight_waves() * (dp <= 128 ? 2 : 1); }
     int parts(int b) const { return (rows(b) + part_rows - 1) / part_rows; }
-    // Floats that the weights need: every row's scores, or the parts' sums.
-    long long scores(int b) const { return (long long)kpad(b) * (many(b) ? (long long)Hkv * parts(b) : (long long)q_len(b) * H); }
+    // Floats that the weights need: every row's scores, and the parts' sums.
+    long long scores(int b) const {
+        return (long long)kpad(b) * (many(b) ? keep ? (long long)Hkv * ((rows(b) + 15) / 16 * 16) : 0 : (long long)q_len(b) * H);
+    }
+    long long sums(int b) const { return many(b) ? (long long)Hkv * parts(b) * kpad(b) : 0; }
 };
 
 // When the last workgroup of kind k ends, in steps, were `limit` the most steps of one: the kernel's order of
@@ -193,40 +198,48 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
 }
 
 PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
-    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0};
+    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0, true};
     int longest[kPagedKinds] = {};
-    long long few = 0, sums = 0;
+    long long few = 0, scores = 0, sums = 0;
     for (int b = 0; b < B; ++b) {
         if (!p.any(b)) continue;
         const PagedKind k = p.kind(b);
         longest[k] = std::max(longest[k], (n_rows[b] + p.unit(k) - 1) / p.unit(k));
         if (paged_few(k)) few += (long long)Hkv * ((n_rows[b] + 63) / 64);
-        else sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
+        else scores += p.scores(b);
     }
+    // Scores that take more room than this (4 GiB: 32 heads of 4096 tokens over 8192 rows) are formed again instead.
+    // Measured on MI355X, the weights' kernels behind the attention: XXX
+    p.keep = tuned(kTunePagedScores, scores <= 1LL << 30) == 1;
+    for (int b = 0; b < B; ++b)
+        if (p.many(b)) sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
     const int wgs = tuned(kTunePagedWgs, 0);
     for (int k = 0; k < kPagedKinds; ++k)
         p.most[k] = !longest[k] ? 1
                     : paged_few((PagedKind)k) && wgs ? (int)std::min<long long>(std::max(1LL, (few + wgs - 1) / wgs), 1 << 24)
                                                      : paged_limit(p, (PagedKind)k, longest[k]);
+    // About 2048 workgroups, of 256 rows at least.
     p.part_rows = (int)std::min(std::max(256LL, (sums / 2048 + 31) / 32 * 32), 1LL << 30);
     return p;
 }
 
 // Offsets of a workspace's parts in bytes.
 struct PagedSpace {
-    size_t ml, stat, scores, bytes;
+    size_t ml, stat, scores, sums, bytes;
 };
 PagedSpace paged_space(const PagedPlan &p, bool weights) {
-    long long slots = 0, scores = 0;
+    long long slots = 0, scores = 0, sums = 0;
     for (int b = 0; b < p.B; ++b) {
         slots += p.slots(b);
         scores += p.scores(b);
+        sums += p.sums(b);
     }
     PagedSpace s{};
     s.ml = align256((size_t)slots * p.part_ld * sizeof(float));
     s.stat = s.ml + align256((size_t)slots * 2 * sizeof(float));
     s.scores = s.stat + (weights ? align256((size_t)p.q_start[p.B] * p.H * 2 * sizeof(float)) : 0);
-    s.bytes = s.scores + (weights ? (size_t)scores * sizeof(float) : 0);
+    s.sums = s.scores + (weights ? align256((size_t)scores * sizeof(float)) : 0);
+    s.bytes = s.sums + (weights ? (size_t)sums * sizeof(float) : 0);
     return s;
 }
 
@@ -327,7 +340,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         const PagedKind kind = (PagedKind)ki;
         const bool few = paged_few(kind);
         const PagedShape shape = paged_shape(kind, dp);
-        a.scores = weights && few ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
+        a.scores = weights && (few || p.keep) ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
         long long part0 = 0, score0 = 0;
         const auto fill = [&](int i, int b) {
             if (i < 0) {
@@ -354,24 +367,33 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     // ... and these the rows' statistics.
     PagedWeightArgs g{};
     g.pool = a.pool; g.q = q; g.stat = a.stat; g.w_in = w_in; g.w_out = w_out;
-    g.scores = g.parts = reinterpret_cast<float *>(ws + space.scores);
+    g.scores = reinterpret_cast<float *>(ws + space.scores);
+    g.parts = reinterpret_cast<float *>(ws + space.sums);
     g.H = n_heads; g.Hkv = n_kv_heads; g.G = p.G; g.dim = dim; g.w_stride = w_stride;
     g.part_rows = p.part_rows;
     g.scale_log2e = a.scale_log2e;
-    long long score0 = 0;
+    long long score0 = 0, parts0 = 0;
     const auto fill = [&](int i, int b) {
-        if (i < 0) score0 += p.scores(b);
-        else g.seq.at0[i] = score0;
+        if (i < 0) {
+            score0 += p.scores(b);
+            parts0 += p.sums(b);
+        } else {
+            g.seq.at0[i] = score0;
+            g.parts0[i] = parts0;
+        }
+    };
+    const auto run = [&](const char *kernel, unsigned threads, bool many, auto items) {
+        score0 = parts0 = 0;
+        return launch_for(kernel, threads, 1, g, [&](int b) { return p.many(b) == many ? items(b) : 0LL; }, fill);
     };
     const auto per_head = [&](int b, int keys) { return (long long)((n_rows[b] + keys - 1) / keys) * n_kv_heads; };
-    if (launch_for("zt_paged_weights", 256u, 1, g, [&](int b) { return p.many(b) ? 0LL : per_head(b, 1024); }, fill)) return 1;
-    score0 = 0;
-    snprintf(name, sizeof name, "zt_paged_wparts_d%d%s", dp, any);
-    const auto parts = [&](int b) { return p.many(b) ? per_head(b, p.weight_keys()) * p.parts(b) : 0LL; };
-    if (launch_for(name, 64u * p.weight_waves(), 1, g, parts, fill)) return 1;
-    score0 = 0;
+    if (run("zt_paged_weights", 256u, false, [&](int b) { return per_head(b, 1024); })) return 1;
+    if (p.keep) snprintf(name, sizeof name, "zt_paged_wcols");
+    else snprintf(name, sizeof name, "zt_paged_wparts_d%d%s", dp, any);
+    const auto parts = [&](int b) { return per_head(b, p.weight_keys()) * p.parts(b); };
+    if (run(name, p.keep ? 256u : 64u * p.weight_waves(), true, parts)) return 1;
     snprintf(name, sizeof name, "zt_paged_wsum_%d", p.weight_keys());
-    return launch_for(name, 256u, 1, g, [&](int b) { return p.many(b) ? per_head(b, 256) : 0LL; }, fill);
+    return run(name, 256u, true, [&](int b) { return per_head(b, 256); });
 }
 
 int zt_paged_append(const float *q, const float *k_new, const float *v_new, float *q_out, float *k_pages, float *v_pages,

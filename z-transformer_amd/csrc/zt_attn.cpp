@@ -172,7 +172,7 @@ int launch(DeviceState *st, const char *name, unsigned blocks, const Args &args,
 enum Tune {
     kTuneBK, kTuneFwdW, kTuneFPF, kTuneFPair, kTuneQPF, kTuneDqW, kTuneHS, kTuneW8, kTunePF, kTuneDMA, kTuneBPair,
     kTuneDSplit, kTuneRSplit, kTuneDecWgs, kTuneGemmTile, kTuneGemmSk, kTuneGemmSkTile, kTuneDqdsTile, kTuneRowG,
-    kTuneRowW, kTuneFKS, kTuneDqdsK, kTuneRScores, kTuneFShape, kTuneBShape, kTuneGemmSplit, kTunePagedWgs, kTuneCount
+    kTuneRowW, kTuneFKS, kTuneDqdsK, kTuneRScores, kTuneFShape, kTuneBShape, kTuneGemmSplit, kTunePagedWgs, kTunePagedScores, kTuneCount
 };
 struct TuneSpec {
     const char *name;
@@ -207,6 +207,7 @@ const TuneSpec kTuneSpecs[kTuneCount] = {
     {"ZT_ATTN_BSHAPE", {1, 2, 4}, 3},
     {"ZT_GEMM_SPLIT", {0, 1}, 2},
     {"ZT_PAGED_WGS", {256, 512, 768, 1024, 1536, 2048, 4096, 8192, 16384, 32768}, 10},
+    {"ZT_PAGED_SCORES", {0, 1}, 2},
 };
 std::atomic<int> g_tune[kTuneCount] = {};  // 0 = unset (no allowed value is 0 except a flag, stored as value + 1)
 
