@@ -720,27 +720,29 @@ DEVI void paged_many(const PagedArgs &a) {
 //
 // Of one (token, head): M = max_c m_c, out = sum_c acc_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).
 // LPR lanes cover a partial row with 16-byte loads.  ROWS false, for few rows of many
-// chunks: a wave takes a row, its lane groups 64 / LPR chunks at a time, and the groups are
-// merged in a fixed order; true, for many rows of few chunks: each lane group takes a row
-// (65536 rows of 3 chunks at d = 128: 43 us with a wave to a row).
+// chunks: a workgroup takes a row, each of its 256 / LPR lane groups eight chunks at a time
+// (64 chunks at d = 128 take one trip to memory), and the groups are merged in a fixed order; true, for many rows of
+// few chunks: each lane group takes a row (65536 rows of 3 chunks at d = 128: 43 us with a wave to a row, 21 so).
 template <int DP, bool ROWS>
 DEVI void paged_merge(const PagedArgs &a) {
-    constexpr int LPR = DP <= 32 ? 8 : DP <= 64 ? 16 : DP <= 128 ? 32 : 64, GR = ROWS ? 1 : 64 / LPR;
+    constexpr int LPR = DP <= 32 ? 8 : DP <= 64 ? 16 : DP <= 128 ? 32 : 64, GR = ROWS ? 1 : 256 / LPR;
     constexpr int U = ROWS ? 4 : 8;  // chunks of a lane group in flight
-    const int lane = lane_id(), g = ROWS ? 0 : lane / LPR, col = 4 * (lane % LPR);
-    const int per_wg = ROWS ? 256 / LPR : 4;
+    const int tid = threadIdx.x, g = ROWS ? 0 : tid / LPR, col = 4 * (tid % LPR);
+    const int per_wg = ROWS ? 256 / LPR : 1;
     const int item0 = (int)blockIdx.x * per_wg;
-    int item = item0 + (int)threadIdx.x / (256 / per_wg);
+    const int item = item0 + (ROWS ? tid / LPR : 0);
     const PagedSeq sq = paged_seq(a.seq, item0);
     // The workgroup's rows, if they are all of one sequence; else each lane group's own.
     int q_len = sq.q_len, n_rows = sq.n_rows, nslots = sq.nch, chunk = sq.chunk, q0 = sq.q0, i = item - sq.first;
     long long at0 = sq.at0;
-    int k = sq.i;
-    while (i >= q_len * a.H) {  // of a sequence behind it, or past the last's end
-        if (++k == a.seq.n) return;
-        i = item - a.seq.first[k];
-        q_len = a.seq.q_len[k]; n_rows = a.seq.n_rows[k]; nslots = a.seq.nch[k]; chunk = a.seq.chunk[k]; q0 = a.seq.q0[k];
-        at0 = a.seq.at0[k];
+    if constexpr (ROWS) {
+        int k = sq.i;
+        while (i >= q_len * a.H) {  // of a sequence behind it, or past the last's end
+            if (++k == a.seq.n) return;
+            i = item - a.seq.first[k];
+            q_len = a.seq.q_len[k]; n_rows = a.seq.n_rows[k]; nslots = a.seq.nch[k]; chunk = a.seq.chunk[k]; q0 = a.seq.q0[k];
+            at0 = a.seq.at0[k];
+        }
     }
     const int rows = q_len * a.G, t = i / a.H, h = i % a.H, kvh = h / a.G, r = t * a.G + h % a.G;
     const int nch = (n_rows - q_len + t) / chunk + 1;  // chunks that hold a key the token sees
@@ -750,12 +752,12 @@ DEVI void paged_merge(const PagedArgs &a) {
     const float *ml = a.part_ml + 2 * slot0;
     float M = -INFINITY, L = 0.f;
     f4 A = zero4();
-    for (int c0 = g; c0 < nch; c0 += U * GR) {
+    for (int c0 = U * g; c0 < nch; c0 += U * GR) {
         f2 e[U];
         f4 x[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int c = c0 + j * GR;
+            const int c = c0 + j;
             const bool in = c < nch;
             e[j] = in ? *reinterpret_cast<const f2 *>(ml + 2 * c) : f2{-INFINITY, 0.f};
             x[j] = in && ok ? *reinterpret_cast<const f4 *>(acc + (size_t)c * a.part_ld) : zero4();
@@ -775,22 +777,24 @@ DEVI void paged_merge(const PagedArgs &a) {
         M = mb;
     }
     if constexpr (!ROWS) {
-#pragma unroll
-        for (int d = LPR; d < 64; d <<= 1) {  // both sides of an exchange form the same sums
-            const float M2 = wave_xor(M, d), mb = fmaxf(M, M2);
-            const float f1 = M == -INFINITY ? 0.f : fast_exp2(M - mb), f2v = M2 == -INFINITY ? 0.f : fast_exp2(M2 - mb);
-            const bool up = lane & d;
-            const float la = L * f1, lb = wave_xor(L, d) * f2v;
-            L = up ? lb + la : la + lb;
-#pragma unroll
-            for (int k2 = 0; k2 < 4; ++k2) {
-                const float xa = A[k2] * f1, xb = wave_xor(A[k2], d) * f2v;
-                A[k2] = up ? xb + xa : xa + xb;
-            }
-            M = mb;
+        __shared__ f4 As[GR][LPR];
+        __shared__ f2 Ms[GR];
+        const int used = min(GR, (nch + U - 1) / U);  // groups that had a chunk
+        if (g < used) As[g][tid % LPR] = A;
+        if (g < used && tid % LPR == 0) Ms[g] = f2{M, L};
+        __syncthreads();
+        if (g != 0) return;
+        for (int x = 1; x < used; ++x) M = fmaxf(M, Ms[x].x);
+        L = 0.f;
+        A = zero4();
+        for (int x = 0; x < used; ++x) {
+            const f2 y = Ms[x];
+            const float f = y.x == -INFINITY ? 0.f : fast_exp2(y.x - M);
+            L += y.y * f;
+            A += As[x][tid % LPR] * f;
         }
     }
-    if (g != 0 || !ok) return;
+    if (!ok) return;
     const size_t row = (size_t)(q0 + t);
     if (col == 0) put_stats(a, row * a.H + h, M, L);
     store4(a.out + row * a.H * a.dim + (size_t)h * a.dim, col, a.dim, (a.dim & 3) == 0, A * (1.f / L));

@@ -168,16 +168,15 @@ double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double 
     return end;
 }
 
-// Steps of a workgroup at most.  Keys are cut where whole row tiles would leave CUs idle or end unevenly: of
+// Steps of a workgroup of the split-operand kernel at most.  Keys are cut where whole row tiles would leave CUs idle or end unevenly: of
 // the whole and some cuts the one of the least estimated time (paged_span, and the partial sums' way to
-// memory and back: of the split-operand kernel 0.011 steps each, a step being RT x 32 keys at 216 TFLOP/s against 4.7
-// TB/s; of the streaming kernel's few rows next to nothing).  Measured on MI355X (us,
+// memory and back: 0.011 steps each, a step being RT x 32 keys at 216 TFLOP/s against 4.7 TB/s).  Measured on MI355X (us,
 // chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8 heads at d = 128 139 / 91, three chunks of
 // 501 on 1850 to 2980 rows at d = 96 470 / 240.
 int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
     const int slots = k == kMany256 || (p.dp > 128 && k == kMany128) ? 256 : 512;  // two workgroups of four waves per CU
-    const double extra = paged_few(k) ? 1 : 3, way = paged_few(k) ? 0.0005 : 0.011;
-    const int least = paged_few(k) ? 2 : 4;
+    const double extra = 3, way = 0.011;
+    const int least = 4;
     int best = longest;
     long long items = 0;
     double time = paged_span(p, k, longest, slots, extra, &items);
@@ -197,27 +196,58 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
     return best;
 }
 
+// Units of a workgroup of the streaming kernel at most: the least time by the same reckoning, one unit for a
+// workgroup's own start and end, 512 workgroups at once.  Chunks are of one length within a sequence and not over all, so
+// that many workgroups count as an even share and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048
+// workgroups aimed at / this): XXX
+int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
+    const int wgs = tuned(kTunePagedWgs, 0);
+    int best = longest;
+    double time = 0;
+    for (int limit = 2; limit <= longest; limit += (limit + 3) / 4) {
+        long long n = 0, units = 0;
+        for (int b = 0; b < p.B; ++b) {
+            if (!p.any(b) || p.kind(b) != k) continue;
+            const int u = (p.n_rows[b] + 63) / 64;
+            n += (u + limit - 1) / limit;
+            units += u;
+        }
+        n *= p.Hkv;
+        units *= p.Hkv;
+        if (wgs) {  // forced
+            if (n <= wgs) return limit;
+            continue;
+        }
+        const double rounds = (double)((n + 511) / 512) * (limit + 1);
+        const double t = std::min(rounds, (double)(units + n) / 512 + 0.5 * (limit + 1));
+        if (limit == 2 || t < time) {
+            time = t;
+            best = limit;
+        }
+        if (n <= 512) break;  // fewer workgroups only take longer
+    }
+    return best;
+}
+
 PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
     PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0, true};
     int longest[kPagedKinds] = {};
-    long long few = 0, scores = 0, sums = 0;
+    long long scores = 0, sums = 0;
     for (int b = 0; b < B; ++b) {
         if (!p.any(b)) continue;
         const PagedKind k = p.kind(b);
         longest[k] = std::max(longest[k], (n_rows[b] + p.unit(k) - 1) / p.unit(k));
-        if (paged_few(k)) few += (long long)Hkv * ((n_rows[b] + 63) / 64);
-        else scores += p.scores(b);
+        if (!paged_few(k)) scores += p.scores(b);
+    }
+    for (int ki = 0; ki < kPagedKinds; ++ki) {
+        const PagedKind k = (PagedKind)ki;
+        p.most[k] = !longest[k] ? 1 : paged_few(k) ? paged_few_limit(p, k, longest[k]) : paged_limit(p, k, longest[k]);
     }
     // Scores that take more room than this (4 GiB: 32 heads of 4096 tokens over 8192 rows) are formed again instead.
     // Measured on MI355X, the weights' kernels behind the attention: XXX
     p.keep = tuned(kTunePagedScores, scores <= 1LL << 30) == 1;
     for (int b = 0; b < B; ++b)
         if (p.many(b)) sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
-    const int wgs = tuned(kTunePagedWgs, 0);
-    for (int k = 0; k < kPagedKinds; ++k)
-        p.most[k] = !longest[k] ? 1
-                    : paged_few((PagedKind)k) && wgs ? (int)std::min<long long>(std::max(1LL, (few + wgs - 1) / wgs), 1 << 24)
-                                                     : paged_limit(p, (PagedKind)k, longest[k]);
     // About 2048 workgroups, of 256 rows at least.
     p.part_rows = (int)std::min(std::max(256LL, (sums / 2048 + 31) / 32 * 32), 1LL << 30);
     return p;
@@ -358,10 +388,10 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         if (launch_for(name, few ? 256u : 64u * shape.nw, 1, a, items, fill)) return 1;
         // Same stream: the merge reads the chunks' partials.
         part0 = score0 = 0;
-        // Few rows of many chunks: a wave to a row; many rows of few: a lane group (256 threads hold 1024 floats).
+        // Few rows of many chunks: a workgroup to a row; many rows of few: a lane group.
         snprintf(name, sizeof name, few ? "zt_paged_merge_d%d" : "zt_paged_merge_rows_d%d", dp);
         const auto merged = [&](int b) { return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads : 0LL; };
-        if (launch_for(name, 256u, few ? 4 : dp <= 32 ? 32 : dp <= 64 ? 16 : dp <= 128 ? 8 : 4, a, merged, fill)) return 1;
+        if (launch_for(name, 256u, few ? 1 : dp <= 32 ? 32 : dp <= 64 ? 16 : dp <= 128 ? 8 : 4, a, merged, fill)) return 1;
     }
     if (!weights) return 0;
     // ... and these the rows' statistics.
