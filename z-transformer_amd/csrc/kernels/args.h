@@ -160,7 +160,6 @@ struct PagedEvictArgs {
     int *kept;           // [B, Hkv, budget]
     int Hkv, dim, w_stride, n_first, n_last, budget;
     int b0, ns;          // sequences b0 .. b0 + ns - 1
-    int slices;          // in place: column parts of a head's row
     int n_rows[ZT_PAGED_MAXB];
 };
 

@@ -527,10 +527,9 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
         // Same stream: the rows move as `kept` says.
         if (table_out == table) {
             if (most <= budget) continue;
-            const unsigned long long waves = (unsigned long long)a.ns * n_kv_heads * 2 * ((per_head + 7) / 8);
-            if (!grid_ok((waves + 3) / 4)) return 1;
-            if (launch(st, n == 4 ? "zt_evict_move_4" : "zt_evict_move_2", (unsigned)((waves + 3) / 4), a, stream))
-                return 1;
+            const unsigned long long blocks = (unsigned long long)a.ns * n_kv_heads * 2;  // K and V
+            if (!grid_ok(blocks, 1024)) return 1;
+            if (launch(st, n == 4 ? "zt_evict_move_4" : "zt_evict_move_2", (unsigned)blocks, a, stream, 1024)) return 1;
         } else {
             const int rows_per_wg = std::max(1, 1024 / (n_kv_heads * per_head));
             const unsigned long long blocks = (unsigned long long)a.ns * ((budget + rows_per_wg - 1) / rows_per_wg);
