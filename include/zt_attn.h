@@ -171,7 +171,8 @@ int zt_attn_decode_step(const float *q, const float *k_new, const float *v_new, 
  * k_pages/v_pages [n_pages, page_size, n_kv_heads*dim], page_size a power of two
  * in [1, 1024], n_pages * page_size < 2^31.  table [B, table_stride] (DEVICE
  * ints): row s of sequence b is row s % page_size of page table[b][s / page_size];
- * entries past a sequence's last page are not read.  Sequences may share pages
+ * entries past a sequence's last page are not read.  A sequence has at most 2^30
+ * rows, and its new tokens times n_heads are at most that.  Sequences may share pages
  * that are only read.  The kernels check every page number that they use: one
  * outside [0, n_pages) is never followed, its rows are not written, and an
  * output row that sees one comes out NaN.
@@ -183,8 +184,10 @@ int zt_attn_decode_step(const float *q, const float *k_new, const float *v_new, 
  * w [B, n_kv_heads, w_stride]: for each row and kv head the attention weight
  * that it has drawn so far, by sequence (not by page).  Keys are stored after
  * RoPE, so a row keeps its position when an eviction moves it.
- * The host arrays are read during the call; a captured call replays with the
- * lengths it was captured with.  Calls whose outputs do not overlap may run at the
+ * Outputs do not overlap inputs, or one another, except where it is said.  The
+ * host arrays are read during the call; a captured call replays with the lengths
+ * it was captured with (make a call of the kind before capturing one: the first
+ * loads the kernels).  Calls whose outputs do not overlap may run at the
  * same time on different streams, each with a workspace of its own.
  *
  * zt_paged_append: q_out = RoPE(q), K row = RoPE(k_new), V row = v_new (as
@@ -413,7 +416,10 @@ int zt_attn_plan(int B, int T, int n_heads, int n_kv_heads, int dim, int max_til
  *   hold falls back to one it does), ZT_ATTN_BSHAPE 1|2|4 (16-key blocks per
  *   workgroup of the score-reading dk/dv kernel, head_dim <= 128), ZT_GEMM_SPLIT
  *   0|1 (the f32 or split-operand form of a dense product's slab tile; a form
- *   the tile does not have falls back to the one it has).
+ *   the tile does not have falls back to the one it has), ZT_PAGED_WGS 256..32768
+ *   (workgroup target of the paged attention with at most 32 rows of a kv head),
+ *   ZT_PAGED_SCORES 0|1 (its weights for more rows from scores formed again or kept;
+ *   both change what zt_attn_paged_workspace returns).
  * Returns 0, or 1 (reason on stderr) for an unknown name or value.  The
  * process environment is never read.  Not synchronised with launches in
  * flight on other threads: set before launching. */

@@ -153,6 +153,89 @@ def test_what_a_token_does_not_see_changes_nothing(gpu, zt, H, Hkv, d, L, n, val
     assert np.all(np.isnan(out2[-1])) and np.all(np.isnan(lse2[-1]))
 
 
+@pytest.mark.parametrize("scores", [0, 1])
+@pytest.mark.parametrize("L", [5, 40, 150])
+@pytest.mark.parametrize("where", ["k", "q", "both", "v"])
+@pytest.mark.parametrize("H,Hkv,d", [(8, 2, 64), (8, 2, 128), (4, 1, 256), (6, 2, 50)])
+def test_large_values(gpu, zt, tune, H, Hkv, d, where, L, scores):
+    """Values past 2^40 (kept out of the split products and added from the full rows): in K against as small ones in Q,
+    the other way round, both, and in V."""
+    n, page = 220, 16
+    rng = np.random.default_rng([H, d, L])
+    c = Cache(gpu, rng, [n], page, Hkv, d)
+    q = rng.standard_normal((L, H, d)).astype(np.float32)
+    big, some = np.float32(2.0 ** 45), rng.random(c.k_h.shape[0]) < 0.1
+    if where in ("k", "both"):
+        c.k_h[some, :, 5] *= big
+        q[:, :, 5] /= big
+    if where in ("q", "both"):
+        q[::3, :, d - 2] *= big
+        c.k_h[:, :, d - 2] /= big
+    if where == "v":
+        c.v_h[some, :, 7] *= big
+    c.k, c.v = gpu.from_numpy(c.k_h).cuda(), gpu.from_numpy(c.v_h).cuda()
+    w = rng.random((1, Hkv, n), np.float32)
+    ref = pagedref.attend(q, c.k_h, c.v_h, c.table_h, [0, L], [n], page, H, Hkv, d)
+    tune({"ZT_PAGED_SCORES": scores})
+    grade(run_attend(gpu, zt, c, q, [0, L], H, w), ref, [0, L], [n], Hkv, w)
+
+
+def test_no_new_tokens(gpu, zt):
+    """Weights are copied, nothing else happens; no tokens and no weights: nothing at all."""
+    H, Hkv, d, page, n_rows = 4, 2, 32, 8, [30, 0, 2000]
+    rng = np.random.default_rng(31)
+    c = Cache(gpu, rng, n_rows, page, Hkv, d)
+    w = rng.random((3, Hkv, 2001), np.float32)
+    out, lse, got = run_attend(gpu, zt, c, np.zeros((2, H, d)), [1, 1, 1, 1], H, w)
+    assert np.all(np.isnan(out)) and np.all(np.isnan(lse))
+    for b, n in enumerate(n_rows):
+        assert np.array_equal(got[b, :, :n], w[b, :, :n]) and np.all(got[b, :, n:] == -7.0)
+    out, lse, _ = run_attend(gpu, zt, c, np.zeros((2, H, d)), [1, 1, 1, 1], H)
+    assert np.all(np.isnan(out)) and np.all(np.isnan(lse))
+    k, before = gpu.zeros(1, Hkv * d, device="cuda"), c.k.clone()
+    zt.paged_append(None, k, k, None, c.k, c.v, c.table, [1, 1, 1, 1], n_rows, [0, 0, 0], page, H, Hkv, d)
+    assert gpu.equal(c.k, before)
+
+
+def test_the_binding_checks_what_the_library_cannot_see(gpu, zt):
+    H, Hkv, d, page = 4, 2, 32, 8
+    c = Cache(gpu, np.random.default_rng(32), [30], page, Hkv, d)
+    q, w = gpu.zeros(3, H * d, device="cuda"), gpu.zeros(1, Hkv, 30, device="cuda")
+    kept = gpu.empty(1, Hkv, 8, device="cuda", dtype=gpu.int32)
+    for bad in (dict(q=q[:2].contiguous()), dict(out=q[:2].contiguous()), dict(w_in=w, w_out=w[:, :1].contiguous()),
+                dict(v=c.v[:-1].contiguous()), dict(table=c.table.long()), dict(q_start=[0, 1, 3])):
+        a = dict(q=q, out=gpu.empty_like(q), v=c.v, table=c.table, q_start=[0, 3], w_in=None, w_out=None)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            zt.attn_paged(a["q"], c.k, a["v"], a["table"], a["out"], a["q_start"], [30], page, H, Hkv, d, None, None,
+                          a["w_in"], a["w_out"])
+    with pytest.raises(zt.ZtRefused):  # a null w_in beside a w_out
+        zt.attn_paged(q, c.k, c.v, c.table, gpu.empty_like(q), [0, 3], [30], page, H, Hkv, d, None, None, None, w)
+    with pytest.raises(ValueError):
+        zt.paged_append(None, q, q, None, c.k, c.v, c.table, [0, 30], [30], [0], page, H, Hkv, d)
+    with pytest.raises(ValueError):
+        zt.paged_evict(c.k, c.v, c.table, c.table, w, w, kept, [30], page, Hkv, d, 1, 1, 9)
+
+
+def test_sequences_that_share_pages(gpu, zt):
+    """Three sequences over one prefix, the third the first again."""
+    H, Hkv, d, page = 8, 2, 64, 16
+    rng = np.random.default_rng(21)
+    n_rows, q_len = [100, 90, 100], [3, 40, 3]
+    c = Cache(gpu, rng, n_rows, page, Hkv, d)
+    c.table_h[1, :5] = c.table_h[0, :5]
+    c.table_h[2] = c.table_h[0]
+    c.table = gpu.from_numpy(c.table_h).cuda()
+    q_start = np.cumsum([0] + q_len).tolist()
+    q = rng.standard_normal((q_start[-1], H, d)).astype(np.float32)
+    q[-3:] = q[:3]
+    w = np.repeat(rng.random((1, Hkv, 100), np.float32), 3, 0)
+    ref = pagedref.attend(q, c.k_h, c.v_h, c.table_h, q_start, n_rows, page, H, Hkv, d)
+    got = run_attend(gpu, zt, c, q, q_start, H, w)
+    grade(got, ref, q_start, n_rows, Hkv, w)
+    assert np.array_equal(got[0][:3], got[0][-3:]) and np.array_equal(got[2][0], got[2][2])
+
+
 @pytest.mark.parametrize("bad", [-1, 10 ** 9, "n_pages"])
 @pytest.mark.parametrize("L", [6, 80])
 def test_a_page_of_no_pool_is_not_followed(gpu, zt, bad, L):

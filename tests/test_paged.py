@@ -36,10 +36,12 @@ def evict(L, n_rows=(5, 9), B=2, n_pages=8, page=4, stride=4, w_stride=9, Hkv=2,
 GEOMETRY = [(dict(B=0), "not launchable"), (dict(n_pages=0), "not launchable"), (dict(stride=0), "not launchable"),
             (dict(page=0), "power of two"), (dict(page=3), "power of two"), (dict(page=2048), "power of two"),
             (dict(page=-4), "power of two"), (dict(n_pages=1 << 21, page=1024), "2^31 - 1"),
-            (dict(n_rows=(5, 17)), "outside [0, 16]"), (dict(n_rows=(-1, 9)), "outside [0, 16]"),
+            (dict(n_rows=(5, 17)), "outside [0, 16]"),
+            (dict(n_rows=(5, (1 << 30) + 1), stride=1 << 21, page=1024), "outside [0, 1073741824]"), (dict(n_rows=(-1, 9)), "outside [0, 16]"),
             (dict(d=33), "head_dim"), (dict(d=300), "head_dim"), (dict(Hkv=0), "not a group")]
 TOKENS = [(dict(q_start=(-1, 1, 3)), "q_start"), (dict(q_start=(0, 2, 1)), "new tokens"),
-          (dict(q_start=(0, 6, 7)), "new tokens"), (dict(H=3), "not a group"), (dict(H=1 << 17), "65535")]
+          (dict(q_start=(0, 6, 7)), "new tokens"),
+          (dict(n_rows=(5, 1 << 20), stride=1 << 20, q_start=(0, 1, 1 + (1 << 20)), H=1 << 11), "new tokens"), (dict(H=3), "not a group"), (dict(H=1 << 17), "65535")]
 
 
 @pytest.mark.parametrize("bad,reason", GEOMETRY + TOKENS + [
@@ -65,7 +67,7 @@ def test_append_refuses(zt, capfd, bad, reason):
 
 
 @pytest.mark.parametrize("bad,reason", GEOMETRY + [
-    (dict(budget=0), "budget"), (dict(first=-1), "budget"), (dict(last=-1), "budget"), (dict(first=3, last=2), "budget"),
+    (dict(budget=0), "budget"), (dict(budget=(1 << 30) + 1), "budget"), (dict(first=-1), "budget"), (dict(last=-1), "budget"), (dict(first=3, last=2), "budget"),
     (dict(first=2 ** 31 - 1, last=2 ** 31 - 1), "budget"), (dict(w_stride=8), "accumulated weights"),
     (dict(k=None), "null"), (dict(v=None), "null"), (dict(table=None), "null"), (dict(table_out=None), "null"),
     (dict(w_in=None), "null"), (dict(w_out=None), "null"), (dict(kept=None), "null"),

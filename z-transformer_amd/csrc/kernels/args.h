@@ -160,6 +160,7 @@ struct PagedEvictArgs {
     int *kept;           // [B, Hkv, budget]
     int Hkv, dim, w_stride, n_first, n_last, budget;
     int b0, ns;          // sequences b0 .. b0 + ns - 1
+    int tiles;           // row tiles of a sequence (to other pages)
     int n_rows[ZT_PAGED_MAXB];
 };
 

@@ -208,13 +208,14 @@ ZT_EVICT_SELECT(4096, 8, 8)
 ZT_EVICT_SELECT(16384, 16, 16)
 ZT_EVICT_SELECT(any, 16, 0)
 
-// Rows to other pages: a thread takes 16 (VEC) or 8 bytes of K and V of (row, column).
+// Rows to other pages: a thread takes 4 N bytes of K and V at a time.  Bound: HBM, a copy (16 sequences of 8192 rows to 4096,
+// 8 kv heads at d = 128, 220 us: 4.7 TB/s, as a copy of 4 GiB).
 template <int N>
 DEVI void evict_copy(const PagedEvictArgs &a) {
     typedef float vec __attribute__((ext_vector_type(N)));
     const int per_head = a.dim / N, per_row = a.Hkv * per_head;
-    const int rows_per_wg = max(1, 1024 / per_row), tiles = (a.budget + rows_per_wg - 1) / rows_per_wg;
-    const int sl = (int)blockIdx.x / tiles, r0 = (int)blockIdx.x % tiles * rows_per_wg, b = a.b0 + sl;
+    const int rows_per_wg = max(1, 1024 / per_row);
+    const int sl = (int)blockIdx.x / a.tiles, r0 = (int)blockIdx.x % a.tiles * rows_per_wg, b = a.b0 + sl;
     const int r1 = min(min(a.budget, a.n_rows[sl]), r0 + rows_per_wg);
     const size_t kld = (size_t)a.Hkv * a.dim;
     const int *from = a.pool.table + (size_t)b * a.pool.table_stride, *to = a.table_out + (size_t)b * a.pool.table_stride;

@@ -5,6 +5,9 @@
 // follows from the host's lengths alone, so that a workspace's size does not depend
 // on the device.
 
+// Rows of a sequence, tokens x heads of one, rows of a budget: no sum of two overflows an int.
+constexpr long long kPagedMost = 1LL << 30;
+
 // The cache's geometry; 0 when usable.
 static int paged_check(const char *who, const int *n_rows, int B, int n_pages, int page_size, int table_stride) {
     if (B < 1 || n_pages < 1 || table_stride < 1) {
@@ -25,10 +28,10 @@ static int paged_check(const char *who, const int *n_rows, int B, int n_pages, i
         fprintf(stderr, "zt_attn: %s needs the host n_rows array.\n", who);
         return 1;
     }
+    const long long most = std::min((long long)table_stride * page_size, kPagedMost);
     for (int b = 0; b < B; ++b) {
-        if (n_rows[b] < 0 || n_rows[b] > (long long)table_stride * page_size) {
-            fprintf(stderr, "zt_attn: sequence %d has n_rows %d, outside [0, %lld].\n", b, n_rows[b],
-                    (long long)table_stride * page_size);
+        if (n_rows[b] < 0 || n_rows[b] > most) {
+            fprintf(stderr, "zt_attn: sequence %d has n_rows %d, outside [0, %lld].\n", b, n_rows[b], most);
             return 1;
         }
     }
@@ -43,7 +46,7 @@ static int paged_tokens_check(const char *who, const int *q_start, const int *n_
     }
     for (int b = 0; b < B; ++b) {
         const long long q_len = (long long)q_start[b + 1] - q_start[b];
-        if (q_len < 0 || q_len > n_rows[b] || q_len * n_heads > INT32_MAX) {
+        if (q_len < 0 || q_len > n_rows[b] || q_len * n_heads > kPagedMost) {
             fprintf(stderr, "zt_attn: sequence %d has %lld new tokens among its %d rows.\n", b, q_len, n_rows[b]);
             return 1;
         }
@@ -199,7 +202,9 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
 // Units of a workgroup of the streaming kernel at most: the least time by the same reckoning, one unit for a
 // workgroup's own start and end, 512 workgroups at once.  Chunks are of one length within a sequence and not over all, so
 // that many workgroups count as an even share and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048
-// workgroups aimed at / this): XXX
+// workgroups aimed at / this): 64 sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128 544 / 557 / 516 / 499, 16 of
+// half that with weights 91 / 89 / 93 / 89, 3 of 6000 rows with 8 tokens each 52 / 65 / 66 / 52, one of 100000 rows 159 /
+// 151 / 140 / 144.  (Chunks of 64 keys: 16 over 4 heads of 8192 rows at d = 256 40 instead of 32.)
 int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
     const int wgs = tuned(kTunePagedWgs, 0);
     int best = longest;
@@ -243,9 +248,11 @@ PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hk
         const PagedKind k = (PagedKind)ki;
         p.most[k] = !longest[k] ? 1 : paged_few(k) ? paged_few_limit(p, k, longest[k]) : paged_limit(p, k, longest[k]);
     }
-    // Scores that take more room than this (4 GiB: 32 heads of 4096 tokens over 8192 rows) are formed again instead.
-    // Measured on MI355X, the weights' kernels behind the attention: XXX
-    p.keep = tuned(kTunePagedScores, scores <= 1LL << 30) == 1;
+    // The split-operand kernel's scores are kept for the weights from d = 64 up while they take no more room than 4
+    // GiB (32 heads of 4096 tokens over 8192 rows), else formed again.  Measured on MI355X (attention and weights,
+    // us, kept / again): a prompt of 2048 rows of 32 over 8 heads at d = 128 340 / 392, 64 tokens on 4096 rows 66 / 80, 2048 rows of
+    // 16 over 4 at d = 256 364 / 482, 4 x 1024 of 8 heads at d = 64 96 / 95; 4096 rows of 4 over 2 at d = 32 165 / 144.
+    p.keep = tuned(kTunePagedScores, p.dp >= 64 && scores <= 1LL << 30) == 1;
     for (int b = 0; b < B; ++b)
         if (p.many(b)) sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
     // About 2048 workgroups, of 256 rows at least.
@@ -282,7 +289,7 @@ size_t zt_attn_paged_workspace(const int *q_start, const int *n_rows, int B, int
         return 0;
     for (int b = 0; b < B; ++b) {
         const long long q_len = (long long)q_start[b + 1] - q_start[b];
-        if (n_rows[b] < 0 || q_len < 0 || q_len > n_rows[b] || q_len * n_heads > INT32_MAX) return 0;
+        if (n_rows[b] < 0 || n_rows[b] > kPagedMost || q_len < 0 || q_len > n_rows[b] || q_len * n_heads > kPagedMost) return 0;
     }
     return paged_space(paged_plan(q_start, n_rows, B, n_heads, n_kv_heads, dim), weights != 0).bytes;
 }
@@ -336,6 +343,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     // to a workgroup.  `each(i, b)` fills in what else argument block x needs for its entry i, sequence b; each(-1, b)
     // comes behind every sequence.
     const auto launch_for = [&](const char *name, unsigned threads, unsigned per_wg, auto &x, auto items, auto each) -> int {
+        const long long most = 0xFFFFFFFFll / threads * per_wg;  // items whose work-items fit a grid
         long long blocks = 0;
         PagedSeqs &s = x.seq;
         s.n = 0;
@@ -349,11 +357,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         for (int b = 0; b < B; ++b) {
             const long long n = items(b);
             if (n > 0) {
-                if ((s.n == ZT_PAGED_MAXB || blocks + n > INT32_MAX) && flush()) return 1;
-                if (n > INT32_MAX) {
-                    grid_ok((unsigned long long)n, threads);  // says why
-                    return 1;
-                }
+                if ((s.n == ZT_PAGED_MAXB || blocks + n > most) && flush()) return 1;
+                if (n > most) return !grid_ok((unsigned long long)n, threads);  // (which says why)
                 const int i = s.n++;
                 s.b[i] = b; s.q0[i] = q_start[b]; s.q_len[i] = p.q_len(b); s.n_rows[i] = n_rows[b];
                 s.first[i] = (int)blocks;
@@ -491,7 +496,7 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
     if (paged_check("paged_evict", n_rows, B, n_pages, page_size, table_stride)) return 1;
     if (!zt_attn_dim_ok(dim)) return refuse_dim(dim);
     if (check_group(n_kv_heads, n_kv_heads)) return 1;
-    if (n_first < 0 || n_last < 0 || budget < 1 || n_first > budget - n_last) {
+    if (n_first < 0 || n_last < 0 || budget < 1 || budget > kPagedMost || n_first > budget - n_last) {
         fprintf(stderr, "zt_attn: a budget of %d rows with the first %d and the last %d kept is not usable.\n", budget,
                 n_first, n_last);
         return 1;
@@ -532,7 +537,9 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
             if (launch(st, n == 4 ? "zt_evict_move_4" : "zt_evict_move_2", (unsigned)blocks, a, stream, 1024)) return 1;
         } else {
             const int rows_per_wg = std::max(1, 1024 / (n_kv_heads * per_head));
-            const unsigned long long blocks = (unsigned long long)a.ns * ((budget + rows_per_wg - 1) / rows_per_wg);
+            a.tiles = (std::min(budget, most) + rows_per_wg - 1) / rows_per_wg;
+            const unsigned long long blocks = (unsigned long long)a.ns * a.tiles;
+            if (most == 0) continue;
             if (!grid_ok(blocks)) return 1;
             if (launch(st, n == 4 ? "zt_evict_copy_4" : "zt_evict_copy_2", (unsigned)blocks, a, stream)) return 1;
         }

@@ -302,10 +302,31 @@ def _i32_cuda(*ts):
             raise ValueError("page tables and row numbers must be contiguous int32 on the GPU")
 
 
+def _here(*ts):
+    """The launches go to the current device."""
+    import torch
+    for t in ts:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise ValueError("tensors must be on the current device")
+
+
 def _host_ints(xs, n):
     if len(xs) != n:
         raise ValueError(f"{len(xs)} lengths where {n} are needed")
     return (ctypes.c_int * n)(*[int(x) for x in xs])
+
+
+def _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages, rows, w, B):
+    """What the C side cannot see: that the tensors are as long as the lengths say.  Returns n_pages."""
+    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    if v_pages.numel() != k_pages.numel() or n_pages * page_size * n_kv_heads * dim != k_pages.numel():
+        raise ValueError("k_pages and v_pages are [n_pages, page_size, n_kv_heads * dim]")
+    for t, per_token in rows:
+        if t is not None and t.numel() < int(q_start[-1]) * per_token:
+            raise ValueError(f"{t.numel()} values where {int(q_start[-1])} tokens have {per_token} each")
+    if w is not None and (w.dim() != 3 or tuple(w.shape[:2]) != (B, n_kv_heads)):
+        raise ValueError("accumulated weights are [B, n_kv_heads, rows]")
+    return n_pages
 
 
 def paged_append(q, k_new, v_new, q_out, k_pages, v_pages, table, q_start, n_rows, pos, page_size, n_heads, n_kv_heads,
@@ -314,8 +335,11 @@ def paged_append(q, k_new, v_new, q_out, k_pages, v_pages, table, q_start, n_row
     q and q_out may both be None."""
     _f32_cuda(k_new, v_new, k_pages, v_pages, *[t for t in (q, q_out, w) if t is not None])
     _i32_cuda(table)
+    _here(q, k_new, v_new, q_out, k_pages, v_pages, table, w)
     B, table_stride = table.shape
-    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    n_pages = _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages,
+                            [(q, n_heads * dim), (q_out, n_heads * dim), (k_new, n_kv_heads * dim),
+                             (v_new, n_kv_heads * dim)], w, B)
     _check(lib().zt_paged_append(*map(_ptr, (q, k_new, v_new, q_out, k_pages, v_pages, table, w)),
                                  _host_ints(q_start, B + 1), _host_ints(n_rows, B), _host_ints(pos, B), B, n_pages,
                                  page_size, table_stride, 0 if w is None else w.shape[-1], n_heads, n_kv_heads, dim,
@@ -333,10 +357,12 @@ def attn_paged(q, k_pages, v_pages, table, out, q_start, n_rows, page_size, n_he
     """workspace: a tensor of attn_paged_workspace_bytes(...) bytes, or None where that is 0."""
     _f32_cuda(q, k_pages, v_pages, out, *[t for t in (lse, w_in, w_out) if t is not None])
     _i32_cuda(table)
+    _here(q, k_pages, v_pages, table, out, workspace, lse, w_in, w_out)
     if w_in is not None and w_out is not None and w_in.shape != w_out.shape:
         raise ValueError("w_in and w_out have the same shape")
     B, table_stride = table.shape
-    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    n_pages = _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages,
+                            [(q, n_heads * dim), (out, n_heads * dim), (lse, n_heads)], w_out, B)
     nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _check(lib().zt_attn_paged(*map(_ptr, (q, k_pages, v_pages, table, out, lse, w_in, w_out)),
                                _host_ints(q_start, B + 1), _host_ints(n_rows, B), B, n_pages, page_size, table_stride,
@@ -349,10 +375,11 @@ def paged_evict(k_pages, v_pages, table, table_out, w_in, w_out, kept, n_rows, p
     """kept [B, n_kv_heads, budget] int32; table_out is table (in place) or a table of other pages."""
     _f32_cuda(k_pages, v_pages, w_in, w_out)
     _i32_cuda(table, table_out, kept)
+    _here(k_pages, v_pages, table, table_out, w_in, w_out, kept)
     B, table_stride = table.shape
     if table_out.shape != table.shape or w_in.shape != w_out.shape or kept.numel() != B * n_kv_heads * budget:
         raise ValueError("table and table_out, and w_in and w_out, have one shape; kept is [B, n_kv_heads, budget]")
-    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
+    n_pages = _paged_shapes((0,), n_kv_heads, dim, page_size, k_pages, v_pages, [], w_in, B)
     _check(lib().zt_paged_evict(*map(_ptr, (k_pages, v_pages, table, table_out, w_in, w_out, kept)),
                                 _host_ints(n_rows, B), B, n_pages, page_size, table_stride, w_in.shape[-1], n_kv_heads,
                                 dim, n_first, n_last, budget, _stream(stream)), "zt_paged_evict")
