@@ -217,6 +217,7 @@ DEVI void paged_few(const PagedArgs &a) {
                 for (int n = 0; n < NQ; ++n) o[n][i] = mfma16(vx[r][i / C][i % C], s[n][r], o[n][i]);
         if (odd_v) {
             // The lane's columns of the key's V row, the weight from the lane group that holds it.
+            const int ll = opaque(lane), lcol = ll & 15, lgrp = ll >> 4;
 #pragma unroll 1
             for (int key = 0; key < 16; ++key) {
                 const int vr = key & 2 ? (key & 1 ? vrow[3] : vrow[2]) : (key & 1 ? vrow[1] : vrow[0]);
@@ -225,14 +226,14 @@ DEVI void paged_few(const PagedArgs &a) {
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
                     const float sr = key & 2 ? (key & 1 ? s[n][3] : s[n][2]) : (key & 1 ? s[n][1] : s[n][0]);
-                    const float pk = __shfl(sr, 16 * (key >> 2) + l16, 64);
+                    const float pk = __shfl(sr, 16 * (key >> 2) + lcol, 64);
                     const bool sees = k0 + key <= last[n] && k0 + key < key1;
 #pragma unroll
                     for (int i = 0; i < NT; ++i)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const int col = i / C * 16 * C + C * (4 * grp + r) + i % C;
-                            if (!sees || col >= a.dim) continue;
+                            const int col = i / C * 16 * C + C * (4 * lgrp + r) + i % C;
+                            if (!sees || (!FULL && col >= a.dim)) continue;
                             const float x = p[col];
                             if (!(__builtin_fabsf(x) < INFINITY)) o[n][i][r] += pk * x;
                         }
@@ -585,12 +586,12 @@ DEVI void paged_many(const PagedArgs &a) {
                     float kv[2], qv[NQ];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        kv[j] = col < a.dim ? krow[j][col] : 0.f;
+                        kv[j] = FULL || col < a.dim ? krow[j][col] : 0.f;
                         if (!qbig) kv[j] = big_part(kv[j]);
                     }
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        qv[n] = col < a.dim ? qrow[n][col] * a.scale_log2e : 0.f;
+                        qv[n] = FULL || col < a.dim ? qrow[n][col] * a.scale_log2e : 0.f;
                         if (!kbig) qv[n] = big_part(qv[n]);
                     }
 #pragma unroll
@@ -669,7 +670,7 @@ DEVI void paged_many(const PagedArgs &a) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 const int col = 16 * i + 4 * lgrp + k;
-                                if (!sees || col >= a.dim) continue;
+                                if (!sees || (!FULL && col >= a.dim)) continue;
                                 const float x = vr[col];
                                 if (__builtin_fabsf(x) >= kBig || (edge && x != x)) o[i][n][k] += pk * x;
                             }
@@ -1110,11 +1111,12 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
     a.w_out[at] = a.w_in[at] + sum;
 }
 
+// (d = 256: one wave per SIMD, since two spill; 64 sequences of 2048 to 4096 rows of 16 over 4 heads 394 -> 307 us.)
 #define ZT_PAGED_FEW(DP, NQ)                                                                        \
-    extern "C" __global__ void __launch_bounds__(256, 2) zt_paged_few_d##DP##_n##NQ(PagedArgs a) {   \
+    extern "C" __global__ void __launch_bounds__(256, (DP) == 256 ? 1 : 2) zt_paged_few_d##DP##_n##NQ(PagedArgs a) {   \
         paged_few<DP, NQ, true>(a);                                                                 \
     }                                                                                               \
-    extern "C" __global__ void __launch_bounds__(256, 2) zt_paged_few_d##DP##_n##NQ##_any(PagedArgs a) { \
+    extern "C" __global__ void __launch_bounds__(256, (DP) == 256 ? 1 : 2) zt_paged_few_d##DP##_n##NQ##_any(PagedArgs a) { \
         paged_few<DP, NQ, false>(a);                                                                \
     }
 #define ZT_PAGED_MANY(DP, NW, NQ)                                                                   \
@@ -1125,7 +1127,7 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
         paged_many<DP, NW, NQ, false>(a);                                                           \
     }
 #define ZT_PAGED(DP)                                                                                \
-    ZT_PAGED_FEW(DP, 1) ZT_PAGED_FEW(DP, 2)                                                         \
+    ZT_PAGED_FEW(DP, 1)                                                                             \
     extern "C" __global__ void __launch_bounds__(256) zt_paged_merge_d##DP(PagedArgs a) {     \
         paged_merge<DP, false>(a);                                                                  \
     }                                                                                               \
@@ -1143,7 +1145,8 @@ ZT_PAGED_MANY(64, 4, 1) ZT_PAGED_MANY(64, 4, 2) ZT_PAGED_MANY(64, 8, 2)
 ZT_PAGED_MANY(96, 4, 1) ZT_PAGED_MANY(96, 4, 2) ZT_PAGED_MANY(96, 8, 2)
 ZT_PAGED_MANY(128, 4, 1) ZT_PAGED_MANY(128, 4, 2) ZT_PAGED_MANY(128, 8, 2)
 ZT_PAGED_MANY(192, 4, 1) ZT_PAGED_MANY(192, 8, 1)
-ZT_PAGED_MANY(256, 4, 1) ZT_PAGED_MANY(256, 8, 1)
+ZT_PAGED_MANY(256, 8, 1)
+ZT_PAGED_FEW(32, 2) ZT_PAGED_FEW(64, 2) ZT_PAGED_FEW(96, 2) ZT_PAGED_FEW(128, 2)
 #define ZT_PAGED_WPARTS(DP, NW, NK)                                                                 \
     extern "C" __global__ void __launch_bounds__(64 * NW, 2) zt_paged_wparts_d##DP(PagedWeightArgs a) { \
         paged_wparts<DP, NW, NK, true>(a);                                                          \

@@ -82,7 +82,8 @@ static int paged_dp(int dim) {
 namespace {
 
 // Which kernel takes a sequence, by its rows per kv head (new tokens x heads of the group): the streaming kernel
-// with one or two 16-row blocks, or the split-operand one with 64, 128 or 256 rows in a workgroup.
+// with one or two 16-row blocks, or the split-operand one with 64, 128 or 256 rows in a workgroup (past d = 128 64 or
+// 128, at d = 256 128: 36 rows of 16 sequences of 2048, 16 over 4 heads, 97 us, in workgroups of 64 106).
 enum PagedKind { kFew1, kFew2, kMany64, kMany128, kMany256, kPagedKinds };
 constexpr bool paged_few(PagedKind k) { return k <= kFew2; }
 // Waves and 16-row blocks per wave of the split-operand kernel.
@@ -100,13 +101,18 @@ struct PagedPlan {
     int most[kPagedKinds];  // units of keys (unit()) of a workgroup at most
     int part_rows;          // rows of a part of the weights' sums
     bool keep;              // the split-operand kernel stores its scores for the weights
+    bool two_blocks;        // the streaming kernel takes 17 to 32 rows
 
     int q_len(int b) const { return q_start[b + 1] - q_start[b]; }
     int rows(int b) const { return q_len(b) * G; }
     bool any(int b) const { return q_len(b) > 0; }
     PagedKind kind(int b) const {
         const int r = rows(b);
-        return r <= 16 ? kFew1 : r <= 32 ? kFew2 : r <= 64 ? kMany64 : r <= 128 || dp > 128 ? kMany128 : kMany256;
+        return r <= 16                ? kFew1
+               : r <= 32 && two_blocks ? kFew2
+               : r <= 64 && dp <= 192 ? kMany64
+               : r <= 128 || dp > 128 ? kMany128
+                                      : kMany256;
     }
     bool many(int b) const { return any(b) && !paged_few(kind(b)); }
     // Rows of a workgroup, and the keys of its steps: a 16-key tile for each of four waves, or 32.
@@ -177,7 +183,8 @@ double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double 
 // chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8 heads at d = 128 139 / 91, three chunks of
 // 501 on 1850 to 2980 rows at d = 96 470 / 240.
 int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
-    const int slots = k == kMany256 || (p.dp > 128 && k == kMany128) ? 256 : 512;  // two workgroups of four waves per CU
+    // Two workgroups of four waves per CU where LDS holds both.
+    const int slots = paged_shape(k, p.dp).nw == 4 && p.dp <= 192 ? 512 : 256;
     const double extra = 3, way = 0.011;
     const int least = 4;
     int best = longest;
@@ -200,13 +207,13 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
 }
 
 // Units of a workgroup of the streaming kernel at most: the least time by the same reckoning, one unit for a
-// workgroup's own start and end, 512 workgroups at once.  Chunks are of one length within a sequence and not over all, so
+// workgroup's own start and end, 512 workgroups at once (256 at d = 256).  Chunks are of one length within a sequence and not over all, so
 // that many workgroups count as an even share and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048
 // workgroups aimed at / this): 64 sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128 544 / 557 / 516 / 499, 16 of
 // half that with weights 91 / 89 / 93 / 89, 3 of 6000 rows with 8 tokens each 52 / 65 / 66 / 52, one of 100000 rows 159 /
 // 151 / 140 / 144.  (Chunks of 64 keys: 16 over 4 heads of 8192 rows at d = 256 40 instead of 32.)
 int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
-    const int wgs = tuned(kTunePagedWgs, 0);
+    const int wgs = tuned(kTunePagedWgs, 0), slots = p.dp <= 192 ? 512 : 256;
     int best = longest;
     double time = 0;
     for (int limit = 2; limit <= longest; limit += (limit + 3) / 4) {
@@ -223,21 +230,28 @@ int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
             if (n <= wgs) return limit;
             continue;
         }
-        const double rounds = (double)((n + 511) / 512) * (limit + 1);
-        const double t = std::min(rounds, (double)(units + n) / 512 + 0.5 * (limit + 1));
+        const double rounds = (double)((n + slots - 1) / slots) * (limit + 1);
+        const double t = std::min(rounds, (double)(units + n) / slots + 0.5 * (limit + 1));
         if (limit == 2 || t < time) {
             time = t;
             best = limit;
         }
-        if (n <= 512) break;  // fewer workgroups only take longer
+        if (n <= slots) break;  // fewer workgroups only take longer
     }
     return best;
 }
 
 PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
-    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0, true};
+    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0, true, true};
     int longest[kPagedKinds] = {};
-    long long scores = 0, sums = 0;
+    long long scores = 0, sums = 0, units = 0;
+    // 17 to 32 rows: with two blocks the streaming kernel's f32 MFMAs weigh as much as its reads, and past d = 128 its
+    // registers spill; where it cannot hide behind latency the split-operand kernel takes them.  Measured on MI355X
+    // (us, streaming / split operands; 32 rows): one sequence of 8192 rows of 32 over 8 heads at d = 128 33 / 36, 4 of 500 19.5 /
+    // 22.9, 16 of 2048 89 / 70, at d = 96 72 / 66; 16 of 2048 of 12 over 4 heads at d = 64 26 / 27, 16 over 4 at d = 256 281 / 95.
+    for (int b = 0; b < B; ++b)
+        if (p.rows(b) > 16 && p.rows(b) <= 32) units += (long long)Hkv * ((n_rows[b] + 63) / 64);
+    p.two_blocks = p.dp <= 64 || (p.dp <= 128 && units <= 2048);  // four 64-key units to each workgroup that fits at once
     for (int b = 0; b < B; ++b) {
         if (!p.any(b)) continue;
         const PagedKind k = p.kind(b);
@@ -393,10 +407,16 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         if (launch_for(name, few ? 256u : 64u * shape.nw, 1, a, items, fill)) return 1;
         // Same stream: the merge reads the chunks' partials.
         part0 = score0 = 0;
-        // Few rows of many chunks: a workgroup to a row; many rows of few: a lane group.
-        snprintf(name, sizeof name, few ? "zt_paged_merge_d%d" : "zt_paged_merge_rows_d%d", dp);
+        // Many rows of few chunks: a lane group to a row; else a workgroup.
+        int chunks = 0;
+        for (int b = 0; b < B; ++b)
+            if (mine(b)) chunks = std::max(chunks, p.chunks(b));
+        if (chunks <= 1) continue;
+        const bool by_rows = !few && chunks <= 8;
+        snprintf(name, sizeof name, by_rows ? "zt_paged_merge_rows_d%d" : "zt_paged_merge_d%d", dp);
         const auto merged = [&](int b) { return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads : 0LL; };
-        if (launch_for(name, 256u, few ? 1 : dp <= 32 ? 32 : dp <= 64 ? 16 : dp <= 128 ? 8 : 4, a, merged, fill)) return 1;
+        const unsigned per_wg = !by_rows ? 1 : dp <= 32 ? 32 : dp <= 64 ? 16 : dp <= 128 ? 8 : 4;
+        if (launch_for(name, 256u, per_wg, a, merged, fill)) return 1;
     }
     if (!weights) return 0;
     // ... and these the rows' statistics.
