@@ -116,6 +116,9 @@ struct PagedArgs {
     float *scores;      // scaled scores (log2 units), or null: sequence i's at score0[i], the streaming kernel's
                         // [Hkv, rows, keys padded to 16], the split-operand one's in 16 x 16 tiles [Hkv, row tile, key tile]
     int H, Hkv, G, dim;
+    const float *w_in;  // [B, Hkv, w_stride] (zt_paged_merge_w_*)
+    float *w_out;
+    int w_stride;
     int part_ld;        // dim rounded up to whole 16 bytes
     float scale_log2e;
     PagedSeqs seq;      // at0: the first partial, slot (kvh * rows + row) * nch + chunk behind it

@@ -717,6 +717,25 @@ DEVI void paged_many(const PagedArgs &a) {
     }
 }
 
+// Weights of few rows from the scores that the attention stored: of four keys of one
+// (sequence, kv head), all rows' added in order.  sp: the keys' scores in row 0; stat(r): row r's base and inverse sum.
+// Rows that do not see the keys are skipped (their scores may not be written).
+template <class Stat>
+DEVI f4 weights_of_few(const float *sp, int kpad, int rows, int G, int seen0, int key, Stat stat) {
+    f4 sum = zero4();
+    int t = 0, g = 0;
+    for (int r = 0; r < rows; ++r) {
+        if (key <= seen0 + t) {  // else none of the four keys is seen
+            const f4 s = *reinterpret_cast<const f4 *>(sp + (size_t)r * kpad);
+            const f2 ml = stat(r);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += key + e <= seen0 + t ? fast_exp2(s[e] - ml.x) * ml.y : 0.f;
+        }
+        if (++g == G) { g = 0; ++t; }
+    }
+    return sum;
+}
+
 // ---- Merge of the key chunks --------------------------------------------------------
 //
 // Of one (token, head): M = max_c m_c, out = sum_c acc_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).
@@ -724,7 +743,9 @@ DEVI void paged_many(const PagedArgs &a) {
 // chunks: a workgroup takes a row, each of its 256 / LPR lane groups eight chunks at a time
 // (64 chunks at d = 128 take one trip to memory), and the groups are merged in a fixed order; true, for many rows of
 // few chunks: each lane group takes a row (65536 rows of 3 chunks at d = 128: 43 us with a wave to a row, 21 so).
-template <int DP, bool ROWS>
+// W (with ROWS false): behind a sequence's rows come its weights, 1024 keys of a kv head to a workgroup, which forms
+// the rows' statistics from the partials itself instead of waiting for the merge.
+template <int DP, bool ROWS, bool W = false>
 DEVI void paged_merge(const PagedArgs &a) {
     constexpr int LPR = DP <= 32 ? 8 : DP <= 64 ? 16 : DP <= 128 ? 32 : 64, GR = ROWS ? 1 : 256 / LPR;
     constexpr int U = ROWS ? 4 : 8;  // chunks of a lane group in flight
@@ -745,7 +766,43 @@ DEVI void paged_merge(const PagedArgs &a) {
             at0 = a.seq.at0[k];
         }
     }
-    const int rows = q_len * a.G, t = i / a.H, h = i % a.H, kvh = h / a.G, r = t * a.G + h % a.G;
+    const int rows = q_len * a.G;
+    if constexpr (W) {
+        if (i >= q_len * a.H) {  // workgroup-uniform
+            __shared__ f2 stats[32];
+            const int per_head = (n_rows + 1023) / 1024, kpad = (n_rows + 15) & ~15, seen0 = n_rows - q_len;
+            const int j = i - q_len * a.H, kvh = j / per_head, key = j % per_head * 1024 + 4 * tid;
+            const int r = tid >> 3;  // eight threads to a row's chunks
+            float M = -INFINITY, L = 0.f;
+            if (r < rows) {
+                const float *ml = a.part_ml + 2 * ((size_t)at0 + ((size_t)kvh * rows + r) * nslots);
+                const int nch = (seen0 + r / a.G) / chunk + 1;
+                for (int c = tid & 7; c < nch; c += 8) {
+                    const f2 e = *reinterpret_cast<const f2 *>(ml + 2 * c);
+                    const float mb = fmaxf(M, e.x);
+                    L = L * (M == -INFINITY ? 0.f : fast_exp2(M - mb)) + e.y * (e.x == -INFINITY ? 0.f : fast_exp2(e.x - mb));
+                    M = mb;
+                }
+            }
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) {
+                const float M2 = wave_xor(M, d), L2 = wave_xor(L, d), mb = fmaxf(M, M2);
+                L = L * (M == -INFINITY ? 0.f : fast_exp2(M - mb)) + L2 * (M2 == -INFINITY ? 0.f : fast_exp2(M2 - mb));
+                M = mb;
+            }
+            if (r < rows && (tid & 7) == 0) stats[r] = f2{M, 1.f / L};
+            __syncthreads();
+            if (key >= n_rows) return;
+            const float *sp = a.scores + a.score0[sq.i] + (size_t)kvh * rows * kpad + key;
+            const f4 sum = weights_of_few(sp, kpad, rows, a.G, seen0, key, [&](int x) { return stats[x]; });
+            const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (key + e < n_rows) a.w_out[at + e] = a.w_in[at + e] + sum[e];
+            return;
+        }
+    }
+    const int t = i / a.H, h = i % a.H, kvh = h / a.G, r = t * a.G + h % a.G;
     const int nch = (n_rows - q_len + t) / chunk + 1;  // chunks that hold a key the token sees
     const size_t slot0 = (size_t)at0 + ((size_t)kvh * rows + r) * nslots;
     const bool ok = col < a.dim;
@@ -803,9 +860,7 @@ DEVI void paged_merge(const PagedArgs &a) {
 
 // ---- Accumulated weights ---------------------------------------------------------------
 //
-// Few rows: from the scores that the attention stored.  A thread takes four keys of one
-// (sequence, kv head) and adds the weights of all rows, in order.  Rows that do not see the keys are skipped
-// (their scores may not be written).  Sequences without new tokens copy their weights.
+// Few rows in one chunk (more: paged_merge).  Sequences without new tokens copy their weights.
 extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightArgs a) {
     const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
     const int n = sq.n_rows, kpad = (n + 15) & ~15, rows = sq.q_len * a.G;
@@ -815,18 +870,10 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
     if (key >= n) return;
     const float *sp = a.scores + sq.at0 + (size_t)kvh * rows * kpad + key;
     const float *st = a.stat + 2 * ((size_t)sq.q0 * a.H + kvh * a.G);
-    const int seen0 = n - sq.q_len;
-    f4 sum = zero4();
-    int t = 0, g = 0;
-    for (int r = 0; r < rows; ++r) {
-        if (key <= seen0 + t) {  // else none of the four keys is seen
-            const f4 s = *reinterpret_cast<const f4 *>(sp + (size_t)r * kpad);
-            const f2 ml = *reinterpret_cast<const f2 *>(st + 2 * ((size_t)t * a.H + g));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += key + e <= seen0 + t ? fast_exp2(s[e] - ml.x) * ml.y : 0.f;
-        }
-        if (++g == a.G) { g = 0; ++t; }
-    }
+    const f4 sum = weights_of_few(sp, kpad, rows, a.G, n - sq.q_len, key, [&](int r) {
+        const int t = r / a.G;
+        return *reinterpret_cast<const f2 *>(st + 2 * ((size_t)t * a.H + r - t * a.G));
+    });
     const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -1133,6 +1180,9 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
     }                                                                                               \
     extern "C" __global__ void __launch_bounds__(256) zt_paged_merge_rows_d##DP(PagedArgs a) {       \
         paged_merge<DP, true>(a);                                                                   \
+    }                                                                                               \
+    extern "C" __global__ void __launch_bounds__(256) zt_paged_merge_w_d##DP(PagedArgs a) {          \
+        paged_merge<DP, false, true>(a);                                                            \
     }
 ZT_PAGED(32)
 ZT_PAGED(64)

@@ -207,13 +207,13 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
 }
 
 // Units of a workgroup of the streaming kernel at most: the least time by the same reckoning, one unit for a
-// workgroup's own start and end, 512 workgroups at once (256 at d = 256).  Chunks are of one length within a sequence and not over all, so
+// workgroup's own start and end, as many workgroups at once as the kernel's registers let stand on the CUs.  Chunks are of one length within a sequence and not over all, so
 // that many workgroups count as an even share and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048
 // workgroups aimed at / this): 64 sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128 544 / 557 / 516 / 499, 16 of
 // half that with weights 91 / 89 / 93 / 89, 3 of 6000 rows with 8 tokens each 52 / 65 / 66 / 52, one of 100000 rows 159 /
 // 151 / 140 / 144.  (Chunks of 64 keys: 16 over 4 heads of 8192 rows at d = 256 40 instead of 32.)
 int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
-    const int wgs = tuned(kTunePagedWgs, 0), slots = p.dp <= 192 ? 512 : 256;
+    const int wgs = tuned(kTunePagedWgs, 0), slots = p.dp <= 64 ? 1024 : p.dp <= 128 ? 768 : p.dp <= 192 ? 512 : 256;
     int best = longest;
     double time = 0;
     for (int limit = 2; limit <= longest; limit += (limit + 3) / 4) {
@@ -349,6 +349,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     a.stat = weights ? reinterpret_cast<float *>(ws + space.stat) : nullptr;
     a.H = n_heads; a.Hkv = n_kv_heads; a.G = p.G; a.dim = dim;
     a.part_ld = p.part_ld;
+    a.w_in = w_in; a.w_out = w_out; a.w_stride = w_stride;
     a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)dim));
     // Whole 16-byte chunks throughout a row.
     const char *const any = dim == dp ? "" : "_any";
@@ -413,8 +414,13 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
             if (mine(b)) chunks = std::max(chunks, p.chunks(b));
         if (chunks <= 1) continue;
         const bool by_rows = !few && chunks <= 8;
-        snprintf(name, sizeof name, by_rows ? "zt_paged_merge_rows_d%d" : "zt_paged_merge_d%d", dp);
-        const auto merged = [&](int b) { return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads : 0LL; };
+        // (Few rows' weights come with it, where they are wanted: 1024 keys to a workgroup.)
+        const bool with = weights && few;
+        snprintf(name, sizeof name, by_rows ? "zt_paged_merge_rows_d%d" : with ? "zt_paged_merge_w_d%d" : "zt_paged_merge_d%d", dp);
+        const auto merged = [&](int b) {
+            const long long sums = with ? (long long)((n_rows[b] + 1023) / 1024) * n_kv_heads : 0;
+            return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads + sums : 0LL;
+        };
         const unsigned per_wg = !by_rows ? 1 : dp <= 32 ? 32 : dp <= 64 ? 16 : dp <= 128 ? 8 : 4;
         if (launch_for(name, 256u, per_wg, a, merged, fill)) return 1;
     }
@@ -442,7 +448,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         return launch_for(kernel, threads, 1, g, [&](int b) { return p.many(b) == many ? items(b) : 0LL; }, fill);
     };
     const auto per_head = [&](int b, int keys) { return (long long)((n_rows[b] + keys - 1) / keys) * n_kv_heads; };
-    if (run("zt_paged_weights", 256u, false, [&](int b) { return per_head(b, 1024); })) return 1;
+    const auto rest = [&](int b) { return p.chunks(b) > 1 ? 0LL : per_head(b, 1024); };  // of those without a merge
+    if (run("zt_paged_weights", 256u, false, rest)) return 1;
     if (p.keep) snprintf(name, sizeof name, "zt_paged_wcols");
     else snprintf(name, sizeof name, "zt_paged_wparts_d%d%s", dp, any);
     const auto parts = [&](int b) { return per_head(b, p.weight_keys()) * p.parts(b); };
