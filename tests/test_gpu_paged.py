@@ -68,7 +68,7 @@ def grade(got, ref, q_start, n_rows, Hkv, w_h=None):
 
 
 SHAPES = [(4, 2, 32), (8, 8, 64), (6, 2, 64), (32, 8, 128), (8, 2, 96), (16, 4, 256), (5, 1, 128), (40, 2, 32), (2, 1, 160),
-          (4, 4, 34), (6, 3, 50), (9, 3, 250), (8, 2, 132), (4, 1, 192), (8, 4, 40)]
+          (4, 4, 34), (6, 3, 50), (9, 3, 250), (8, 2, 132), (4, 1, 192), (8, 4, 40), (64, 1, 64), (33, 1, 32)]
 # (rows with the new tokens, new tokens): one token, none, no rows, ends inside a 16-key tile and at it, prompts.
 BATCHES = {
     "single_tokens": ([1, 2, 15, 16, 17, 33, 200], [1] * 7),
@@ -456,6 +456,40 @@ def test_other_streams_and_two_at_once(gpu, zt):
     gpu.cuda.synchronize()
     for o, x in zip(outs, want):
         assert np.array_equal(o.cpu().numpy(), x[0])
+
+
+def test_two_graphs_with_one_workspace(gpu, zt):
+    """Two captured calls of different lengths that share a workspace, replayed in turn on one stream."""
+    H, Hkv, d, page = 8, 2, 64, 16
+    rng = np.random.default_rng(16)
+    cs = [Cache(gpu, rng, n, page, Hkv, d) for n in ([1500, 700], [300])]
+    starts = [[0, 1, 41], [0, 90]]
+    qs = [gpu.from_numpy(rng.standard_normal((s[-1], H, d)).astype(np.float32)).cuda() for s in starts]
+    ws_w = [gpu.from_numpy(rng.random((len(c.n_rows), Hkv, max(c.n_rows)), np.float32)).cuda() for c in cs]
+    need = max(zt.attn_paged_workspace_bytes(s, c.n_rows, H, Hkv, d, True) for s, c in zip(starts, cs))
+    ws = gpu.empty(need, device="cuda", dtype=gpu.uint8)
+    outs, w_outs = [gpu.zeros_like(q) for q in qs], [gpu.zeros_like(w) for w in ws_w]  # (later w_out: left as it is)
+
+    def call(i):
+        zt.attn_paged(qs[i], cs[i].k, cs[i].v, cs[i].table, outs[i], starts[i], cs[i].n_rows, page, H, Hkv, d, ws,
+                      w_in=ws_w[i], w_out=w_outs[i])
+
+    want = []
+    for i in (0, 1):
+        call(i)
+        want.append((outs[i].clone(), w_outs[i].clone()))
+    graphs = []
+    for i in (0, 1):
+        graphs.append(gpu.cuda.CUDAGraph())
+        gpu.cuda.synchronize()
+        with gpu.cuda.graph(graphs[i]):
+            call(i)
+    for i in (0, 1, 1, 0, 1, 0):
+        outs[i].zero_()
+        w_outs[i].zero_()
+        graphs[i].replay()
+        gpu.cuda.synchronize()
+        assert gpu.equal(outs[i], want[i][0]) and gpu.equal(w_outs[i], want[i][1])
 
 
 def test_captured_and_replayed(gpu, zt):

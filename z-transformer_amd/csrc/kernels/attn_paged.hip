@@ -17,13 +17,15 @@
 #include "split.h"
 
 // N consecutive floats (2 or 4) of a row at column c; FULL: the row has DP aligned
-// columns; else columns past dim are 0 and rows may be 8-byte aligned only.
-template <int N, bool FULL>
+// columns; else columns past dim are 0 and rows may be 8-byte aligned only.  ONCE: read by one
+// workgroup only, and kept out of the caches (a prompt, whose workgroups share its K and V rows, 667 us so, 653 not).
+template <int N, bool FULL, bool ONCE>
 DEVI void load_cols(float *dst, const float *row, int c, int dim, bool vec4) {
     if constexpr (N == 4) {
         f4 x = zero4();
         if (FULL || (vec4 && c < dim)) {
-            x = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(row + c));
+            const f4 *p = reinterpret_cast<const f4 *>(row + c);
+            x = ONCE ? __builtin_nontemporal_load(p) : *p;
         } else if (!vec4) {
             if (c < dim) {
                 const f2 y = *reinterpret_cast<const f2 *>(row + c);
@@ -38,7 +40,10 @@ DEVI void load_cols(float *dst, const float *row, int c, int dim, bool vec4) {
         for (int e = 0; e < 4; ++e) dst[e] = x[e];
     } else {
         f2 x = f2{0.f, 0.f};
-        if (FULL || c < dim) x = __builtin_nontemporal_load(reinterpret_cast<const f2 *>(row + c));
+        if (FULL || c < dim) {
+            const f2 *p = reinterpret_cast<const f2 *>(row + c);
+            x = ONCE ? __builtin_nontemporal_load(p) : *p;
+        }
         dst[0] = x.x; dst[1] = x.y;
     }
 }
@@ -51,8 +56,10 @@ DEVI void put_stats(const PagedArgs &a, size_t row, float m, float l) {
 
 // ---- Few rows: K and V stream through registers -----------------------------------
 //
-// A workgroup takes one (sequence, kv head, chunk of keys, tile of 16 NQ rows); its four waves
-// take the chunk's 16-key tiles in turn.  Bound: HBM, each K and V row read once per kv head.
+// A workgroup takes one (sequence, kv head, chunk of keys) and all of its rows, at most 16 NQ; its
+// four waves take the chunk's 16-key tiles in turn.  Bound: HBM, each K and V row read once per kv
+// head: a token of each of 64 sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128, 505 us, 6.4 TB/s
+// (a streaming read reaches 7.1), the matrix cores 39 % busy, with 1 row or 16.
 //   * S^T = K Q^T on v_mfma_f32_16x16x4_f32 with the contraction dealt so that k-step
 //     (j, e) of lane group grp is column 16 j + 4 grp + e: the A operand is then what
 //     lane (l16, grp) loads of key l16 with 16-byte loads, straight from memory.
@@ -69,15 +76,10 @@ DEVI void paged_few(const PagedArgs &a) {
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
-    const int nch = sq.nch, q_len = sq.q_len, rows = q_len * a.G;
-    int item = (int)blockIdx.x - sq.first;
-    const int c = item % nch;
-    item /= nch;
-    const int kvh = item % a.Hkv, row0 = item / a.Hkv * 16 * NQ;
+    const int nch = sq.nch, q_len = sq.q_len, rows = q_len * a.G;  // at most 16 NQ rows
+    const int item = (int)blockIdx.x - sq.first, c = item % nch, kvh = item / nch;
     const int seen0 = sq.n_rows - q_len;  // the cache row of token 0, the last it sees
-    const int kend = seen0 + (min(rows, row0 + 16 * NQ) - 1) / a.G + 1;
-    const int key0 = c * sq.chunk, key1 = min(kend, key0 + sq.chunk);
-    if (key0 >= kend) return;  // workgroup-uniform
+    const int key0 = c * sq.chunk, key1 = min(sq.n_rows, key0 + sq.chunk);
     const int *table = a.pool.table + (size_t)sq.b * a.pool.table_stride;
     const size_t qld = (size_t)a.H * a.dim, kld = (size_t)a.Hkv * a.dim;
     const bool vec4 = (a.dim & 3) == 0;
@@ -88,12 +90,12 @@ DEVI void paged_few(const PagedArgs &a) {
     int last[NQ];  // the last key that the lane's row sees
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int r = min(row0 + 16 * n + l16, rows - 1), t = r / a.G;
+        const int r = min(16 * n + l16, rows - 1), t = r / a.G;
         last[n] = seen0 + t;
         const float *row = a.q + (size_t)(sq.q0 + t) * qld + (size_t)(kvh * a.G + r - t * a.G) * a.dim;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            load_cols<4, FULL>(q[n][j], row, 16 * j + 4 * grp, a.dim, vec4);
+            load_cols<4, FULL, true>(q[n][j], row, 16 * j + 4 * grp, a.dim, vec4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) q[n][j][e] *= a.scale_log2e;
         }
@@ -116,7 +118,7 @@ DEVI void paged_few(const PagedArgs &a) {
     auto load_k = [&](int row) {
         const float *p = kb + (size_t)max(row, 0) * kld;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) load_cols<4, FULL>(kx[j], p, 16 * j + 4 * grp, a.dim, vec4);
+        for (int j = 0; j < NT; ++j) load_cols<4, FULL, true>(kx[j], p, 16 * j + 4 * grp, a.dim, vec4);
     };
     auto load_v = [&](int row) {
 #pragma unroll
@@ -124,7 +126,7 @@ DEVI void paged_few(const PagedArgs &a) {
             vrow[r] = __shfl(row, 4 * grp + r, 64);
             const float *p = vb + (size_t)max(vrow[r], 0) * kld;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) load_cols<C, FULL>(vx[r][i], p, 16 * C * i + C * l16, a.dim, vec4);
+            for (int i = 0; i < NV; ++i) load_cols<C, FULL, true>(vx[r][i], p, 16 * C * i + C * l16, a.dim, vec4);
         }
     };
     int next = 0;
@@ -166,7 +168,7 @@ DEVI void paged_few(const PagedArgs &a) {
             float *sp = a.scores + a.score0[sq.i] + (size_t)kvh * rows * kpad + k0 + 4 * grp;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                const int r = row0 + 16 * n + l16;
+                const int r = 16 * n + l16;
                 if (r < rows) *reinterpret_cast<f4 *>(sp + (size_t)r * kpad) = s[n];
             }
         }
@@ -256,7 +258,7 @@ DEVI void paged_few(const PagedArgs &a) {
         for (int r = 0; r < 4; ++r) store_run<NT>(Wacc[w][l16], 4 * grp + r, DP, true, o[n], r, 1.f);
         __syncthreads();
         for (int e = tid; e < 16 * (DP / 4); e += 64 * NW) {
-            const int i = e / (DP / 4), col = 4 * (e % (DP / 4)), r = row0 + 16 * n + i;
+            const int i = e / (DP / 4), col = 4 * (e % (DP / 4)), r = 16 * n + i;
             if (r >= rows || col >= a.dim) continue;
             float M = Wm[0][i];
 #pragma unroll
@@ -293,11 +295,14 @@ DEVI void paged_few(const PagedArgs &a) {
 // split once for all waves: two buffers of each, and the second half of the waves runs half a step behind the
 // first, so that one half's softmax and splitting run beside the other's products.
 //   A step is phase A (S^T = K Q^T, softmax; the next K tile into LDS) and phase B (O^T += V^T P^T; the
-//   next V tile); tiles are loaded a whole step before they are written to LDS where registers allow (DEEP), else in that phase.
+//   next V tile); tiles are loaded a whole step before they are written to LDS where registers allow (DEEP),
+//   else in that phase.
 //   * The pool rows that a thread stages are looked up in the page table one tile ahead of its loads.
 //   * The rows of V hold a value that is big (split.h), or that is not finite where a pair of the tile is
 //     hidden, as 0 in the split, and it is added from the full row to the rows that see it.
 //   * A key whose page is none of the pool's is staged as NaN: the scores it meets are NaN.
+// Bound: as the contiguous forward, the vector instructions beside the MFMAs, two to each, at two waves per SIMD:
+// a prompt of 4096 rows, 32 over 8 heads at d = 128, 645 us, 213 TFLOP/s, the matrix cores 57 % busy.
 template <int DP, int NW, int NQ>
 struct PagedMany {
     static constexpr int NT = DP / 16, NKS = DP / 32, NTH = 64 * NW;
@@ -363,7 +368,7 @@ DEVI void paged_many(const PagedArgs &a) {
             float y[4];
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
-                load_cols<4, FULL>(y, p, e % CPR * 8 + i, a.dim, vec4);
+                load_cols<4, FULL, false>(y, p, e % CPR * 8 + i, a.dim, vec4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[n][i + k] = y[k];
             }
@@ -408,7 +413,7 @@ DEVI void paged_many(const PagedArgs &a) {
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
                 float z[4];
-                load_cols<4, FULL>(z, row, 32 * ks + 8 * grp + i, a.dim, vec4);
+                load_cols<4, FULL, false>(z, row, 32 * ks + 8 * grp + i, a.dim, vec4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) y[i + k] = z[k] * a.scale_log2e;
             }
@@ -449,8 +454,10 @@ DEVI void paged_many(const PagedArgs &a) {
                         (((size_t)kvh * ((rows + 15) >> 4) + (row0 >> 4)) * ktiles + (k0 >> 4)) * 256;
 #pragma unroll
             for (int i = 0; i < 2 * NQ; ++i)
-                if (row0 + 16 * (i % NQ) < rows && k0 + 16 * (i / NQ) < key1)  // wave-uniform
-                    __builtin_nontemporal_store(s[i], reinterpret_cast<f4 *>(sp + ((size_t)(i % NQ) * ktiles + i / NQ) * 256));
+                if (row0 + 16 * (i % NQ) < rows && k0 + 16 * (i / NQ) < key1) {  // wave-uniform
+                    float *p = sp + ((size_t)(i % NQ) * ktiles + i / NQ) * 256;
+                    __builtin_nontemporal_store(s[i], reinterpret_cast<f4 *>(p));
+                }
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -762,7 +769,8 @@ DEVI void paged_merge(const PagedArgs &a) {
         while (i >= q_len * a.H) {  // of a sequence behind it, or past the last's end
             if (++k == a.seq.n) return;
             i = item - a.seq.first[k];
-            q_len = a.seq.q_len[k]; n_rows = a.seq.n_rows[k]; nslots = a.seq.nch[k]; chunk = a.seq.chunk[k]; q0 = a.seq.q0[k];
+            q_len = a.seq.q_len[k]; n_rows = a.seq.n_rows[k]; nslots = a.seq.nch[k]; chunk = a.seq.chunk[k];
+            q0 = a.seq.q0[k];
             at0 = a.seq.at0[k];
         }
     }
@@ -773,6 +781,7 @@ DEVI void paged_merge(const PagedArgs &a) {
             const int per_head = (n_rows + 1023) / 1024, kpad = (n_rows + 15) & ~15, seen0 = n_rows - q_len;
             const int j = i - q_len * a.H, kvh = j / per_head, key = j % per_head * 1024 + 4 * tid;
             const int r = tid >> 3;  // eight threads to a row's chunks
+            auto from = [](float m, float to) { return m == -INFINITY ? 0.f : fast_exp2(m - to); };
             float M = -INFINITY, L = 0.f;
             if (r < rows) {
                 const float *ml = a.part_ml + 2 * ((size_t)at0 + ((size_t)kvh * rows + r) * nslots);
@@ -780,14 +789,14 @@ DEVI void paged_merge(const PagedArgs &a) {
                 for (int c = tid & 7; c < nch; c += 8) {
                     const f2 e = *reinterpret_cast<const f2 *>(ml + 2 * c);
                     const float mb = fmaxf(M, e.x);
-                    L = L * (M == -INFINITY ? 0.f : fast_exp2(M - mb)) + e.y * (e.x == -INFINITY ? 0.f : fast_exp2(e.x - mb));
+                    L = L * from(M, mb) + e.y * from(e.x, mb);
                     M = mb;
                 }
             }
 #pragma unroll
             for (int d = 1; d < 8; d <<= 1) {
                 const float M2 = wave_xor(M, d), L2 = wave_xor(L, d), mb = fmaxf(M, M2);
-                L = L * (M == -INFINITY ? 0.f : fast_exp2(M - mb)) + L2 * (M2 == -INFINITY ? 0.f : fast_exp2(M2 - mb));
+                L = L * from(M, mb) + L2 * from(M2, mb);
                 M = mb;
             }
             if (r < rows && (tid & 7) == 0) stats[r] = f2{M, 1.f / L};
@@ -881,9 +890,10 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
 }
 
 // Many rows: from the tiles that the attention stored.  A workgroup takes 128 keys of one
-// (sequence, kv head) and a part of the rows; a wave two neighbouring key tiles, 2 KB a row tile, four row tiles in flight:
-// lane (l16, grp) adds row l16's weights of keys 4 grp .. 4 grp + 3 over the row tiles, and the 16 rows' lanes are added
-// at the end.  Bound: HBM, the scores read once.
+// (sequence, kv head) and a part of the rows; a wave two neighbouring key tiles, 2 KB a row tile, four
+// row tiles in flight: lane (l16, grp) adds row l16's weights of keys 4 grp .. 4 grp + 3 over the row
+// tiles, and the 16 rows' lanes are added at the end.  Bound: HBM, the scores read once (a 2048-row
+// prompt of 32 heads, 268 MB, about 45 us, 6 TB/s).
 extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs a) {
     const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
     const int n = sq.n_rows, rows = sq.q_len * a.G, seen0 = n - sq.q_len, ktiles = (n + 15) >> 4;
@@ -892,11 +902,12 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs
     const int kvh = item % a.Hkv;
     item /= a.Hkv;
     const int part = nparts - 1 - item / ntiles, kt0 = item % ntiles * 128;
-    if (max(0, kt0 - seen0) * a.G >= (part + 1) * a.part_rows) return;  // no row sees the keys; zt_paged_wsum does not read it
+    if (max(0, kt0 - seen0) * a.G >= (part + 1) * a.part_rows) return;  // no row sees the keys; wsum skips it
     const int lane = lane_id(), l16 = lane & 15, grp = lane >> 4;
     const int k0 = kt0 + 32 * __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (k0 >= n) return;
-    const int rt0 = max(part * a.part_rows, max(0, k0 - seen0) * a.G) >> 4, rt1 = (min(rows, (part + 1) * a.part_rows) + 15) >> 4;
+    const int rt0 = max(part * a.part_rows, max(0, k0 - seen0) * a.G) >> 4;
+    const int rt1 = (min(rows, (part + 1) * a.part_rows) + 15) >> 4;
     const bool two = k0 + 16 < n;
     const float *sp = a.scores + sq.at0 + 4 * lane + ((size_t)kvh * ((rows + 15) >> 4) * ktiles + (k0 >> 4)) * 256;
     const float *st = a.stat + 2 * ((size_t)sq.q0 * a.H + kvh * a.G);
@@ -928,7 +939,8 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) four[e] += key + e <= last[j] ? fast_exp2(s[j][i][e] - ml[j].x) * ml[j].y : 0.f;
+                for (int e = 0; e < 4; ++e)
+                    four[e] += key + e <= last[j] ? fast_exp2(s[j][i][e] - ml[j].x) * ml[j].y : 0.f;
             sum[i] += four;
         }
     }
@@ -939,11 +951,11 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[i][e] += wave_xor(sum[i][e], m);
     if (l16 > 1 || (l16 == 1 && !two)) return;
-    *reinterpret_cast<f4 *>(a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * 16 * ktiles + k0 + 16 * l16 + 4 * grp) =
-        l16 ? sum[1] : sum[0];
+    float *out = a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * 16 * ktiles + k0;
+    *reinterpret_cast<f4 *>(out + 16 * l16 + 4 * grp) = l16 ? sum[1] : sum[0];
 }
 
-// Many rows whose scores would take too much room: the scores again, on split operands.  A workgroup takes one (sequence, kv
+// Many rows whose scores are not kept: the scores again, on split operands.  A workgroup takes one (sequence, kv
 // head, tile of 16 NK NW keys, part of the rows); a wave holds 16 NK keys (K's parts in registers), and Q
 // passes through LDS in 32-row tiles, split once for all waves, two buffers, beside the rows'
 // statistics.  S = Q K^T has a key per lane and four rows, so that the sum over rows
@@ -963,7 +975,8 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
     int item = (int)blockIdx.x - sq.first;
     const int kvh = item % a.Hkv;
     item /= a.Hkv;
-    // Part by part, the last, which all keys of a prompt have rows in, first (neighbours of like length, as in paged_many).
+    // Part by part, the last, which all keys of a prompt have rows in, first (neighbours of like length, as in
+    // paged_many).
     const int ntiles = (n + KT - 1) / KT, part = nparts - 1 - item / ntiles, kt0 = item % ntiles * KT;
     // Rows of the part that see the tile's first key.
     const int r0 = max(part * a.part_rows, max(0, kt0 - seen0) * a.G) & ~31, r1 = min(rows, (part + 1) * a.part_rows);
@@ -989,7 +1002,7 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
 #pragma unroll
             for (int h = 0; h < 8; h += 4) {
                 float z[4];
-                load_cols<4, FULL>(z, krow[i], 32 * ks + 8 * grp + h, a.dim, vec4);
+                load_cols<4, FULL, false>(z, krow[i], 32 * ks + 8 * grp + h, a.dim, vec4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[h + e] = r < 0 ? __builtin_nanf("") : z[e];
             }
@@ -1022,14 +1035,15 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
 #pragma unroll
             for (int h = 0; h < 8; h += 4) {
                 float z[4];
-                load_cols<4, FULL>(z, p, e % CPR * 8 + h, a.dim, vec4);
+                load_cols<4, FULL, false>(z, p, e % CPR * 8 + h, a.dim, vec4);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) px[i][h + x] = z[x] * a.scale_log2e;
             }
         }
         if (tid < 32) {
             const int r = min(rt + tid, r1 - 1), t = r / a.G;
-            const f2 ml = *reinterpret_cast<const f2 *>(a.stat + 2 * ((size_t)(sq.q0 + t) * a.H + kvh * a.G + r - t * a.G));
+            const size_t row = (size_t)(sq.q0 + t) * a.H + kvh * a.G + r - t * a.G;
+            const f2 ml = *reinterpret_cast<const f2 *>(a.stat + 2 * row);
             sm = ml.x;
             si = ml.y;
             sl = rt + tid < r1 ? seen0 + t : -1;  // a row past the part's last sees nothing

@@ -208,8 +208,8 @@ ZT_EVICT_SELECT(4096, 8, 8)
 ZT_EVICT_SELECT(16384, 16, 16)
 ZT_EVICT_SELECT(any, 16, 0)
 
-// Rows to other pages: a thread takes 4 N bytes of K and V at a time.  Bound: HBM, a copy (16 sequences of 8192 rows to 4096,
-// 8 kv heads at d = 128, 220 us: 4.7 TB/s, as a copy of 4 GiB).
+// Rows to other pages: a thread takes 4 N bytes of K and V at a time.  Bound: HBM, a copy (16 sequences of up to
+// 8192 rows to 4096, 8 kv heads at d = 128, 220 us: 4.7 TB/s, as a copy of 4 GiB).
 template <int N>
 DEVI void evict_copy(const PagedEvictArgs &a) {
     typedef float vec __attribute__((ext_vector_type(N)));
@@ -218,7 +218,8 @@ DEVI void evict_copy(const PagedEvictArgs &a) {
     const int sl = (int)blockIdx.x / a.tiles, r0 = (int)blockIdx.x % a.tiles * rows_per_wg, b = a.b0 + sl;
     const int r1 = min(min(a.budget, a.n_rows[sl]), r0 + rows_per_wg);
     const size_t kld = (size_t)a.Hkv * a.dim;
-    const int *from = a.pool.table + (size_t)b * a.pool.table_stride, *to = a.table_out + (size_t)b * a.pool.table_stride;
+    const size_t entry = (size_t)b * a.pool.table_stride;
+    const int *from = a.pool.table + entry, *to = a.table_out + entry;
     for (int e = threadIdx.x; e < (r1 - r0) * per_row; e += 256) {
         const int j = r0 + e / per_row, c = e % per_row, h = c / per_head;
         const int src = pool_row(a.pool, from, a.kept[((size_t)b * a.Hkv + h) * a.budget + j]);
@@ -237,9 +238,9 @@ extern "C" __global__ void __launch_bounds__(256) zt_evict_copy_2(PagedEvictArgs
 // have moved already.  A workgroup takes K or V of one (sequence, kv head) and walks the rows upwards, a tile of
 // 4 x 1024 16-byte (8-byte) pieces at a time: all of a tile's rows are in registers, in every
 // wave, before one is written, and what a later tile reads lies past all that earlier ones write.
-// Bound: HBM for many sequences, the tiles' trips to memory one after the other for few: 8 kv heads at d = 128, 8192 rows
-// cut to 4096, 16 sequences 234 us (4.6 TB/s), one 70; with a wave to 64 rows of 128 bytes at a time instead 555
-// and 311, with 8 x 512 pieces 239 and 80.
+// Bound: HBM for many sequences, the tiles' trips to memory one after the other for few: 8 kv heads at d = 128,
+// 8192 rows cut to 4096, 16 sequences 234 us (4.6 TB/s), one 70; with a wave to 64 rows of 128 bytes at a time
+// instead 555 and 311, with 8 x 512 pieces 239 and 80.
 template <int N>
 DEVI void evict_move(const PagedEvictArgs &a) {
     typedef float vec __attribute__((ext_vector_type(N)));

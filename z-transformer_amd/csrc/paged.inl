@@ -91,7 +91,10 @@ struct PagedShape {
     int nw, nq;
 };
 constexpr PagedShape paged_shape(PagedKind k, int dp) {
-    return k == kMany64 ? PagedShape{4, 1} : k == kMany256 ? PagedShape{8, 2} : dp <= 128 ? PagedShape{4, 2} : PagedShape{8, 1};
+    return k == kMany64    ? PagedShape{4, 1}
+           : k == kMany256 ? PagedShape{8, 2}
+           : dp <= 128     ? PagedShape{4, 2}
+                           : PagedShape{8, 1};
 }
 
 // What a call does for each sequence.
@@ -116,7 +119,9 @@ struct PagedPlan {
     }
     bool many(int b) const { return any(b) && !paged_few(kind(b)); }
     // Rows of a workgroup, and the keys of its steps: a 16-key tile for each of four waves, or 32.
-    int tile_rows(PagedKind k) const { return k == kFew1 ? 16 : k == kFew2 ? 32 : 16 * paged_shape(k, dp).nw * paged_shape(k, dp).nq; }
+    int tile_rows(PagedKind k) const {
+        return k == kFew1 ? 16 : k == kFew2 ? 32 : 16 * paged_shape(k, dp).nw * paged_shape(k, dp).nq;
+    }
     static int unit(PagedKind k) { return paged_few(k) ? 64 : 32; }
     int tiles(int b) const { return (rows(b) + tile_rows(kind(b)) - 1) / tile_rows(kind(b)); }
     // Keys of a chunk: as few chunks as the limit allows, of one length.
@@ -136,7 +141,8 @@ struct PagedPlan {
     int parts(int b) const { return (rows(b) + part_rows - 1) / part_rows; }
     // Floats that the weights need: every row's scores, and the parts' sums.
     long long scores(int b) const {
-        return (long long)kpad(b) * (many(b) ? keep ? (long long)Hkv * ((rows(b) + 15) / 16 * 16) : 0 : (long long)q_len(b) * H);
+        if (many(b)) return keep ? (long long)kpad(b) * Hkv * ((rows(b) + 15) / 16 * 16) : 0;
+        return (long long)kpad(b) * q_len(b) * H;
     }
     long long sums(int b) const { return many(b) ? (long long)Hkv * parts(b) * kpad(b) : 0; }
 };
@@ -157,7 +163,8 @@ double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double 
         const int chunks = ((p.n_rows[b] + unit - 1) / unit + c - 1) / c;
         for (int ci = 0; ci < chunks; ++ci) {
             for (int t = nt - 1; t >= 0; --t) {
-                const int keys = p.n_rows[b] - p.q_len(b) + (std::min(p.rows(b), (t + 1) * p.tile_rows(k)) - 1) / p.G + 1;
+                const int last = (std::min(p.rows(b), (t + 1) * p.tile_rows(k)) - 1) / p.G;  // the tile's last token
+                const int keys = p.n_rows[b] - p.q_len(b) + last + 1;
                 const int left = (keys + unit - 1) / unit - ci * c;
                 if (left <= 0) break;  // nor have the tiles before it
                 const double at = busy[0] + std::min(left, c) + extra;
@@ -177,11 +184,11 @@ double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double 
     return end;
 }
 
-// Steps of a workgroup of the split-operand kernel at most.  Keys are cut where whole row tiles would leave CUs idle or end unevenly: of
-// the whole and some cuts the one of the least estimated time (paged_span, and the partial sums' way to
-// memory and back: 0.011 steps each, a step being RT x 32 keys at 216 TFLOP/s against 4.7 TB/s).  Measured on MI355X (us,
-// chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8 heads at d = 128 139 / 91, three chunks of
-// 501 on 1850 to 2980 rows at d = 96 470 / 240.
+// Steps of a workgroup of the split-operand kernel at most.  Keys are cut where whole row tiles would leave CUs
+// idle or end unevenly: of the whole and some cuts the one of the least estimated time (paged_span, and the
+// partial sums' way to memory and back: 0.011 steps each, a step being RT x 32 keys at 216 TFLOP/s against 4.7 TB/s).
+// Measured on MI355X (us, chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8
+// heads at d = 128 139 / 89, a batch with three chunks of 501 on 1850 to 2980 rows at d = 96 513 / 301.
 int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
     // Two workgroups of four waves per CU where LDS holds both.
     const int slots = paged_shape(k, p.dp).nw == 4 && p.dp <= 192 ? 512 : 256;
@@ -207,11 +214,12 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
 }
 
 // Units of a workgroup of the streaming kernel at most: the least time by the same reckoning, one unit for a
-// workgroup's own start and end, as many workgroups at once as the kernel's registers let stand on the CUs.  Chunks are of one length within a sequence and not over all, so
-// that many workgroups count as an even share and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048
-// workgroups aimed at / this): 64 sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128 544 / 557 / 516 / 499, 16 of
-// half that with weights 91 / 89 / 93 / 89, 3 of 6000 rows with 8 tokens each 52 / 65 / 66 / 52, one of 100000 rows 159 /
-// 151 / 140 / 144.  (Chunks of 64 keys: 16 over 4 heads of 8192 rows at d = 256 40 instead of 32.)
+// workgroup's own start and end, as many workgroups at once as the kernel's registers let stand on the CUs.
+// Chunks are of one length within a sequence and not over all, so that many workgroups count as an even share
+// and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048 workgroups aimed at / this): 64
+// sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128 541 / 572 / 524 / 506, 16 of half that with weights
+// 89 / 92 / 88 / 85, 8 of 5200 to 8192 of 8 heads at d = 64 49 / 54 / 49 / 49, one of 100000 rows 158 / 161 / 154 /
+// 155.  (Chunks of 64 keys, half of the least: 16 over 4 heads of 8192 rows at d = 256 40 instead of 32.)
 int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
     const int wgs = tuned(kTunePagedWgs, 0), slots = p.dp <= 64 ? 1024 : p.dp <= 128 ? 768 : p.dp <= 192 ? 512 : 256;
     int best = longest;
@@ -245,13 +253,14 @@ PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hk
     PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0, true, true};
     int longest[kPagedKinds] = {};
     long long scores = 0, sums = 0, units = 0;
-    // 17 to 32 rows: with two blocks the streaming kernel's f32 MFMAs weigh as much as its reads, and past d = 128 its
-    // registers spill; where it cannot hide behind latency the split-operand kernel takes them.  Measured on MI355X
-    // (us, streaming / split operands; 32 rows): one sequence of 8192 rows of 32 over 8 heads at d = 128 33 / 36, 4 of 500 19.5 /
-    // 22.9, 16 of 2048 89 / 70, at d = 96 72 / 66; 16 of 2048 of 12 over 4 heads at d = 64 26 / 27, 16 over 4 at d = 256 281 / 95.
+    // 17 to 32 rows: with two blocks the streaming kernel's f32 MFMAs weigh as much as its reads, and past d =
+    // 128 its registers spill; where that does not hide behind latency the split-operand kernel takes them.
+    // Measured on MI355X (us, streaming / split operands; 32 rows): one sequence of 8192 rows of 32 over 8 heads at
+    // d = 128 33 / 36, 4 of 500 19.5 / 22.9, 16 of 2048 89 / 70, at d = 96 72 / 66; 16 of 2048 of 12 over 4 heads
+    // at d = 64 26 / 27, of 16 over 4 at d = 256 281 / 95.
     for (int b = 0; b < B; ++b)
         if (p.rows(b) > 16 && p.rows(b) <= 32) units += (long long)Hkv * ((n_rows[b] + 63) / 64);
-    p.two_blocks = p.dp <= 64 || (p.dp <= 128 && units <= 2048);  // four 64-key units to each workgroup that fits at once
+    p.two_blocks = p.dp <= 64 || (p.dp <= 128 && units <= 2048);  // (64 keys a unit: four to each of 512 workgroups)
     for (int b = 0; b < B; ++b) {
         if (!p.any(b)) continue;
         const PagedKind k = p.kind(b);
@@ -262,10 +271,11 @@ PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hk
         const PagedKind k = (PagedKind)ki;
         p.most[k] = !longest[k] ? 1 : paged_few(k) ? paged_few_limit(p, k, longest[k]) : paged_limit(p, k, longest[k]);
     }
-    // The split-operand kernel's scores are kept for the weights from d = 64 up while they take no more room than 4
-    // GiB (32 heads of 4096 tokens over 8192 rows), else formed again.  Measured on MI355X (attention and weights,
-    // us, kept / again): a prompt of 2048 rows of 32 over 8 heads at d = 128 340 / 392, 64 tokens on 4096 rows 66 / 80, 2048 rows of
-    // 16 over 4 at d = 256 364 / 482, 4 x 1024 of 8 heads at d = 64 96 / 95; 4096 rows of 4 over 2 at d = 32 165 / 144.
+    // The split-operand kernel's scores are kept for the weights from d = 64 up while they take no more room than
+    // 4 GiB (32 heads of 4096 tokens over 8192 rows), else formed again.  Measured on MI355X (attention and
+    // weights, us, kept / again): a prompt of 2048 rows of 32 over 8 heads at d = 128 339 / 388, 64 tokens on 4096
+    // rows 66 / 80, 4096 tokens on 8192 rows 2695 / 3048, 2048 rows of 16 over 4 at d = 256 366 / 478, 4 x 1024 of
+    // 8 heads at d = 64 96 / 95; 4096 rows of 4 over 2 at d = 32 165 / 143.
     p.keep = tuned(kTunePagedScores, p.dp >= 64 && scores <= 1LL << 30) == 1;
     for (int b = 0; b < B; ++b)
         if (p.many(b)) sums += (long long)p.rows(b) * Hkv * ((n_rows[b] + p.weight_keys() - 1) / p.weight_keys());
@@ -357,7 +367,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     // Launches `name` for the sequences that `items` has work items for, up to ZT_PAGED_MAXB at a time; per_wg items
     // to a workgroup.  `each(i, b)` fills in what else argument block x needs for its entry i, sequence b; each(-1, b)
     // comes behind every sequence.
-    const auto launch_for = [&](const char *name, unsigned threads, unsigned per_wg, auto &x, auto items, auto each) -> int {
+    const auto launch_for = [&](const char *name, unsigned threads, unsigned per_wg, auto &x, auto items,
+                                auto each) -> int {
         const long long most = 0xFFFFFFFFll / threads * per_wg;  // items whose work-items fit a grid
         long long blocks = 0;
         PagedSeqs &s = x.seq;
@@ -416,7 +427,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         const bool by_rows = !few && chunks <= 8;
         // (Few rows' weights come with it, where they are wanted: 1024 keys to a workgroup.)
         const bool with = weights && few;
-        snprintf(name, sizeof name, by_rows ? "zt_paged_merge_rows_d%d" : with ? "zt_paged_merge_w_d%d" : "zt_paged_merge_d%d", dp);
+        snprintf(name, sizeof name,
+                 by_rows ? "zt_paged_merge_rows_d%d" : with ? "zt_paged_merge_w_d%d" : "zt_paged_merge_d%d", dp);
         const auto merged = [&](int b) {
             const long long sums = with ? (long long)((n_rows[b] + 1023) / 1024) * n_kv_heads : 0;
             return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads + sums : 0LL;
@@ -494,7 +506,8 @@ int zt_paged_append(const float *q, const float *k_new, const float *v_new, floa
     a.q = q; a.k_new = k_new; a.v_new = v_new; a.q_out = q_out; a.w = w;
     a.H = n_heads; a.Hkv = n_kv_heads; a.dim = dim; a.w_stride = w_stride; a.theta = theta;
     const int per = std::min(16, 256 / (dim / 2));  // tokens of a workgroup
-    const int vw = dim % 8 == 0 ? 4 : dim % 4 == 0 ? 2 : 1;  // pairs of a thread: both halves of a head in whole chunks of that
+    // Pairs of a thread: both halves of a head in whole chunks of that.
+    const int vw = dim % 8 == 0 ? 4 : dim % 4 == 0 ? 2 : 1;
     const long long tasks = ((q ? n_heads : 0) + 2LL * n_kv_heads) * (dim / 2) / vw;
     char name[64];
     snprintf(name, sizeof name, "zt_rope_paged_%d", vw);
