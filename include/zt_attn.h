@@ -223,9 +223,9 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
  * of table_out's pages, and their weights w_out's.  kept [B, n_kv_heads, budget]
  * (device ints) receives the row that each was, -1 past a sequence's last.  A sequence within the
  * budget keeps all rows.  The sequence's new n_rows is min(n_rows, budget).
- * table_out is table (in place: the sequences' pages must not be shared) or
- * another table of the same stride, none of whose pages is in table (a copy: table's
- * pages, which may be shared, stay as they are); w_out is w_in or a buffer that
+ * table_out is table, the same pointer (in place: the sequences' pages must not be
+ * shared), or another table of the same stride, none of whose pages is in table (a
+ * copy: table's pages, which may be shared, stay as they are); w_out is w_in or a buffer that
  * does not overlap it. */
 int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *table_out, const float *w_in,
                    float *w_out, int *kept, const int *n_rows, int B, int n_pages, int page_size, int table_stride,

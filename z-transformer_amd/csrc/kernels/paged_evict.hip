@@ -58,7 +58,8 @@ DEVI int wave_scan(int v) {
 // two sums over the waves place every row.
 //   KPT 0, any number: w is read again for every digit, and rows are placed 64 NW at a time, in order.
 // w may be compacted in place: what a step overwrites has been read, since a row never moves up.
-// Latency: 8192 rows take 72 us by single bits that read w again, 39 by two bits, counted by ballots, from registers.
+// Bound: latency, a few trips through LDS to a digit: 128 heads of up to 8192 rows 13 us (72 by single bits that read
+// w again, 39 by two bits at a time, counted by ballots, from registers).
 template <int NW, int KPT>
 DEVI void evict_select(const PagedEvictArgs &a) {
     constexpr int NTH = 64 * NW, BINS = 2048, BPT = BINS / NTH;
