@@ -889,6 +889,25 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_weights(PagedWeightAr
         if (key + e < n) a.w_out[at + e] = a.w_in[at + e] + sum[e];
 }
 
+// Sums of consecutive keys (N of them, some possibly past the last) over a part of the rows: to the part's
+// place, or, where there is one part only, to the weights.
+template <class V>
+DEVI void put_part(const PagedWeightArgs &a, const PagedSeq &sq, int kvh, int nparts, int part, int key, V sum) {
+    constexpr int N = sizeof(V) / sizeof(float);
+    if (nparts == 1) {
+        const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float x;
+            if constexpr (N == 1) x = sum; else x = sum[e];
+            if (key + e < sq.n_rows) a.w_out[at + e] = a.w_in[at + e] + x;
+        }
+    } else if (key < sq.n_rows) {  // (a whole f4 fits: the parts' rows are padded to 16 keys)
+        const int kpad = (sq.n_rows + 15) & ~15;
+        *reinterpret_cast<V *>(a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * kpad + key) = sum;
+    }
+}
+
 // Many rows: from the tiles that the attention stored.  A workgroup takes 128 keys of one
 // (sequence, kv head) and a part of the rows; a wave two neighbouring key tiles, 2 KB a row tile, four
 // row tiles in flight: lane (l16, grp) adds row l16's weights of keys 4 grp .. 4 grp + 3 over the row
@@ -951,8 +970,7 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[i][e] += wave_xor(sum[i][e], m);
     if (l16 > 1 || (l16 == 1 && !two)) return;
-    float *out = a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * 16 * ktiles + k0;
-    *reinterpret_cast<f4 *>(out + 16 * l16 + 4 * grp) = l16 ? sum[1] : sum[0];
+    put_part(a, sq, kvh, nparts, part, k0 + 16 * l16 + 4 * grp, l16 ? sum[1] : sum[0]);
 }
 
 // Many rows whose scores are not kept: the scores again, on split operands.  A workgroup takes one (sequence, kv
@@ -1144,17 +1162,14 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
         }
         __syncthreads();
     }
-    const int kpad = (n + 15) & ~15;
-    float *out = a.parts + a.parts0[sq.i] + ((size_t)kvh * nparts + part) * kpad;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
         const float sum = sum4grp(acc[i]);
-        const int key = k0 + 16 * i + l16;
-        if (grp == 0 && key < n) out[key] = sum;
+        if (grp == 0) put_part(a, sq, kvh, nparts, part, k0 + 16 * i + l16, sum);
     }
 }
 
-// The parts of the rows, added in order.
+// The parts of the rows, where there are several, added in order.
 template <int KT>
 DEVI void paged_wsum(const PagedWeightArgs &a) {
     const PagedSeq sq = paged_seq(a.seq, blockIdx.x);

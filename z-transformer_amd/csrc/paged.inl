@@ -144,7 +144,7 @@ struct PagedPlan {
         if (many(b)) return keep ? (long long)kpad(b) * Hkv * ((rows(b) + 15) / 16 * 16) : 0;
         return (long long)kpad(b) * q_len(b) * H;
     }
-    long long sums(int b) const { return many(b) ? (long long)Hkv * parts(b) * kpad(b) : 0; }
+    long long sums(int b) const { return many(b) && parts(b) > 1 ? (long long)Hkv * parts(b) * kpad(b) : 0; }
 };
 
 // When the last workgroup of kind k ends, in steps, were `limit` the most steps of one: the kernel's order of
@@ -467,7 +467,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     const auto parts = [&](int b) { return per_head(b, p.weight_keys()) * p.parts(b); };
     if (run(name, p.keep ? 256u : 64u * p.weight_waves(), true, parts)) return 1;
     snprintf(name, sizeof name, "zt_paged_wsum_%d", p.weight_keys());
-    return run(name, 256u, true, [&](int b) { return per_head(b, 256); });
+    return run(name, 256u, true, [&](int b) { return p.parts(b) > 1 ? per_head(b, 256) : 0LL; });
 }
 
 int zt_paged_append(const float *q, const float *k_new, const float *v_new, float *q_out, float *k_pages, float *v_pages,
