@@ -115,6 +115,24 @@ def test_forced_variants(gpu, zt, tune, settings, H, Hkv, d):
     grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
 
 
+@pytest.mark.parametrize("H,Hkv,d", [(4, 2, 32), (8, 2, 64), (6, 2, 50), (8, 2, 96), (32, 8, 128), (8, 2, 192), (16, 4, 256)])
+def test_a_batch_and_its_sequences_alone(gpu, zt, H, Hkv, d):
+    """Few and many new tokens in one call, whose short sequences share a launch, and each of them in a call of its own."""
+    n_rows, q_len, page = [300, 77, 9, 140, 33, 1, 260], [1, 4, 8, 9, 33, 1, 130], 8
+    rng = np.random.default_rng([H, d, 7])
+    c = Cache(gpu, rng, n_rows, page, Hkv, d, garbage=np.nan)
+    q_start = np.cumsum([1] + q_len).tolist()
+    q = rng.standard_normal((q_start[-1] + 2, H, d)).astype(np.float32)
+    w = rng.random((len(n_rows), Hkv, max(n_rows) + 5), np.float32)
+    ref = pagedref.attend(q, c.k_h, c.v_h, c.table_h, q_start, n_rows, page, H, Hkv, d)
+    grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
+    table = c.table
+    for b, n in enumerate(n_rows):
+        c.table, c.n_rows = table[b:b + 1].contiguous(), [n]
+        mine = [x[b:b + 1] if i in (2, 4) else x for i, x in enumerate(ref)]
+        grade(run_attend(gpu, zt, c, q, q_start[b:b + 2], H, w[b:b + 1]), mine, q_start[b:b + 2], [n], Hkv, w[b:b + 1])
+
+
 def test_more_sequences_than_a_launch_takes(gpu, zt):
     B, H, Hkv, d, page = 150, 4, 2, 32, 8
     rng = np.random.default_rng(5)

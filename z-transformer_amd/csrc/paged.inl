@@ -101,15 +101,17 @@ constexpr PagedShape paged_shape(PagedKind k, int dp) {
 struct PagedPlan {
     const int *q_start, *n_rows;
     int B, H, Hkv, G, dim, dp, part_ld;
-    int most[kPagedKinds];  // units of keys (unit()) of a workgroup at most
-    int part_rows;          // rows of a part of the weights' sums
-    bool keep;              // the split-operand kernel stores its scores for the weights
-    bool two_blocks;        // the streaming kernel takes 17 to 32 rows
+    PagedKind as[kPagedKinds];  // the kind whose launch takes each (itself, or a larger one)
+    int most[kPagedKinds];      // units of keys (unit()) of a workgroup at most
+    int part_rows;              // rows of a part of the weights' sums
+    bool keep;                  // the split-operand kernel stores its scores for the weights
+    bool two_blocks;            // the streaming kernel takes 17 to 32 rows
 
     int q_len(int b) const { return q_start[b + 1] - q_start[b]; }
     int rows(int b) const { return q_len(b) * G; }
     bool any(int b) const { return q_len(b) > 0; }
-    PagedKind kind(int b) const {
+    PagedKind kind(int b) const { return as[kind_of(b)]; }
+    PagedKind kind_of(int b) const {
         const int r = rows(b);
         return r <= 16                ? kFew1
                : r <= 32 && two_blocks ? kFew2
@@ -146,6 +148,13 @@ struct PagedPlan {
     }
     long long sums(int b) const { return many(b) && parts(b) > 1 ? (long long)Hkv * parts(b) * kpad(b) : 0; }
 };
+
+// Workgroups of a kind on the device at once: as many of the streaming kernel as its registers let stand on the CUs;
+// of the split-operand kernel two of four waves per CU where LDS holds both, else one.
+int paged_slots(const PagedPlan &p, PagedKind k) {
+    if (paged_few(k)) return p.dp <= 64 ? 1024 : p.dp <= 128 ? 768 : p.dp <= 192 ? 512 : 256;
+    return paged_shape(k, p.dp).nw == 4 && p.dp <= 192 ? 512 : 256;
+}
 
 // When the last workgroup of kind k ends, in steps, were `limit` the most steps of one: the kernel's order of
 // items, each to whichever of the device's places (`slots` workgroups) is free first, a workgroup's own
@@ -190,8 +199,7 @@ double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double 
 // Measured on MI355X (us, chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8
 // heads at d = 128 139 / 89, a batch with three chunks of 501 on 1850 to 2980 rows at d = 96 513 / 301.
 int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
-    // Two workgroups of four waves per CU where LDS holds both.
-    const int slots = paged_shape(k, p.dp).nw == 4 && p.dp <= 192 ? 512 : 256;
+    const int slots = paged_slots(p, k);
     const double extra = 3, way = 0.011;
     const int least = 4;
     int best = longest;
@@ -214,14 +222,14 @@ int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
 }
 
 // Units of a workgroup of the streaming kernel at most: the least time by the same reckoning, one unit for a
-// workgroup's own start and end, as many workgroups at once as the kernel's registers let stand on the CUs.
+// workgroup's own start and end.
 // Chunks are of one length within a sequence and not over all, so that many workgroups count as an even share
 // and half a workgroup besides.  Measured on MI355X (us; 512 / 1024 / 2048 workgroups aimed at / this): 64
 // sequences of 4096 to 8192 rows, 32 over 8 heads at d = 128 541 / 572 / 524 / 506, 16 of half that with weights
 // 89 / 92 / 88 / 85, 8 of 5200 to 8192 of 8 heads at d = 64 49 / 54 / 49 / 49, one of 100000 rows 158 / 161 / 154 /
 // 155.  (Chunks of 64 keys, half of the least: 16 over 4 heads of 8192 rows at d = 256 40 instead of 32.)
 int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
-    const int wgs = tuned(kTunePagedWgs, 0), slots = p.dp <= 64 ? 1024 : p.dp <= 128 ? 768 : p.dp <= 192 ? 512 : 256;
+    const int wgs = tuned(kTunePagedWgs, 0), slots = paged_slots(p, k);
     int best = longest;
     double time = 0;
     for (int limit = 2; limit <= longest; limit += (limit + 3) / 4) {
@@ -249,8 +257,38 @@ int paged_few_limit(const PagedPlan &p, PagedKind k, int longest) {
     return best;
 }
 
+// A kind of few steps joins the next larger kind of the batch, whose empty rows cost less than a launch more (two,
+// with a merge), while the workgroups of both are on the device at once and their steps of 32 keys few for each
+// place: 7 of the split-operand kernel, 4 of the streaming one.  Measured on MI355X (us, a launch for each /
+// joined): every fourth of 12 sequences with 40 new tokens, the others one, 32 over 8 heads at d = 128, 60 rows 26.6
+// / 20.9, 200 (2 steps of each place) 46 / 41, 500 (4) 54 / 51; 900, 16 over 4 at d = 256 (7) 68 / 61; 1800 (13) 92
+// / 97, at d = 128 82 / 135; 100 sequences of 60 rows (800 workgroups) 36 / 46.  Every fourth of 16 with 6 tokens,
+// 500 rows (3) 37 / 28, 900 (5) 44 / 50.
+void paged_join(PagedPlan &p) {
+    long long wgs[kPagedKinds] = {}, steps[kPagedKinds] = {};
+    for (int b = 0; b < p.B; ++b) {
+        if (!p.any(b)) continue;
+        const long long n = (long long)p.tiles(b) * p.Hkv;
+        wgs[p.kind(b)] += n;
+        steps[p.kind(b)] += n * ((p.n_rows[b] + 31) / 32);
+    }
+    for (int k = 0; k + 1 < kPagedKinds; ++k) {
+        int larger = k + 1;
+        while (larger < kPagedKinds && !wgs[larger]) ++larger;
+        if (!wgs[k] || larger == kPagedKinds) continue;
+        const int slots = paged_slots(p, (PagedKind)larger);
+        if (wgs[k] + wgs[larger] > slots || steps[k] + steps[larger] > (paged_few((PagedKind)larger) ? 4 : 7) * slots)
+            continue;
+        wgs[larger] += wgs[k];
+        steps[larger] += steps[k];
+        for (PagedKind &as : p.as)
+            if (as == k) as = (PagedKind)larger;
+    }
+}
+
 PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hkv, int dim) {
-    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, 0, true, true};
+    PagedPlan p{q_start, n_rows, B, H, Hkv, H / Hkv, dim, paged_dp(dim), (dim + 3) / 4 * 4, {}, {}, 0, true, true};
+    for (int k = 0; k < kPagedKinds; ++k) p.as[k] = (PagedKind)k;
     int longest[kPagedKinds] = {};
     long long scores = 0, sums = 0, units = 0;
     // 17 to 32 rows: with two blocks the streaming kernel's f32 MFMAs weigh as much as its reads, and past d =
@@ -261,6 +299,7 @@ PagedPlan paged_plan(const int *q_start, const int *n_rows, int B, int H, int Hk
     for (int b = 0; b < B; ++b)
         if (p.rows(b) > 16 && p.rows(b) <= 32) units += (long long)Hkv * ((n_rows[b] + 63) / 64);
     p.two_blocks = p.dp <= 64 || (p.dp <= 128 && units <= 2048);  // (64 keys a unit: four to each of 512 workgroups)
+    paged_join(p);
     for (int b = 0; b < B; ++b) {
         if (!p.any(b)) continue;
         const PagedKind k = p.kind(b);
