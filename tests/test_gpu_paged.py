@@ -616,3 +616,31 @@ def test_a_serving_run(gpu, zt, H, Hkv, d, page):
                     k_ref[b][h], v_ref[b][h] = k_ref[b][h][want], v_ref[b][h][want]
             n = [min(x, budget) for x in n]
     assert pos[0] > limit  # it did evict
+
+
+@pytest.mark.parametrize("scores", [0, 1])
+@pytest.mark.parametrize("L", [12, 40, 150])
+@pytest.mark.parametrize("H,Hkv,d", [(4, 2, 32), (8, 2, 64), (6, 2, 50), (8, 2, 128), (4, 1, 192), (4, 1, 256)])
+def test_a_page_of_no_pool_beside_large_values(gpu, zt, tune, H, Hkv, d, L, scores):
+    """The 32-key tile of the page's keys holds a K value past 2^40 too, and a few query rows hold one: every row that
+    sees the page is NaN, those with ordinary values among them; the rest, and the other sequence, as without it."""
+    page, n, bad, big = 8, 200, 23, np.float32(2.0 ** 45)
+    first = bad * page  # rows 184 .. 191 have no page; the large key is row 168, of the tile 160 .. 191
+    rng = np.random.default_rng([H, d, L])
+    c = Cache(gpu, rng, [n, n], page, Hkv, d)
+    q = rng.standard_normal((2 * L, H, d)).astype(np.float32)
+    q[:, :, 5] /= big
+    c.k_h[pagedref.places(c.table_h, 1, n, page)[168], :, 5] *= big
+    q[1::7, :, d - 2] *= big
+    c.k_h[:, :, d - 2] /= big
+    c.k = gpu.from_numpy(c.k_h).cuda()
+    q_start, w = [0, L, 2 * L], np.zeros((2, Hkv, n), np.float32)
+    tune({"ZT_PAGED_SCORES": scores})
+    good = run_attend(gpu, zt, c, q, q_start, H, w)
+    assert all(np.all(np.isfinite(x)) for x in good)
+    c.table[1, bad] = c.n_pages
+    out, lse, w1 = run_attend(gpu, zt, c, q, q_start, H, w)
+    see = L + max(0, first - (n - L))  # the first token that sees the page
+    assert np.array_equal(out[:see], good[0][:see]) and np.array_equal(lse[:see], good[1][:see])
+    assert np.all(np.isnan(out[see:])) and np.all(np.isnan(lse[see:]))
+    assert np.array_equal(w1[0], good[2][0]) and np.all(np.isnan(w1[1]))

@@ -576,11 +576,11 @@ DEVI void paged_many(const PagedArgs &a) {
                     for (int i = 0; i < 2 * NQ; ++i) s[i] = zero4();
                 }
                 const int ll = opaque(lane), lrow = ll & 15, lgrp = ll >> 4;
-                const float *krow[2], *qrow[NQ];
+                const float *krow[2], *qrow[NQ];  // (null: a key without a page, NaN here as where it was staged)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int r = pool_row(a.pool, table, min(k0 + 16 * j + lrow, key1 - 1));
-                    krow[j] = kb + (size_t)max(r, 0) * kld;
+                    krow[j] = r < 0 ? nullptr : kb + (size_t)r * kld;
                 }
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
@@ -593,7 +593,7 @@ DEVI void paged_many(const PagedArgs &a) {
                     float kv[2], qv[NQ];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        kv[j] = FULL || col < a.dim ? krow[j][col] : 0.f;
+                        kv[j] = !krow[j] ? __builtin_nanf("") : FULL || col < a.dim ? krow[j][col] : 0.f;
                         if (!qbig) kv[j] = big_part(kv[j]);
                     }
 #pragma unroll
@@ -1008,19 +1008,19 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
     const int k0 = kt0 + 16 * NK * w;  // the wave's first key
     Tri k[NKS][NK];
     float acc[NK], kmax = 0.f;
-    const float *krow[NK];
+    const float *krow[NK];  // (null: a key without a page, whose scores are NaN)
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
         acc[i] = 0.f;
         const int r = pool_row(a.pool, table, min(k0 + 16 * i + l16, n - 1));
-        krow[i] = kb + (size_t)max(r, 0) * kld;
+        krow[i] = r < 0 ? nullptr : kb + (size_t)r * kld;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
             float y[8];
 #pragma unroll
             for (int h = 0; h < 8; h += 4) {
                 float z[4];
-                load_cols<4, FULL, false>(z, krow[i], 32 * ks + 8 * grp + h, a.dim, vec4);
+                load_cols<4, FULL, false>(z, kb + (size_t)max(r, 0) * kld, 32 * ks + 8 * grp + h, a.dim, vec4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[h + e] = r < 0 ? __builtin_nanf("") : z[e];
             }
@@ -1124,7 +1124,7 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
                 float kv[NK], qv[2];
 #pragma unroll
                 for (int i = 0; i < NK; ++i) {
-                    kv[i] = col < a.dim ? krow[i][col] : 0.f;
+                    kv[i] = !krow[i] ? __builtin_nanf("") : col < a.dim ? krow[i][col] : 0.f;
                     if (!qbig) kv[i] = big_part(kv[i]);
                 }
 #pragma unroll
