@@ -644,3 +644,40 @@ def test_a_page_of_no_pool_beside_large_values(gpu, zt, tune, H, Hkv, d, L, scor
     assert np.array_equal(out[:see], good[0][:see]) and np.array_equal(lse[:see], good[1][:see])
     assert np.all(np.isnan(out[see:])) and np.all(np.isnan(lse[see:]))
     assert np.array_equal(w1[0], good[2][0]) and np.all(np.isnan(w1[1]))
+
+
+def test_eviction_of_a_long_sequence_among_short_ones(gpu, zt):
+    """64 sequences, one of 262200 rows: a workgroup for each row of the longest, had every sequence as many, would be
+    more than a launch takes.  Only the first and the last page of the long one are there."""
+    B, Hkv, d, page, n, budget, drop = 64, 9, 256, 64, 262200, 262190, (100, 110)
+    n_rows = [5] * B
+    n_rows[37] = n
+    stride = -(-n // page)
+    pages = 2 * (B + 1)  # in and out, two of the long sequence
+    k, v = (gpu.randn(pages * page, Hkv, d, device="cuda") for _ in range(2))
+    tables = []
+    for at in (0, B + 1):
+        t = gpu.full((B, stride), -1, dtype=gpu.int32)
+        t[:, 0] = at + gpu.arange(B, dtype=gpu.int32)
+        t[37, stride - 1] = at + B
+        tables.append(t.cuda())
+    w = gpu.ones(B, Hkv, n, device="cuda")
+    w[37, :, drop[0]:drop[1]] = 0
+    kept = gpu.full((B, Hkv, budget), -7, device="cuda", dtype=gpu.int32)
+    want_k, want_v = k.clone(), v.clone()
+    zt.paged_evict(k, v, *tables, w, w, kept, n_rows, page, Hkv, d, 0, 0, budget)
+    stay = gpu.cat((gpu.arange(drop[0]), gpu.arange(drop[1], n))).int().cuda()
+    for b in range(B):
+        if b == 37:
+            assert gpu.equal(kept[b], stay.expand(Hkv, budget)) and gpu.all(w[b, :, :budget] == 1)
+        else:
+            assert gpu.equal(kept[b, :, :5], gpu.arange(5, device="cuda", dtype=gpu.int32).expand(Hkv, 5))
+            assert gpu.all(kept[b, :, 5:] == -1)
+    out0, tail0 = (B + 1) * page, (stride - 1) * page  # the copies' first row; the last page's first
+    for x, y in ((want_k, k), (want_v, v)):
+        for b in range(B):
+            m = page if b == 37 else 5
+            x[out0 + b * page:out0 + b * page + m] = x[b * page:b * page + m]
+        gone, m = drop[1] - drop[0], budget - tail0  # rows of the last page that get one of the same page
+        x[out0 + B * page:out0 + B * page + m] = x[B * page + gone:B * page + gone + m]
+        assert gpu.equal(x, y)

@@ -594,6 +594,19 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
     a.Hkv = n_kv_heads; a.dim = dim; a.w_stride = w_stride;
     a.n_first = n_first; a.n_last = n_last; a.budget = budget;
     const int n = dim % 4 == 0 ? 4 : 2, per_head = dim / n;
+    const bool in_place = table_out == table;
+    const char *const move = in_place ? n == 4 ? "zt_evict_move_4" : "zt_evict_move_2"
+                                      : n == 4 ? "zt_evict_copy_4" : "zt_evict_copy_2";
+    const unsigned move_threads = in_place ? 1024 : kThreads;
+    const int rows_per_wg = std::max(1, 1024 / (n_kv_heads * per_head));  // of a copy
+    // Workgroups that move a sequence of `most` rows at most: K and V of each head, or its row tiles.
+    const auto move_wgs = [&](int most) {
+        return in_place ? 2LL * n_kv_heads : ((long long)std::min(budget, most) + rows_per_wg - 1) / rows_per_wg;
+    };
+    const long long move_most = 0xFFFFFFFFll / move_threads;  // workgroups of a launch
+    // All is refused before anything is launched.
+    for (int b = 0; b < B; ++b)
+        if (n_rows[b] && move_wgs(n_rows[b]) > move_most) return !grid_ok(move_wgs(n_rows[b]), move_threads);
     for (int b0 = 0; b0 < B; b0 += ZT_PAGED_MAXB) {
         a.b0 = b0;
         a.ns = std::min(B - b0, ZT_PAGED_MAXB);
@@ -606,21 +619,18 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
         const char *select = most <= 1024 ? "zt_evict_select_1024" : most <= 4096 ? "zt_evict_select_4096"
                              : most <= 16384 ? "zt_evict_select_16384" : "zt_evict_select_any";
         const unsigned threads = most <= 1024 ? 256 : most <= 4096 ? 512 : 1024;
-        if (!grid_ok((unsigned long long)a.ns * n_kv_heads, threads)) return 1;
+        static_assert(ZT_PAGED_MAXB * 65535ull * 1024 <= 0xFFFFFFFFull, "a launch has room for every head's workgroup");
         if (launch(st, select, (unsigned)(a.ns * n_kv_heads), a, stream, threads)) return 1;
-        // Same stream: the rows move as `kept` says.
-        if (table_out == table) {
-            if (most <= budget) continue;
-            const unsigned long long blocks = (unsigned long long)a.ns * n_kv_heads * 2;  // K and V
-            if (!grid_ok(blocks, 1024)) return 1;
-            if (launch(st, n == 4 ? "zt_evict_move_4" : "zt_evict_move_2", (unsigned)blocks, a, stream, 1024)) return 1;
-        } else {
-            const int rows_per_wg = std::max(1, 1024 / (n_kv_heads * per_head));
-            a.tiles = (std::min(budget, most) + rows_per_wg - 1) / rows_per_wg;
-            const unsigned long long blocks = (unsigned long long)a.ns * a.tiles;
-            if (most == 0) continue;
-            if (!grid_ok(blocks)) return 1;
-            if (launch(st, n == 4 ? "zt_evict_copy_4" : "zt_evict_copy_2", (unsigned)blocks, a, stream)) return 1;
+        if (in_place ? most <= budget : most == 0) continue;
+        // Same stream: the rows move as `kept` says.  As many sequences at a time as a launch has room for, each counted
+        // as the longest.
+        a.tiles = in_place ? 0 : (int)move_wgs(most);
+        const int at_once = (int)std::min<long long>(a.ns, move_most / move_wgs(most));
+        for (int i0 = 0, ns = a.ns; i0 < ns; i0 += at_once) {
+            a.b0 = b0 + i0;
+            a.ns = std::min(ns - i0, at_once);
+            for (int i = 0; i < a.ns; ++i) a.n_rows[i] = n_rows[a.b0 + i];
+            if (launch(st, move, (unsigned)(a.ns * move_wgs(most)), a, stream, move_threads)) return 1;
         }
     }
     return 0;
