@@ -681,3 +681,24 @@ def test_eviction_of_a_long_sequence_among_short_ones(gpu, zt):
         gone, m = drop[1] - drop[0], budget - tail0  # rows of the last page that get one of the same page
         x[out0 + B * page:out0 + B * page + m] = x[B * page + gone:B * page + gone + m]
         assert gpu.equal(x, y)
+
+
+def test_append_of_more_tokens_than_one_launch_takes(gpu, zt):
+    """2^25 + 77 tokens of d = 256, two to a workgroup.  Only the first and the last page are there."""
+    Hkv, d, page, N = 1, 256, 1024, (1 << 25) + 77
+    table = gpu.full((1, -(-N // page)), -1, device="cuda", dtype=gpu.int32)
+    table[0, 0], table[0, -1] = 1, 0
+    pool_k, pool_v = (gpu.zeros(2 * page, Hkv, d, device="cuda") for _ in range(2))
+    new = gpu.empty(N, Hkv, d, device="cuda")
+    new[:page].normal_()
+    new[-77:].normal_()
+    w = gpu.ones(1, Hkv, N, device="cuda")
+    zt.paged_append(None, new, new, None, pool_k, pool_v, table, [0, N], [N], [0], page, 1, Hkv, d, w=w)
+    assert not gpu.any(w)
+    for rows, at, pos in ((new[:page], page, 0), (new[-77:], 0, N - 77)):
+        n = len(rows)
+        want = gpu.empty_like(rows)
+        zt.rope_qk(rows.contiguous(), rows.contiguous(), want, gpu.empty_like(rows), 1, n, 1, 1, d, pos=pos)
+        assert gpu.equal(pool_v[at:at + n], rows) and gpu.equal(pool_k[at:at + n], want)
+    del new, rows
+    gpu.cuda.empty_cache()

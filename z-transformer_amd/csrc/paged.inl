@@ -550,21 +550,23 @@ int zt_paged_append(const float *q, const float *k_new, const float *v_new, floa
     const long long tasks = ((q ? n_heads : 0) + 2LL * n_kv_heads) * (dim / 2) / vw;
     char name[64];
     snprintf(name, sizeof name, "zt_rope_paged_%d", vw);
+    const int most = (int)(0xFFFFFFFFu / kThreads) * per;  // tokens of a launch
     for (int b = 0; b < B;) {
         a.ns = 0;
-        a.token0 = q_start[b];
+        const int first = q_start[b];
         for (; b < B && a.ns < ZT_PAGED_MAXB; ++b) {
             const int q_len = q_start[b + 1] - q_start[b];
             if (q_len == 0) continue;
             const int i = a.ns++;
             a.b[i] = b; a.q0[i] = q_start[b]; a.row0[i] = n_rows[b] - q_len; a.pos[i] = pos[b];
         }
-        a.tokens = q_start[b] - a.token0;
-        if (a.tokens == 0) continue;
-        const long long groups = (a.tokens + per - 1) / per;
-        a.slices = (int)std::max(1LL, std::min(512 / groups, (std::min(a.tokens, per) * tasks + kThreads - 1) / kThreads));
-        if (!grid_ok((unsigned long long)groups * a.slices)) return 1;
-        if (launch(st, name, (unsigned)(groups * a.slices), a, stream)) return 1;
+        for (long long t = first; t < q_start[b]; t += most) {
+            a.token0 = (int)t;
+            a.tokens = (int)std::min<long long>(most, q_start[b] - t);
+            const long long groups = ((long long)a.tokens + per - 1) / per;
+            a.slices = (int)std::max(1LL, std::min(512 / groups, (std::min(a.tokens, per) * tasks + kThreads - 1) / kThreads));
+            if (launch(st, name, (unsigned)(groups * a.slices), a, stream)) return 1;
+        }
     }
     return 0;
 }
