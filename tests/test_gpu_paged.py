@@ -702,3 +702,36 @@ def test_append_of_more_tokens_than_one_launch_takes(gpu, zt):
         assert gpu.equal(pool_v[at:at + n], rows) and gpu.equal(pool_k[at:at + n], want)
     del new, rows
     gpu.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("d", [32, 128])
+def test_weights_of_very_many_rows(gpu, zt, tune, d):
+    """131072 tokens of eight heads over one, whose weight goes to the first key (0.65) and the second: sums of 2^20
+    rows, formed again part by part.  All other keys have score -60.
+
+    Tolerance, of a sum of positive terms, in half steps of f32: a weight's own error is its score's, 2 (d + 4) |s| at |s| <=
+    0.62, and 24 for the exponential (2), the difference with the base (1), the row's sum (two terms, with a rescaling for
+    each of a few bases, 12), its inverse (3), the product and storing (6).  A lane adds at most 128 sums of four (3 roundings)
+    in 32 bits before it goes on to a wider sum, whose result is rounded once, as are those over 4 lane groups
+    (2), the parts' and w_in's: 128 + 3 + 1 + 2 + 1 + 1.  The number of rows is not in it."""
+    T, H, Hkv, page = 131072, 8, 1, 64
+    s = np.array([np.log(0.65 / 0.35), 0.0, -60.0], np.float32)
+    q0 = np.float32(np.sqrt(d))
+    k = gpu.zeros(T, d, device="cuda")
+    k[:, 0] = float(s[2])
+    k[0, 0], k[1, 0] = float(s[0]), float(s[1])
+    q = gpu.zeros(T, H * d, device="cuda")
+    q.view(T, H, d)[:, :, 0] = float(q0)
+    v, out = gpu.ones(T, d, device="cuda"), gpu.empty(T, H * d, device="cuda")
+    table = gpu.arange(T // page, device="cuda", dtype=gpu.int32)[None].contiguous()
+    w_in, w_out = gpu.zeros(1, 1, T, device="cuda"), gpu.empty(1, 1, T, device="cuda")
+    tune({"ZT_PAGED_SCORES": 0})
+    ws = gpu.empty(zt.attn_paged_workspace_bytes([0, T], [T], H, Hkv, d, True), device="cuda", dtype=gpu.uint8)
+    zt.attn_paged(q, k, v, table, out, [0, T], [T], page, H, Hkv, d, ws, w_in=w_in, w_out=w_out)
+    got = w_out[0, 0, :2].cpu().numpy().astype(np.float64)
+    e = np.exp(s.astype(np.float64) * float(q0) / np.sqrt(d))
+    t = np.arange(1, T)
+    total = e[0] + e[1] + (t - 1) * e[2]
+    want = H * np.array([1 + (e[0] / total).sum(), (e[1] / total).sum()])
+    bound = (2 * (d + 4) * 0.62 + 24 + 136) * EPS
+    assert np.all(np.abs(got / want - 1) <= bound), (got / want - 1, bound)

@@ -977,7 +977,8 @@ extern "C" __global__ void __launch_bounds__(256) zt_paged_wcols(PagedWeightArgs
 // head, tile of 16 NK NW keys, part of the rows); a wave holds 16 NK keys (K's parts in registers), and Q
 // passes through LDS in 32-row tiles, split once for all waves, two buffers, beside the rows'
 // statistics.  S = Q K^T has a key per lane and four rows, so that the sum over rows
-// stays in the lane until the end.
+// stays in the lane until the end: in 32 bits over 64 tiles, those sums in 64 bits, so that
+// its error does not grow with the rows (2^20 rows of weight 0.65 in 32 bits alone were off by 3.3e-4).
 template <int DP, int NW, int NK, bool FULL>
 DEVI void paged_wparts(const PagedWeightArgs &a) {
     constexpr int NKS = DP / 32, NTH = 64 * NW, TILE = split_bytes(DP, 32), KT = 16 * NK * NW;
@@ -1008,10 +1009,12 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
     const int k0 = kt0 + 16 * NK * w;  // the wave's first key
     Tri k[NKS][NK];
     float acc[NK], kmax = 0.f;
+    double total[NK];
     const float *krow[NK];  // (null: a key without a page, whose scores are NaN)
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
         acc[i] = 0.f;
+        total[i] = 0.0;
         const int r = pool_row(a.pool, table, min(k0 + 16 * i + l16, n - 1));
         krow[i] = r < 0 ? nullptr : kb + (size_t)r * kld;
 #pragma unroll
@@ -1156,6 +1159,13 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
                 acc[i] += sum;
             }
         }
+        if ((id & 63) == 63) {
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                total[i] += acc[i];
+                acc[i] = 0.f;
+            }
+        }
         if (id + 1 < nsteps) {
             put(id + 1);
             if (id + 2 < nsteps) fetch(rt + 64);
@@ -1164,12 +1174,12 @@ DEVI void paged_wparts(const PagedWeightArgs &a) {
     }
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-        const float sum = sum4grp(acc[i]);
+        const float sum = sum4grp((float)(total[i] + acc[i]));
         if (grp == 0) put_part(a, sq, kvh, nparts, part, k0 + 16 * i + l16, sum);
     }
 }
 
-// The parts of the rows, where there are several, added in order.
+// The parts of the rows, where there are several (2048 or so at most), added in order, in 64 bits.
 template <int KT>
 DEVI void paged_wsum(const PagedWeightArgs &a) {
     const PagedSeq sq = paged_seq(a.seq, blockIdx.x);
@@ -1181,10 +1191,10 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
     if (key >= n) return;
     const int from = max(0, key / KT * KT - (n - q_len)) * a.G / a.part_rows;  // the first part that saw the tile
     const float *p = a.parts + a.parts0[sq.i] + (size_t)kvh * nparts * kpad + key;
-    float sum = 0.f;
+    double sum = 0.0;
     for (int i = from; i < nparts; ++i) sum += p[(size_t)i * kpad];
     const size_t at = ((size_t)sq.b * a.Hkv + kvh) * a.w_stride + key;
-    a.w_out[at] = a.w_in[at] + sum;
+    a.w_out[at] = (float)(a.w_in[at] + sum);
 }
 
 // (d = 256: one wave per SIMD, since two spill; 64 sequences of 2048 to 4096 rows of 16 over 4 heads 394 -> 307 us.)
