@@ -114,3 +114,16 @@ def test_the_reference_keeps_ties_by_row_and_nan_last():
     assert pagedref.evict(w, 9, 5, 1, 2).tolist() == [0, 2, 4, 7, 8]
     assert pagedref.evict(w, 9, 8, 1, 2).tolist() == [0, 1, 2, 4, 5, 6, 7, 8]
     assert pagedref.evict(w, 9, 9, 1, 2).tolist() == list(range(9))
+
+
+@pytest.mark.parametrize("q_start,n_rows", [([0, 1], [(1 << 32) + 16]), ([0, (1 << 32) + 1], [16]), ([0, 1], [1 << 31]),
+                                            ([0, 1], [-(1 << 31) - 1])])
+def test_the_binding_does_not_wrap_lengths(zt, q_start, n_rows):
+    with pytest.raises(ValueError, match="32 bits"):
+        zt.attn_paged_workspace_bytes(q_start, n_rows, 4, 2, 32)
+
+
+def test_the_binding_does_not_wrap_heads(zt):
+    for bad in (((1 << 32) + 4, 2, 32), (4, (1 << 32) + 2, 32), (4, 2, (1 << 32) + 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            zt.attn_paged_workspace_bytes([0, 1], [16], *bad)

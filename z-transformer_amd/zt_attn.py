@@ -310,10 +310,19 @@ def _here(*ts):
             raise ValueError("tensors must be on the current device")
 
 
+def _c_ints(*xs):
+    """The C ABI's ints; ctypes alone would cut off what does not fit."""
+    xs = [int(x) for x in xs]
+    for x in xs:
+        if not -(1 << 31) <= x < 1 << 31:
+            raise ValueError(f"{x} does not fit 32 bits")
+    return xs
+
+
 def _host_ints(xs, n):
     if len(xs) != n:
         raise ValueError(f"{len(xs)} lengths where {n} are needed")
-    return (ctypes.c_int * n)(*[int(x) for x in xs])
+    return (ctypes.c_int * n)(*_c_ints(*xs))
 
 
 def _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages, rows, w, B):
@@ -341,15 +350,15 @@ def paged_append(q, k_new, v_new, q_out, k_pages, v_pages, table, q_start, n_row
                             [(q, n_heads * dim), (q_out, n_heads * dim), (k_new, n_kv_heads * dim),
                              (v_new, n_kv_heads * dim)], w, B)
     _check(lib().zt_paged_append(*map(_ptr, (q, k_new, v_new, q_out, k_pages, v_pages, table, w)),
-                                 _host_ints(q_start, B + 1), _host_ints(n_rows, B), _host_ints(pos, B), B, n_pages,
-                                 page_size, table_stride, 0 if w is None else w.shape[-1], n_heads, n_kv_heads, dim,
-                                 theta, _stream(stream)), "zt_paged_append")
+                                 _host_ints(q_start, B + 1), _host_ints(n_rows, B), _host_ints(pos, B),
+                                 *_c_ints(B, n_pages, page_size, table_stride, 0 if w is None else w.shape[-1], n_heads,
+                                          n_kv_heads, dim), theta, _stream(stream)), "zt_paged_append")
 
 
 def attn_paged_workspace_bytes(q_start, n_rows, n_heads, n_kv_heads, dim, weights=False):
     B = len(n_rows)
-    return lib().zt_attn_paged_workspace(_host_ints(q_start, B + 1), _host_ints(n_rows, B), B, n_heads, n_kv_heads,
-                                         dim, int(weights))
+    return lib().zt_attn_paged_workspace(_host_ints(q_start, B + 1), _host_ints(n_rows, B), B,
+                                         *_c_ints(n_heads, n_kv_heads, dim), int(weights))
 
 
 def attn_paged(q, k_pages, v_pages, table, out, q_start, n_rows, page_size, n_heads, n_kv_heads, dim, workspace,
@@ -365,9 +374,10 @@ def attn_paged(q, k_pages, v_pages, table, out, q_start, n_rows, page_size, n_he
                             [(q, n_heads * dim), (out, n_heads * dim), (lse, n_heads)], w_out, B)
     nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _check(lib().zt_attn_paged(*map(_ptr, (q, k_pages, v_pages, table, out, lse, w_in, w_out)),
-                               _host_ints(q_start, B + 1), _host_ints(n_rows, B), B, n_pages, page_size, table_stride,
-                               0 if w_out is None else w_out.shape[-1], n_heads, n_kv_heads, dim, _ptr(workspace),
-                               nbytes, _stream(stream)), "zt_attn_paged")
+                               _host_ints(q_start, B + 1), _host_ints(n_rows, B),
+                               *_c_ints(B, n_pages, page_size, table_stride, 0 if w_out is None else w_out.shape[-1],
+                                        n_heads, n_kv_heads, dim), _ptr(workspace), nbytes, _stream(stream)),
+           "zt_attn_paged")
 
 
 def paged_evict(k_pages, v_pages, table, table_out, w_in, w_out, kept, n_rows, page_size, n_kv_heads, dim, n_first,
@@ -381,8 +391,9 @@ def paged_evict(k_pages, v_pages, table, table_out, w_in, w_out, kept, n_rows, p
         raise ValueError("table and table_out, and w_in and w_out, have one shape; kept is [B, n_kv_heads, budget]")
     n_pages = _paged_shapes((0,), n_kv_heads, dim, page_size, k_pages, v_pages, [], w_in, B)
     _check(lib().zt_paged_evict(*map(_ptr, (k_pages, v_pages, table, table_out, w_in, w_out, kept)),
-                                _host_ints(n_rows, B), B, n_pages, page_size, table_stride, w_in.shape[-1], n_kv_heads,
-                                dim, n_first, n_last, budget, _stream(stream)), "zt_paged_evict")
+                                _host_ints(n_rows, B),
+                                *_c_ints(B, n_pages, page_size, table_stride, w_in.shape[-1], n_kv_heads, dim, n_first,
+                                         n_last, budget), _stream(stream)), "zt_paged_evict")
 
 
 def rmsnorm(x, w, y, rows, cols, eps=1e-5, stream=None):
