@@ -735,3 +735,15 @@ def test_weights_of_very_many_rows(gpu, zt, tune, d):
     want = H * np.array([1 + (e[0] / total).sum(), (e[1] / total).sum()])
     bound = (2 * (d + 4) * 0.62 + 24 + 136) * EPS
     assert np.all(np.abs(got / want - 1) <= bound), (got / want - 1, bound)
+
+
+def test_the_binding_refuses_a_workspace_of_another_layout(gpu, zt):
+    """An expanded tensor has as many bytes as it says nowhere."""
+    H, Hkv, d, page, n = 4, 2, 32, 8, 3000
+    c = Cache(gpu, np.random.default_rng(33), [n], page, Hkv, d)
+    q, w = gpu.zeros(3, H * d, device="cuda"), gpu.zeros(1, Hkv, n, device="cuda")
+    need = zt.attn_paged_workspace_bytes([0, 3], [n], H, Hkv, d, True)
+    whole = gpu.empty(2 * need, device="cuda", dtype=gpu.uint8)
+    for ws in (whole[:1].expand(need), whole[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            zt.attn_paged(q, c.k, c.v, c.table, gpu.empty_like(q), [0, 3], [n], page, H, Hkv, d, ws, w_in=w, w_out=w)

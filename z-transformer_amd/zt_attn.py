@@ -369,6 +369,8 @@ def attn_paged(q, k_pages, v_pages, table, out, q_start, n_rows, page_size, n_he
     _here(q, k_pages, v_pages, table, out, workspace, lse, w_in, w_out)
     if w_in is not None and w_out is not None and w_in.shape != w_out.shape:
         raise ValueError("w_in and w_out have the same shape")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
     B, table_stride = table.shape
     n_pages = _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages,
                             [(q, n_heads * dim), (out, n_heads * dim), (lse, n_heads)], w_out, B)
