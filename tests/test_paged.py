@@ -127,3 +127,13 @@ def test_the_binding_does_not_wrap_heads(zt):
     for bad in (((1 << 32) + 4, 2, 32), (4, (1 << 32) + 2, 32), (4, 2, (1 << 32) + 32)):
         with pytest.raises(ValueError, match="32 bits"):
             zt.attn_paged_workspace_bytes([0, 1], [16], *bad)
+
+
+@pytest.mark.parametrize("page,Hkv,d", [(0, 2, 32), (8, 0, 32), (8, 2, 0), (-8, -2, 32)])
+def test_the_binding_refuses_empty_pages(zt, page, Hkv, d):
+    class Pool:
+        def numel(self):
+            return 512
+
+    with pytest.raises(ValueError, match="holds nothing"):
+        zt._paged_shapes((0,), Hkv, d, page, Pool(), Pool(), [], None, 1)

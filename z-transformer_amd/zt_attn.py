@@ -327,8 +327,11 @@ def _host_ints(xs, n):
 
 def _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages, rows, w, B):
     """What the C side cannot see: that the tensors are as long as the lengths say.  Returns n_pages."""
-    n_pages = k_pages.numel() // (page_size * n_kv_heads * dim)
-    if v_pages.numel() != k_pages.numel() or n_pages * page_size * n_kv_heads * dim != k_pages.numel():
+    of_page = page_size * n_kv_heads * dim
+    if page_size < 1 or n_kv_heads < 1 or dim < 1:
+        raise ValueError(f"a page of {page_size} rows of {n_kv_heads} kv heads, {dim} wide, holds nothing")
+    n_pages = k_pages.numel() // of_page
+    if v_pages.numel() != k_pages.numel() or n_pages * of_page != k_pages.numel():
         raise ValueError("k_pages and v_pages are [n_pages, page_size, n_kv_heads * dim]")
     for t, per_token in rows:
         if t is not None and t.numel() < int(q_start[-1]) * per_token:
