@@ -207,7 +207,7 @@ int zt_paged_append(const float *q, const float *k_new, const float *v_new, floa
  * w_out[b, j, s] = w_in[b, j, s] + the sum of row s's softmax weights over the new
  * tokens and the query heads of kv head j, for s < n_rows[b]; later w_out are left
  * as they are.  K and V rows that no token sees, and what they hold (inf, NaN), change
- * no result.  `workspace`: zt_attn_paged_workspace(...) bytes for the same lengths,
+ * no result.  The new tokens of all sequences times n_heads are at most 2^31.  `workspace`: zt_attn_paged_workspace(...) bytes for the same lengths,
  * 16-byte aligned (null where that is 0). */
 size_t zt_attn_paged_workspace(const int *q_start, const int *n_rows, int B, int n_heads, int n_kv_heads, int dim,
                                int weights);

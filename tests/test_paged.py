@@ -137,3 +137,15 @@ def test_the_binding_refuses_empty_pages(zt, page, Hkv, d):
 
     with pytest.raises(ValueError, match="holds nothing"):
         zt._paged_shapes((0,), Hkv, d, page, Pool(), Pool(), [], None, 1)
+
+
+@pytest.mark.parametrize("B", [2, 8, 16])
+def test_scores_past_64_bits_are_refused(zt, capfd, B):
+    """2^25 tokens of 32 heads over 2^30 rows are 2^60 scores a sequence: two are counted, eight have no number."""
+    q_start, n_rows = [b << 25 for b in range(B + 1)], [1 << 30] * B
+    need = zt.lib().zt_attn_paged_workspace(ints(*q_start), ints(*n_rows), B, 32, 8, 128, 1)
+    rc = attend(zt.lib(), q_start, n_rows, B, n_pages=8, page=1024, stride=1 << 20, H=32, Hkv=8, d=128, w_stride=1 << 30,
+                w_in=N, w_out=N, nbytes=64)
+    assert rc == 1
+    assert (need > 0) == (B == 2)
+    assert ("short of" if B == 2 else "tokens x heads") in capfd.readouterr().err

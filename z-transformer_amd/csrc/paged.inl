@@ -8,6 +8,12 @@
 // Rows of a sequence, tokens x heads of one, rows of a budget: no sum of two overflows an int.
 constexpr long long kPagedMost = 1LL << 30;
 
+// The tokens x heads that one call attends with: over as many rows as a sequence has, every row's scores are still
+// counted in 64 bits.
+static bool paged_batch_ok(const int *q_start, int B, int n_heads) {
+    return ((long long)q_start[B] - q_start[0]) * n_heads <= 2 * kPagedMost;
+}
+
 // The cache's geometry; 0 when usable.
 static int paged_check(const char *who, const int *n_rows, int B, int n_pages, int page_size, int table_stride) {
     if (B < 1 || n_pages < 1 || table_stride < 1) {
@@ -354,6 +360,7 @@ size_t zt_attn_paged_workspace(const int *q_start, const int *n_rows, int B, int
         const long long q_len = (long long)q_start[b + 1] - q_start[b];
         if (n_rows[b] < 0 || n_rows[b] > kPagedMost || q_len < 0 || q_len > n_rows[b] || q_len * n_heads > kPagedMost) return 0;
     }
+    if (!paged_batch_ok(q_start, B, n_heads)) return 0;
     return paged_space(paged_plan(q_start, n_rows, B, n_heads, n_kv_heads, dim), weights != 0).bytes;
 }
 
@@ -365,6 +372,10 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     if (!zt_attn_dim_ok(dim)) return refuse_dim(dim);
     if (check_group(n_heads, n_kv_heads)) return 1;
     if (paged_tokens_check("attn_paged", q_start, n_rows, B, n_heads)) return 1;
+    if (!paged_batch_ok(q_start, B, n_heads)) {
+        fprintf(stderr, "zt_attn: attn_paged takes at most %lld new tokens x heads in a call.\n", 2 * kPagedMost);
+        return 1;
+    }
     if (!w_in != !w_out) {
         fprintf(stderr, "zt_attn: attn_paged takes w_in and w_out together or neither.\n");
         return 1;
