@@ -64,3 +64,31 @@ def evict(w, n, budget, first, last):
     x = np.where(nan, np.float32(-np.inf), w[middle]).astype(np.float64)
     best = middle[np.lexsort((middle, nan, -x))[:budget - first - last]]
     return np.sort(np.concatenate((rows[:first], best, rows[n - last:])))
+
+
+def rows_kind(rows, d):
+    """The launch kind of so many rows per kv head (new tokens x heads of the group): their limit, 0 for the last kind."""
+    dp = 32 * -(-d // 32)
+    kinds = [16, 32, 64, 128] if dp <= 128 else [16, 64] if dp <= 192 else [16]
+    return next((k for k in kinds if rows <= k), 0)
+
+
+# (heads, kv heads, width) for batch_of_kinds; the same with the most rows per kv head for batch_of_few.
+KIND_SHAPES = [(8, 8, 32), (16, 8, 50), (8, 8, 64), (24, 8, 96), (32, 8, 128), (16, 8, 192), (16, 8, 256)]
+FEW_SHAPES = [(8, 8, 32, 16), (8, 8, 32, 32), (16, 8, 64, 16), (16, 8, 64, 32), (16, 8, 50, 32), (24, 8, 96, 16),
+              (32, 8, 128, 16), (32, 8, 128, 32), (16, 8, 192, 16), (32, 8, 256, 16)]
+
+
+def batch_of_kinds(H, Hkv):
+    """(rows, new tokens) of 74 sequences that need every kind at once, each with too many workgroups or steps to join
+    another's launch: 70 with one token, among them four with 24, 60, 120 and 400 rows per kv head."""
+    g = H // Hkv
+    ones = [(400 + (i * 37) % 500, 1) for i in range(70)]
+    longs = [(7300, 120 // g), (900, 400 // g), (7300, 24 // g), (7300, 60 // g)]
+    return list(zip(*(ones[:30] + longs[:2] + ones[30:] + longs[2:])))
+
+
+def batch_of_few(H, Hkv, rows):
+    """(rows, new tokens) of sequences with at most `rows` rows per kv head, 16 or 32, all of one launch kind."""
+    most = rows // (H // Hkv)
+    return [5000, 2700, 900, 65, 1300], [most, most - 1, most, most - 2, max(most - 3, rows // 2 // (H // Hkv) + 1)]

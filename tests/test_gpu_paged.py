@@ -747,3 +747,114 @@ def test_the_binding_refuses_a_workspace_of_another_layout(gpu, zt):
     for ws in (whole[:1].expand(need), whole[::2]):
         with pytest.raises(ValueError, match="workspace"):
             zt.attn_paged(q, c.k, c.v, c.table, gpu.empty_like(q), [0, 3], [n], page, H, Hkv, d, ws, w_in=w, w_out=w)
+
+
+def attend64(gpu, q, c, q_start, H):
+    """pagedref.attend by whole-matrix products on the device in 64 bits, for batches too large for its loops: the same
+    outputs and bounds, the weights' with the rounding of a sum over heads and tokens counted once."""
+    Hkv, d, g = c.Hkv, c.d, H // c.Hkv
+    N, B = len(q), len(c.n_rows)
+    f64 = dict(device="cuda", dtype=gpu.float64)
+    out, bound, lse = gpu.zeros(N, H, d, **f64), gpu.zeros(N, H, d, **f64), gpu.zeros(N, H, **f64)
+    w, w_bound = (gpu.zeros(B, Hkv, max(c.n_rows), **f64) for _ in range(2))
+    qd = gpu.from_numpy(q).cuda()
+    for b, n in enumerate(c.n_rows):
+        t0, t1 = q_start[b], q_start[b + 1]
+        at = gpu.from_numpy(pagedref.places(c.table_h, b, n, c.page)).cuda()
+        m = (gpu.arange(n - (t1 - t0), n, **f64) + 1)[:, None, None]  # keys that each token sees
+        seen = gpu.ones(t1 - t0, n, device="cuda", dtype=gpu.bool).tril(n - (t1 - t0))[:, None]
+        for j in range(Hkv):
+            k, v = c.k[at, j].double(), c.v[at, j].double()
+            x = qd[t0:t1, j * g:(j + 1) * g].double().reshape(-1, d)
+            s = gpu.mm(x, k.t().contiguous()).view(t1 - t0, g, n) / np.sqrt(d)
+            size = gpu.mm(x.abs(), k.abs().t().contiguous()).view(t1 - t0, g, n) / np.sqrt(d)
+            s = gpu.where(seen, s, -np.inf)
+            l = gpu.logsumexp(s, 2)
+            p = gpu.exp(s - l[:, :, None])
+            e = 2 * (d + 4) * EPS * gpu.where(seen, size, 0.0).amax(2, keepdim=True)
+            rel = gpu.expm1(e) + (m + m / 16 + 32) * EPS
+            out[t0:t1, j * g:(j + 1) * g] = gpu.mm(p.view(-1, n), v).view(t1 - t0, g, d)
+            bound[t0:t1, j * g:(j + 1) * g] = rel * gpu.mm(p.view(-1, n), v.abs()).view(t1 - t0, g, d)
+            lse[t0:t1, j * g:(j + 1) * g] = l
+            w[b, j, :n] = p.sum((0, 1))
+            w_bound[b, j, :n] = (rel * p).sum((0, 1)) + g * (t1 - t0) * EPS * w[b, j, :n]
+    return [x.cpu().numpy() for x in (out, lse, w, bound, w_bound)]
+
+
+def test_the_two_references_agree(gpu):
+    H, Hkv, d, page, n_rows, q_len = 6, 2, 50, 8, [40, 7, 129], [3, 7, 17]
+    rng = np.random.default_rng(41)
+    c = Cache(gpu, rng, n_rows, page, Hkv, d, garbage=np.nan)
+    q_start = np.cumsum([0] + q_len).tolist()
+    q = rng.standard_normal((q_start[-1], H, d)).astype(np.float32)
+    *want, w_bound = pagedref.attend(q, c.k_h, c.v_h, c.table_h, q_start, n_rows, page, H, Hkv, d)
+    *got, mine = attend64(gpu, q, c, q_start, H)
+    for x, y in zip(want, got):
+        assert np.allclose(x, y, rtol=1e-10, atol=1e-13)
+    assert np.all(mine <= w_bound * (1 + 1e-10)) and np.all(mine >= w_bound / (H // Hkv))
+
+
+@pytest.mark.parametrize("H,Hkv,d", pagedref.KIND_SHAPES)
+def test_a_batch_of_every_kind(gpu, zt, tune, H, Hkv, d):
+    """Launches of every kind beside one another in one workspace, over more sequences than one launch takes, with weights
+    from kept scores and from scores formed again (test_paged.py shows that the kinds stay apart)."""
+    n_rows, q_len = pagedref.batch_of_kinds(H, Hkv)
+    rng = np.random.default_rng([H, d, 42])
+    c = Cache(gpu, rng, n_rows, 16, Hkv, d, garbage=np.nan)
+    q_start = np.cumsum([1] + list(q_len)).tolist()
+    q = rng.standard_normal((q_start[-1] + 2, H, d)).astype(np.float32)
+    w = rng.random((len(n_rows), Hkv, max(n_rows) + 5), np.float32)
+    ref = attend64(gpu, q, c, q_start, H)
+    for scores in (0, 1):
+        tune({"ZT_PAGED_SCORES": scores})
+        grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
+    grade(run_attend(gpu, zt, c, q, q_start, H), ref, q_start, n_rows, Hkv)
+
+
+@pytest.mark.parametrize("target", [256, 32768])
+@pytest.mark.parametrize("H,Hkv,d,rows", pagedref.FEW_SHAPES)
+def test_few_rows_in_fewer_and_in_more_chunks(gpu, zt, tune, H, Hkv, d, rows, target):
+    """The streaming kernel's chunks and their merges, forced (test_paged.py shows that both targets reach the plan)."""
+    n_rows, q_len = pagedref.batch_of_few(H, Hkv, rows)
+    rng = np.random.default_rng([H, d, rows])
+    c = Cache(gpu, rng, n_rows, 16, Hkv, d, garbage=np.nan)
+    q_start = np.cumsum([2] + list(q_len)).tolist()
+    q = rng.standard_normal((q_start[-1] + 3, H, d)).astype(np.float32)
+    w = rng.random((len(n_rows), Hkv, max(n_rows) + 5), np.float32)
+    ref = attend64(gpu, q, c, q_start, H)
+    tune({"ZT_PAGED_WGS": target})
+    grade(run_attend(gpu, zt, c, q, q_start, H, w), ref, q_start, n_rows, Hkv, w)
+    grade(run_attend(gpu, zt, c, q, q_start, H), ref, q_start, n_rows, Hkv)
+
+
+@pytest.mark.parametrize("kind", ["random", "odd"])
+@pytest.mark.parametrize("pages_in_place", [True, False])
+@pytest.mark.parametrize("n_rows,budget,first,last,Hkv,d,page", [
+    ([40, 7, 33, 0, 32], 32, 4, 8, 2, 32, 1), ([2100, 1000], 700, 1, 64, 2, 34, 16), ([5000, 1500], 1300, 4, 64, 2, 96, 64),
+    ([20000, 90], 9000, 1, 1, 1, 32, 16)])
+def test_eviction_of_pages_and_weights_each_its_way(gpu, zt, n_rows, budget, first, last, Hkv, d, page, pages_in_place, kind):
+    """Pages in place and weights to another buffer, and the other way round."""
+    rng = np.random.default_rng([len(n_rows), budget, d, 1])
+    B, stride = len(n_rows), max(n_rows) + 3
+    c = Cache(gpu, rng, n_rows + [budget] * B, page, Hkv, d)
+    table = c.table[:B].contiguous()
+    table_out, out_h = (table, c.table_h[:B]) if pages_in_place else (c.table[B:].contiguous(), c.table_h[B:])
+    w = _weights(rng, B, Hkv, stride, kind)
+    w_in = gpu.from_numpy(w.copy()).cuda()
+    w_out = gpu.full_like(w_in, -7.0) if pages_in_place else w_in
+    kept = gpu.full((B, Hkv, budget), 12345, device="cuda", dtype=gpu.int32)
+    zt.paged_evict(c.k, c.v, table, table_out, w_in, w_out, kept, n_rows, page, Hkv, d, first, last, budget)
+    k, v, kept_want = c.k_h.copy(), c.v_h.copy(), np.full((B, Hkv, budget), -1)
+    w_want = np.full_like(w, -7.0) if pages_in_place else w.copy()
+    for b, n in enumerate(n_rows):
+        src, dst = pagedref.places(c.table_h, b, n, page), pagedref.places(out_h, b, min(n, budget), page)
+        for h in range(Hkv):
+            rows = pagedref.evict(w[b, h], n, budget, first, last)
+            kept_want[b, h, :len(rows)] = rows
+            k[dst, h], v[dst, h] = c.k_h[src[rows], h], c.v_h[src[rows], h]
+            w_want[b, h, :len(rows)] = w[b, h, rows]
+    assert np.array_equal(kept.cpu().numpy(), kept_want)
+    assert np.array_equal(c.k.cpu().numpy(), k) and np.array_equal(c.v.cpu().numpy(), v)
+    assert np.array_equal(w_out.cpu().numpy().view(np.uint32), w_want.view(np.uint32))
+    if pages_in_place:
+        assert np.array_equal(w_in.cpu().numpy().view(np.uint32), w.view(np.uint32))

@@ -149,3 +149,39 @@ def test_scores_past_64_bits_are_refused(zt, capfd, B):
     assert rc == 1
     assert (need > 0) == (B == 2)
     assert ("short of" if B == 2 else "tokens x heads") in capfd.readouterr().err
+
+
+def _apart(zt, n_rows, q_len, H, Hkv, d):
+    """Whether the batch's workspace is its launch kinds' own added up (a kind that joins another's is cut otherwise)."""
+    def need(pick):  # without weights and with
+        ls = [l for l, p in zip(q_len, pick) if p]
+        ns = [n for n, p in zip(n_rows, pick) if p]
+        return np.array([zt.attn_paged_workspace_bytes(np.cumsum([0] + ls), ns, H, Hkv, d, w) for w in (False, True)])
+
+    of = [pagedref.rows_kind(l * (H // Hkv), d) for l in q_len]
+    own = [need([x == kind for x in of]) for kind in sorted(set(of))]
+    assert np.all(np.array(own) > 0)  # each is cut into key chunks
+    return bool(np.all(need([True] * len(of)) == sum(own))), len(own)
+
+
+@pytest.mark.parametrize("H,Hkv,d", pagedref.KIND_SHAPES)
+def test_a_batch_of_every_kind(zt, H, Hkv, d):
+    """pagedref.batch_of_kinds has launches of every kind beside one another (its figures: test_gpu_paged.py)."""
+    n_rows, q_len = pagedref.batch_of_kinds(H, Hkv)
+    assert _apart(zt, n_rows, q_len, H, Hkv, d) == (True, 5 if d <= 128 else 3 if d <= 192 else 2)
+
+
+def test_a_short_batch_is_not_one(zt):
+    """What the sum above would look like were the kinds joined."""
+    assert not _apart(zt, [700, 900], [1, 90], 8, 2, 128)[0]
+
+
+@pytest.mark.parametrize("H,Hkv,d,rows", pagedref.FEW_SHAPES)
+def test_the_workgroup_target_reaches_the_plan(zt, tune, H, Hkv, d, rows):
+    """pagedref.batch_of_few is cut into other chunks for one target than for the other."""
+    n_rows, q_len = pagedref.batch_of_few(H, Hkv, rows)
+    need = []
+    for target in (256, 32768):
+        tune({"ZT_PAGED_WGS": target})
+        need.append(zt.attn_paged_workspace_bytes(np.cumsum([0] + q_len), n_rows, H, Hkv, d))
+    assert 0 < need[0] < need[1]
