@@ -207,8 +207,9 @@ int zt_paged_append(const float *q, const float *k_new, const float *v_new, floa
  * w_out[b, j, s] = w_in[b, j, s] + the sum of row s's softmax weights over the new
  * tokens and the query heads of kv head j, for s < n_rows[b]; later w_out are left
  * as they are.  K and V rows that no token sees, and what they hold (inf, NaN), change
- * no result.  The new tokens of all sequences times n_heads are at most 2^31.  `workspace`: zt_attn_paged_workspace(...) bytes for the same lengths,
- * 16-byte aligned (null where that is 0). */
+ * no result.  The new tokens of all sequences times n_heads are at most 2^31.
+ * `workspace`: zt_attn_paged_workspace(...) bytes for the same lengths, 16-byte aligned
+ * (null where that is 0). */
 size_t zt_attn_paged_workspace(const int *q_start, const int *n_rows, int B, int n_heads, int n_kv_heads, int dim,
                                int weights);
 int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, float *out, float *lse,
@@ -226,7 +227,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
  * table_out is table, the same pointer (in place: the sequences' pages must not be
  * shared), or another table of the same stride, none of whose pages is in table (a
  * copy: table's pages, which may be shared, stay as they are); w_out is w_in or a buffer that
- * does not overlap it. */
+ * does not overlap it, whichever table_out is.  Where a kept row's old or new page is none of
+ * the pool's, its K and V are not moved: the new place, if there is one, keeps what it held. */
 int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *table_out, const float *w_in,
                    float *w_out, int *kept, const int *n_rows, int B, int n_pages, int page_size, int table_stride,
                    int w_stride, int n_kv_heads, int dim, int n_first, int n_last, int budget, hipStream_t stream);

@@ -10,7 +10,9 @@
 // A page number outside the pool is never followed: a row that sees such a key comes
 // out NaN.  A key that a row must not see gets the score -inf, and where a tile
 // holds such a pair, V's values that are not finite are kept out of the products (0 x inf)
-// and added to the rows that see them: nothing hidden reaches an output.
+// and added to the rows that see them: nothing hidden reaches an output.  (A hidden K value of 2^40
+// or more beside such a q moves a tile's products to f32 in the split-operand kernel, so that visible
+// ones may be rounded otherwise.)
 #include "common.h"
 #include "args.h"
 #include "paged.h"
@@ -1197,7 +1199,7 @@ DEVI void paged_wsum(const PagedWeightArgs &a) {
     a.w_out[at] = (float)(a.w_in[at] + sum);
 }
 
-// (d = 256: one wave per SIMD, since two spill; 64 sequences of 2048 to 4096 rows of 16 over 4 heads 394 -> 307 us.)
+// (d = 256: one wave per SIMD, since two spill; 64 sequences of 2048 to 4096 rows of 16 over 4 heads 394 -> 290 us.)
 #define ZT_PAGED_FEW(DP, NQ)                                                                        \
     extern "C" __global__ void __launch_bounds__(256, (DP) == 256 ? 1 : 2) zt_paged_few_d##DP##_n##NQ(PagedArgs a) {   \
         paged_few<DP, NQ, true>(a);                                                                 \

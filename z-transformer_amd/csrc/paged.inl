@@ -155,8 +155,10 @@ struct PagedPlan {
     long long sums(int b) const { return many(b) && parts(b) > 1 ? (long long)Hkv * parts(b) * kpad(b) : 0; }
 };
 
-// Workgroups of a kind on the device at once: as many of the streaming kernel as its registers let stand on the CUs;
-// of the split-operand kernel two of four waves per CU where LDS holds both, else one.
+// Workgroups of a kind on the device at once, as the plan counts them: of the streaming kernel what the registers of
+// one 16-row block allow from d = 64 up (fewer than the 1792 of d = 32; with two blocks 768 stand at d = 64 and 512 at d = 96
+// and 128, a quarter to a third less than counted); of the split-operand kernel two of four waves per CU where LDS
+// holds both, else one.
 int paged_slots(const PagedPlan &p, PagedKind k) {
     if (paged_few(k)) return p.dp <= 64 ? 1024 : p.dp <= 128 ? 768 : p.dp <= 192 ? 512 : 256;
     return paged_shape(k, p.dp).nw == 4 && p.dp <= 192 ? 512 : 256;
@@ -204,6 +206,10 @@ double paged_span(const PagedPlan &p, PagedKind k, int limit, int slots, double 
 // partial sums' way to memory and back: 0.011 steps each, a step being RT x 32 keys at 216 TFLOP/s against 4.7 TB/s).
 // Measured on MI355X (us, chunks of an even share of all steps / these): 333 tokens on 2340 rows of 32 over 8
 // heads at d = 128 139 / 89, a batch with three chunks of 501 on 1850 to 2980 rows at d = 96 513 / 301.
+// A workgroup's own start and end count three steps, and a chunk has four at least.  Counted as one or six, eleven of
+// twelve shapes take the same time (four sequences of 24 tokens on 2000 rows 46 instead of 53 with either).  With eight
+// steps at least 64 tokens on 4096 rows take 58 instead of 46; with two the small grids are 5 to 10 % faster (200 tokens on
+// 3000 rows of 8 heads over one 39 / 43) and none of the twelve is slower.
 int paged_limit(const PagedPlan &p, PagedKind k, int longest) {
     const int slots = paged_slots(p, k);
     const double extra = 3, way = 0.011;
