@@ -185,3 +185,11 @@ def test_the_workgroup_target_reaches_the_plan(zt, tune, H, Hkv, d, rows):
         tune({"ZT_PAGED_WGS": target})
         need.append(zt.attn_paged_workspace_bytes(np.cumsum([0] + q_len), n_rows, H, Hkv, d))
     assert 0 < need[0] < need[1]
+
+
+def test_an_eviction_past_a_launch_is_refused(zt, capfd):
+    """2^24 + 1 rows to other pages, a workgroup each."""
+    n = (1 << 24) + 1
+    assert evict(zt.lib(), n_rows=(5, n), stride=1 << 15, page=1024, w_stride=n, Hkv=9, d=256, budget=n,
+                 table_out=ctypes.c_void_p(32)) == 1
+    assert "workgroups" in capfd.readouterr().err

@@ -605,13 +605,6 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
         return 1;
     }
     if (!rows_aligned(dim, {k_pages, v_pages})) return 1;
-    DeviceState *st = require_device();
-    if (!st) return 1;
-    PagedEvictArgs a{};
-    a.pool = page_pool(k_pages, v_pages, table, n_pages, page_size, table_stride);
-    a.table_out = table_out; a.w_in = w_in; a.w_out = w_out; a.kept = kept;
-    a.Hkv = n_kv_heads; a.dim = dim; a.w_stride = w_stride;
-    a.n_first = n_first; a.n_last = n_last; a.budget = budget;
     const int n = dim % 4 == 0 ? 4 : 2, per_head = dim / n;
     const bool in_place = table_out == table;
     const char *const move = in_place ? n == 4 ? "zt_evict_move_4" : "zt_evict_move_2"
@@ -623,9 +616,15 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
         return in_place ? 2LL * n_kv_heads : ((long long)std::min(budget, most) + rows_per_wg - 1) / rows_per_wg;
     };
     const long long move_most = 0xFFFFFFFFll / move_threads;  // workgroups of a launch
-    // All is refused before anything is launched.
     for (int b = 0; b < B; ++b)
         if (n_rows[b] && move_wgs(n_rows[b]) > move_most) return !grid_ok(move_wgs(n_rows[b]), move_threads);
+    DeviceState *st = require_device();
+    if (!st) return 1;
+    PagedEvictArgs a{};
+    a.pool = page_pool(k_pages, v_pages, table, n_pages, page_size, table_stride);
+    a.table_out = table_out; a.w_in = w_in; a.w_out = w_out; a.kept = kept;
+    a.Hkv = n_kv_heads; a.dim = dim; a.w_stride = w_stride;
+    a.n_first = n_first; a.n_last = n_last; a.budget = budget;
     for (int b0 = 0; b0 < B; b0 += ZT_PAGED_MAXB) {
         a.b0 = b0;
         a.ns = std::min(B - b0, ZT_PAGED_MAXB);

@@ -313,9 +313,8 @@ def _here(*ts):
 def _c_ints(*xs):
     """The C ABI's ints; ctypes alone would cut off what does not fit."""
     xs = [int(x) for x in xs]
-    for x in xs:
-        if not -(1 << 31) <= x < 1 << 31:
-            raise ValueError(f"{x} does not fit 32 bits")
+    if xs and (min(xs) < -(1 << 31) or max(xs) >= 1 << 31):
+        raise ValueError(f"{max(xs, key=abs)} does not fit 32 bits")
     return xs
 
 
