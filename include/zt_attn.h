@@ -233,6 +233,110 @@ int zt_paged_evict(float *k_pages, float *v_pages, const int *table, const int *
                    float *w_out, int *kept, const int *n_rows, int B, int n_pages, int page_size, int table_stride,
                    int w_stride, int n_kv_heads, int dim, int n_first, int n_last, int budget, hipStream_t stream);
 
+/* ---- Trees of drafted tokens over the paged cache (no reference counterpart) ----
+ * A sequence's new tokens may be a tree instead of a line: several continuations, drafted by
+ * a smaller model, say, are attended at once, and one line of them stays.  They are the last
+ * rows of the cache as before, in any order in which a parent comes before its children.
+ *
+ * zt_tree_mask: parent [.., DEVICE ints, packed as q's rows] the number, among its sequence's new
+ * tokens, of each token's parent, an earlier one; -1 (as any number that is not an
+ * earlier token's) where it follows the cache's row before them.  mask [.., words] (DEVICE, 8-byte
+ * aligned): bit j % 64 of a token's word j / 64 is set where new token j is the token itself or an
+ * ancestor.  64 * words is at least the new tokens of every sequence.  pos (HOST, B ints: a root's
+ * position) and pos_out (DEVICE, a token's: pos + the number of its ancestors) may both be
+ * null.  A step's masks and positions serve all its layers. */
+int zt_tree_mask(const int *parent, uint64_t *mask, int *pos_out, const int *q_start, const int *pos, int B, int words,
+                 hipStream_t stream);
+
+/* zt_attn_paged where a new token sees the rows before the new ones, as there, and of those
+ * only the tokens of its mask, none behind itself (bits of later tokens are ignored): zt_tree_mask's, or any
+ * other.  A token that sees nothing (no row before the new ones, and an empty mask) has out 0 and lse
+ * -inf.  `workspace`: zt_attn_paged_workspace(..., 0) bytes for the same lengths.  All else as zt_attn_paged. */
+int zt_attn_paged_tree(const float *q, const float *k_pages, const float *v_pages, const int *table, const uint64_t *mask,
+                       float *out, float *lse, const int *q_start, const int *n_rows, int B, int n_pages, int page_size,
+                       int table_stride, int words, int n_heads, int n_kv_heads, int dim, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* The rows that stay of the new ones: of each sequence's new tokens the one with number path[i] becomes new
+ * row i, for i < count[b] (DEVICE ints; path packed as q's rows, path[i] >= i, as in any tree; others, and
+ * numbers of no new token, move nothing).  The sequence's new n_rows is n_rows less its new tokens plus
+ * count[b]; rows behind hold what they held, or parts of it.  n_rows and q_start (HOST) are those of the append.  The pages of the
+ * new rows must not be shared.  Where a row's old or new page is none of the pool's, it is not moved. */
+int zt_paged_keep(float *k_pages, float *v_pages, const int *table, const int *path, const int *count, const int *q_start,
+                  const int *n_rows, int B, int n_pages, int page_size, int table_stride, int n_kv_heads, int dim,
+                  hipStream_t stream);
+
+/* ---- Shared pages (no reference counterpart) ------------------------------------------
+ * refs [n_pages] (DEVICE ints): how many page-table entries name a page; 0: it is free.  Tables hold -1
+ * where a sequence has no page.  The layers of a model share table and refs, each with K and V pages of its own:
+ * tables and counts change once, and zt_paged_copy moves what each layer holds.  Calls that change the same
+ * table or counts are made in order (one stream).
+ *
+ * zt_paged_fork: for i < n (HOST arrays), sequence dst[i] goes on from the first n_rows[i] rows of sequence src[i], with
+ * pages for n_room[i] rows (>= n_rows[i], within the table).  Where src[i] != dst[i] (a fork), dst's entries, which are
+ * overwritten, should be -1 (zt_paged_free); whole pages of the rows are shared, a partly filled one gets a copy, and the
+ * rest are free pages.  Where src[i] == dst[i] (growth), pages that are there stay, but a page from the
+ * partly filled one on that another entry names as well is replaced, as every page that the sequence may write must be
+ * its own.  pairs [n, 2] (DEVICE) receives the old and the new number of the page to copy, -1, -1 where there is
+ * none.  Pages are taken from the lowest free number up, in the order of entries and columns.  If fewer are free than
+ * needed, *missing (DEVICE) receives how many, pairs -1, and nothing else changes; else 0.  dst are all different, and none is another
+ * entry's src.  n <= B.  `workspace`: zt_paged_fork_workspace(...) bytes, 16-byte aligned. */
+size_t zt_paged_fork_workspace(const int *n_rows, const int *n_room, int n, int n_pages, int page_size);
+int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *src, const int *dst, const int *n_rows,
+                  const int *n_room, int n, int B, int n_pages, int page_size, int table_stride, void *workspace,
+                  size_t workspace_bytes, hipStream_t stream);
+/* Sequence b keeps the pages of its first n_keep[b] rows (HOST, B ints; 0: none, a whole table's rows or more:
+ * all): its later entries become -1, and their pages lose a reference. */
+int zt_paged_free(int *table, int *refs, const int *n_keep, int B, int n_pages, int page_size, int table_stride,
+                  hipStream_t stream);
+/* Pages in use move to the pool's beginning: of the L in use, the k-th highest that is not below L takes
+ * the k-th lowest free number, for k < max_pairs.  pairs [max_pairs, 2] (DEVICE) receives old and new number, -1, -1
+ * behind the last; moved [2] how many they are, and how many are left for another call.  table_out and refs_out are
+ * table and refs with the new numbers, the same pointers or buffers that do not overlap.  Every reference to a page
+ * must be in table.  `workspace`: zt_paged_compact_workspace(n_pages) bytes, 16-byte aligned. */
+size_t zt_paged_compact_workspace(int n_pages);
+int zt_paged_compact(const int *table, const int *refs, int *table_out, int *refs_out, int *pairs, int *moved,
+                     int max_pairs, int B, int n_pages, int table_stride, void *workspace, size_t workspace_bytes,
+                     hipStream_t stream);
+/* A layer's K and V pages pairs[2 i] to pairs[2 i + 1], i < n_pairs; pairs with a number outside the pool are passed
+ * over.  No page is written that another pair names. */
+int zt_paged_copy(float *k_pages, float *v_pages, const int *pairs, int n_pairs, int n_pages, int page_size,
+                  int n_kv_heads, int dim, hipStream_t stream);
+
+/* ---- Rotary positions in general (no reference counterpart) -----------------------------
+ * Rows at positions of their own, neighbouring columns or halves as pairs, a part of the head, and angles scaled for
+ * contexts longer than the trained one.
+ *
+ * zt_rope_frequencies (host only): freq [rot_dim / 2], the angle per position of each pair:
+ *   ZT_ROPE_PLAIN   f_i = theta^(-2 i / rot_dim), as zt_rope_forward's;
+ *   ZT_ROPE_LINEAR  f_i / factor;
+ *   ZT_ROPE_BASE    theta times factor^(rot_dim / (rot_dim - 2)) for theta: the lowest frequency is divided
+ *                   by factor, the highest stays;
+ *   ZT_ROPE_TURNS   by the turns r = context f_i / 2 pi that a pair makes within the trained context: f_i where r >= high,
+ *                   f_i / factor where r <= low, and between them (1 - s) f_i / factor + s f_i, s = (r - low) / (high - low).
+ * Arguments that a scaling does not name are not read. */
+enum { ZT_ROPE_PLAIN = 0, ZT_ROPE_LINEAR = 1, ZT_ROPE_BASE = 2, ZT_ROPE_TURNS = 3 };
+int zt_rope_frequencies(double *freq, int rot_dim, double theta, int scaling, double factor, double low, double high,
+                        double context);
+/* q/q_out [rows, n_heads*head_dim], k/k_out [rows, n_kv_heads*head_dim] (either may be absent: 0 heads), pos [rows] (DEVICE
+ * ints, any value), freq [rot_dim / 2] (HOST, read during the call).  Pair i of a head's first rot_dim columns, (i, i +
+ * rot_dim / 2), or with interleaved 1 (2 i, 2 i + 1), becomes amplitude (lo c - hi s, hi c + lo s), c and s of the angle
+ * pos freq[i]; the other columns are copied.  Angle and products in 64 bits, rounded once.  In place is allowed.  Rows
+ * are aligned as head_dim needs (16 bytes where it is a multiple of 4, else 8); head_dim <= 256. */
+int zt_rope_at_forward(const float *q, const float *k, float *q_out, float *k_out, const int *pos, const double *freq,
+                       int rows, int n_heads, int n_kv_heads, int head_dim, int rot_dim, int interleaved, double amplitude,
+                       hipStream_t stream);
+/* The transpose, for gradients: amplitude (lo c + hi s, hi c - lo s). */
+int zt_rope_at_backward(const float *dq, const float *dk, float *dq_out, float *dk_out, const int *pos, const double *freq,
+                        int rows, int n_heads, int n_kv_heads, int head_dim, int rot_dim, int interleaved,
+                        double amplitude, hipStream_t stream);
+/* zt_paged_append with these: pos [.., DEVICE ints, packed as q's rows] the position of each new token (zt_tree_mask's
+ * pos_out: tokens of a tree share positions). */
+int zt_paged_append_at(const float *q, const float *k_new, const float *v_new, float *q_out, float *k_pages,
+                       float *v_pages, const int *table, float *w, const int *pos, const double *freq, const int *q_start,
+                       const int *n_rows, int B, int n_pages, int page_size, int table_stride, int w_stride, int n_heads,
+                       int n_kv_heads, int dim, int rot_dim, int interleaved, double amplitude, hipStream_t stream);
+
 /* RMSNorm, src/norm.zig:18-47 on the device (the reference's src/cuda/norm.cu
  * kernel has no C entry point).  x/y [rows, cols], w [cols]; eps is
  * src/norm.zig:14's 1e-5 for the reference's behaviour.  rows == 0 launches

@@ -123,6 +123,8 @@ struct PagedArgs {
     float scale_log2e;
     PagedSeqs seq;      // at0: the first partial, slot (kvh * rows + row) * nch + chunk behind it
     long long score0[ZT_PAGED_MAXB];
+    const unsigned *mask;  // [N, mask_ld] which new tokens a token sees (trees only)
+    int mask_ld;
 };
 
 // Accumulated weights: w_out = w_in + sum over the rows of exp2(score - m) / sum, from stored scores at once
@@ -139,6 +141,15 @@ struct PagedWeightArgs {
     float scale_log2e;
     PagedSeqs seq;      // at0: the sequence's scores
     long long parts0[ZT_PAGED_MAXB];
+};
+
+// Masks and positions of trees of new tokens, from their parents.
+struct TreeMaskArgs {
+    const int *parent;         // [N]
+    unsigned long long *mask;  // [N, words]
+    int *pos;                  // [N], or null
+    int words;
+    PagedSeqs seq;             // n_rows: a root's position
 };
 
 // Append of new tokens to a paged cache, with RoPE on q and k.
@@ -167,6 +178,53 @@ struct PagedEvictArgs {
     int n_rows[ZT_PAGED_MAXB];
 };
 
+// Pages: refs[p] counts the table entries that name page p.
+#define ZT_PAGES_SEGMENT 4096  // pages that a workgroup counts
+
+// Sequences that go on from others, or grow: a launch's entries entry0 .. entry0 + n - 1 of `entries`.
+struct ForkArgs {
+    int *table;             // [B, table_stride]
+    int *refs;
+    int *pairs;             // [n, 2] of this launch's entries
+    int *missing;
+    int *seg_free;          // [segments] free pages
+    int *entry_fresh;       // [entries] pages wanted
+    int *rank;              // [slots] which of its entry's fresh pages a column takes, or -1
+    int *list;              // the free pages in order, `slots` at most
+    int n_pages, shift, table_stride, segments, entries, entry0, n, slots;
+    int src[ZT_PAGED_MAXB], dst[ZT_PAGED_MAXB], n_rows[ZT_PAGED_MAXB], n_room[ZT_PAGED_MAXB], slot0[ZT_PAGED_MAXB];
+};
+
+struct FreeArgs {
+    int *table, *refs;
+    int n_pages, table_stride, blocks;  // workgroups of a sequence
+    int b[ZT_PAGED_MAXB], from[ZT_PAGED_MAXB];
+};
+
+struct CompactArgs {
+    const int *table, *refs;
+    int *table_out, *refs_out;
+    int *pairs, *moved;
+    int *seg_used, *becomes;  // [segments], [n_pages]
+    long long entries;        // of the table
+    int n_pages, segments, max_pairs;
+};
+
+struct CopyArgs {
+    float *k, *v;
+    const int *pairs;
+    long long page_floats;
+    int n_pairs, n_pages, pieces;
+};
+
+// The rows of a tree's tokens that stay.
+struct KeepArgs {
+    PagePool pool;
+    const int *path, *count;  // [N], [B]
+    int Hkv, dim, blocks;     // workgroups of a sequence
+    int b[ZT_PAGED_MAXB], q0[ZT_PAGED_MAXB], q_len[ZT_PAGED_MAXB], row0[ZT_PAGED_MAXB];
+};
+
 struct NormArgs {
     const float *x, *w;
     float *y;
@@ -182,6 +240,27 @@ struct RopeArgs {
     float *y1, *y2;
     int rows, seq_len, heads1, heads2, pos, head_dim;
     double theta;
+};
+
+// Rotary positions of rows row0 .. row0 + rows - 1 of q (H heads) and k (Hkv heads): q_out, k_out.
+struct TurnArgs {
+    const float *q, *k;
+    float *q_out, *k_out;
+    const int *pos;            // [rows of the batch]
+    int rows, row0, H, Hkv, dim, rot;
+    int slices;                // parts that a row group's heads are cut into
+    double amplitude, sine;    // of the cosines, and of the sines, negative for the way back
+    double freq[ZT_MAX_DIM / 2];
+};
+
+// The same for new tokens, k into a paged cache with v.
+struct TurnPagedArgs {
+    TurnArgs turn;  // q null: none; k: the new keys
+    PagePool pool;
+    const float *v_new;
+    float *w;                                                  // [B, Hkv, w_stride] accumulated weights, or null
+    int w_stride, ns;
+    int b[ZT_PAGED_MAXB], q0[ZT_PAGED_MAXB], first[ZT_PAGED_MAXB];  // a sequence, its first token and that one's row
 };
 
 struct FillArgs {

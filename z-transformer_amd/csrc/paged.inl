@@ -15,7 +15,7 @@ static bool paged_batch_ok(const int *q_start, int B, int n_heads) {
 }
 
 // The cache's geometry; 0 when usable.
-static int paged_check(const char *who, const int *n_rows, int B, int n_pages, int page_size, int table_stride) {
+static int paged_geometry(const char *who, int B, int n_pages, int page_size, int table_stride) {
     if (B < 1 || n_pages < 1 || table_stride < 1) {
         fprintf(stderr, "zt_attn: %s over %d sequences of at most %d pages in a pool of %d is not launchable.\n", who, B,
                 table_stride, n_pages);
@@ -30,6 +30,12 @@ static int paged_check(const char *who, const int *n_rows, int B, int n_pages, i
         fprintf(stderr, "zt_attn: %d pages of %d rows are more than 2^31 - 1 rows.\n", n_pages, page_size);
         return 1;
     }
+    return 0;
+}
+
+// And its sequences' rows.
+static int paged_check(const char *who, const int *n_rows, int B, int n_pages, int page_size, int table_stride) {
+    if (paged_geometry(who, B, n_pages, page_size, table_stride)) return 1;
     if (!n_rows) {
         fprintf(stderr, "zt_attn: %s needs the host n_rows array.\n", who);
         return 1;
@@ -370,34 +376,54 @@ size_t zt_attn_paged_workspace(const int *q_start, const int *n_rows, int B, int
     return paged_space(paged_plan(q_start, n_rows, B, n_heads, n_kv_heads, dim), weights != 0).bytes;
 }
 
-int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, float *out, float *lse,
-                  const float *w_in, float *w_out, const int *q_start, const int *n_rows, int B, int n_pages,
-                  int page_size, int table_stride, int w_stride, int n_heads, int n_kv_heads, int dim, void *workspace,
-                  size_t workspace_bytes, hipStream_t stream) {
-    if (paged_check("attn_paged", n_rows, B, n_pages, page_size, table_stride)) return 1;
+// New tokens' masks: 64-bit words, one bit per new token of a sequence.
+static int tree_words_check(const char *who, const int *q_start, int B, int words) {
+    for (int b = 0; b < B; ++b) {
+        const int q_len = q_start[b + 1] - q_start[b];
+        if (words < 1 || words > (1 << 24) || (long long)words * 64 < q_len) {
+            fprintf(stderr, "zt_attn: %s: masks of %d 64-bit words do not hold sequence %d's %d new tokens.\n", who, words,
+                    b, q_len);
+            return 1;
+        }
+    }
+    return 0;
+}
+
+// Attention of a batch's new tokens, with the weights of the rows or without, of a chunk or (mask) of trees.
+static int paged_attend(const char *who, const float *q, const float *k_pages, const float *v_pages, const int *table,
+                        float *out, float *lse, const float *w_in, float *w_out, const uint64_t *mask, int words,
+                        const int *q_start, const int *n_rows, int B, int n_pages, int page_size, int table_stride,
+                        int w_stride, int n_heads, int n_kv_heads, int dim, void *workspace, size_t workspace_bytes,
+                        bool tree, hipStream_t stream) {
+    if (paged_check(who, n_rows, B, n_pages, page_size, table_stride)) return 1;
     if (!zt_attn_dim_ok(dim)) return refuse_dim(dim);
     if (check_group(n_heads, n_kv_heads)) return 1;
-    if (paged_tokens_check("attn_paged", q_start, n_rows, B, n_heads)) return 1;
+    if (paged_tokens_check(who, q_start, n_rows, B, n_heads)) return 1;
     if (!paged_batch_ok(q_start, B, n_heads)) {
-        fprintf(stderr, "zt_attn: attn_paged takes at most %lld new tokens x heads in a call.\n", 2 * kPagedMost);
+        fprintf(stderr, "zt_attn: %s takes at most %lld new tokens x heads in a call.\n", who, 2 * kPagedMost);
         return 1;
     }
     if (!w_in != !w_out) {
-        fprintf(stderr, "zt_attn: attn_paged takes w_in and w_out together or neither.\n");
+        fprintf(stderr, "zt_attn: %s takes w_in and w_out together or neither.\n", who);
         return 1;
     }
+    if (tree && tree_words_check(who, q_start, B, words)) return 1;
     const bool weights = w_out != nullptr;
-    if (weights && paged_weights_check("attn_paged", n_rows, B, w_stride)) return 1;
+    if (weights && paged_weights_check(who, n_rows, B, w_stride)) return 1;
     const PagedPlan p = paged_plan(q_start, n_rows, B, n_heads, n_kv_heads, dim);
     const PagedSpace space = paged_space(p, weights);
     if (space.bytes && (!workspace || workspace_bytes < space.bytes)) {
-        fprintf(stderr, "zt_attn: attn_paged workspace of %zu bytes is short of the %zu needed.\n", workspace_bytes,
+        fprintf(stderr, "zt_attn: %s workspace of %zu bytes is short of the %zu needed.\n", who, workspace_bytes,
                 space.bytes);
         return 1;
     }
-    if (space.bytes && !workspace_aligned(workspace, "attn_paged")) return 1;
-    if (!k_pages || !v_pages || !table || (q_start[B] > q_start[0] && (!q || !out))) {
+    if (space.bytes && !workspace_aligned(workspace, who)) return 1;
+    if (!k_pages || !v_pages || !table || (q_start[B] > q_start[0] && (!q || !out || (tree && !mask)))) {
         fprintf(stderr, "zt_attn: a null tensor pointer is not launchable.\n");
+        return 1;
+    }
+    if (tree && ((uintptr_t)mask & 7)) {
+        fprintf(stderr, "zt_attn: masks at %p are not 8-byte aligned.\n", (const void *)mask);
         return 1;
     }
     if (!rows_aligned(dim, {q, k_pages, v_pages, out})) return 1;
@@ -416,9 +442,10 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     a.H = n_heads; a.Hkv = n_kv_heads; a.G = p.G; a.dim = dim;
     a.part_ld = p.part_ld;
     a.w_in = w_in; a.w_out = w_out; a.w_stride = w_stride;
+    a.mask = reinterpret_cast<const unsigned *>(mask); a.mask_ld = 2 * words;
     a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)dim));
     // Whole 16-byte chunks throughout a row.
-    const char *const any = dim == dp ? "" : "_any";
+    const char *const any = dim == dp ? "" : "_any", *const set = tree ? "tree" : "paged";
 
     // Launches `name` for the sequences that `items` has work items for, up to ZT_PAGED_MAXB at a time; per_wg items
     // to a workgroup.  `each(i, b)` fills in what else argument block x needs for its entry i, sequence b; each(-1, b)
@@ -469,8 +496,8 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
             a.score0[i] = score0;
         };
         const auto mine = [&](int b) { return p.any(b) && p.kind(b) == kind; };
-        if (few) snprintf(name, sizeof name, "zt_paged_few_d%d_n%d%s", dp, kind == kFew1 ? 1 : 2, any);
-        else snprintf(name, sizeof name, "zt_paged_many_d%d_%d%d%s", dp, shape.nw, shape.nq, any);
+        if (few) snprintf(name, sizeof name, "zt_%s_few_d%d_n%d%s", set, dp, kind == kFew1 ? 1 : 2, any);
+        else snprintf(name, sizeof name, "zt_%s_many_d%d_%d%d%s", set, dp, shape.nw, shape.nq, any);
         const auto items = [&](int b) { return mine(b) ? p.items(b) : 0LL; };
         if (launch_for(name, few ? 256u : 64u * shape.nw, 1, a, items, fill)) return 1;
         // Same stream: the merge reads the chunks' partials.
@@ -484,7 +511,7 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
         // (Few rows' weights come with it, where they are wanted: 1024 keys to a workgroup.)
         const bool with = weights && few;
         snprintf(name, sizeof name,
-                 by_rows ? "zt_paged_merge_rows_d%d" : with ? "zt_paged_merge_w_d%d" : "zt_paged_merge_d%d", dp);
+                 by_rows ? "zt_%s_merge_rows_d%d" : with ? "zt_%s_merge_w_d%d" : "zt_%s_merge_d%d", set, dp);
         const auto merged = [&](int b) {
             const long long sums = with ? (long long)((n_rows[b] + 1023) / 1024) * n_kv_heads : 0;
             return mine(b) && p.chunks(b) > 1 ? (long long)p.q_len(b) * n_heads + sums : 0LL;
@@ -524,6 +551,77 @@ int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, co
     if (run(name, p.keep ? 256u : 64u * p.weight_waves(), true, parts)) return 1;
     snprintf(name, sizeof name, "zt_paged_wsum_%d", p.weight_keys());
     return run(name, 256u, true, [&](int b) { return p.parts(b) > 1 ? per_head(b, 256) : 0LL; });
+}
+
+int zt_attn_paged(const float *q, const float *k_pages, const float *v_pages, const int *table, float *out, float *lse,
+                  const float *w_in, float *w_out, const int *q_start, const int *n_rows, int B, int n_pages,
+                  int page_size, int table_stride, int w_stride, int n_heads, int n_kv_heads, int dim, void *workspace,
+                  size_t workspace_bytes, hipStream_t stream) {
+    return paged_attend("attn_paged", q, k_pages, v_pages, table, out, lse, w_in, w_out, nullptr, 0, q_start, n_rows, B,
+                        n_pages, page_size, table_stride, w_stride, n_heads, n_kv_heads, dim, workspace, workspace_bytes,
+                        false, stream);
+}
+
+int zt_attn_paged_tree(const float *q, const float *k_pages, const float *v_pages, const int *table, const uint64_t *mask,
+                       float *out, float *lse, const int *q_start, const int *n_rows, int B, int n_pages, int page_size,
+                       int table_stride, int words, int n_heads, int n_kv_heads, int dim, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream) {
+    return paged_attend("attn_paged_tree", q, k_pages, v_pages, table, out, lse, nullptr, nullptr, mask, words, q_start,
+                        n_rows, B, n_pages, page_size, table_stride, 0, n_heads, n_kv_heads, dim, workspace,
+                        workspace_bytes, true, stream);
+}
+
+int zt_tree_mask(const int *parent, uint64_t *mask, int *pos_out, const int *q_start, const int *pos, int B, int words,
+                 hipStream_t stream) {
+    if (B < 1 || !q_start || q_start[0] < 0) {
+        fprintf(stderr, "zt_attn: tree_mask of %d sequences needs the host q_start array, from 0 up.\n", B);
+        return 1;
+    }
+    for (int b = 0; b < B; ++b) {
+        if (q_start[b + 1] < q_start[b]) {
+            fprintf(stderr, "zt_attn: sequence %d has %lld new tokens.\n", b, (long long)q_start[b + 1] - q_start[b]);
+            return 1;
+        }
+    }
+    if (tree_words_check("tree_mask", q_start, B, words)) return 1;
+    if (!pos != !pos_out) {
+        fprintf(stderr, "zt_attn: tree_mask takes the host pos array and pos_out together or neither.\n");
+        return 1;
+    }
+    for (int b = 0; pos && b < B; ++b) {
+        if (pos[b] < 0 || (long long)pos[b] + (q_start[b + 1] - q_start[b]) > INT32_MAX) {
+            fprintf(stderr, "zt_attn: sequence %d's tree begins at position %d.\n", b, pos[b]);
+            return 1;
+        }
+    }
+    if (q_start[B] > q_start[0] && (!parent || !mask)) {
+        fprintf(stderr, "zt_attn: a null tensor pointer is not launchable.\n");
+        return 1;
+    }
+    if ((uintptr_t)mask & 7) {
+        fprintf(stderr, "zt_attn: masks at %p are not 8-byte aligned.\n", (const void *)mask);
+        return 1;
+    }
+    DeviceState *st = require_device();
+    if (!st) return 1;
+    TreeMaskArgs a{};
+    a.parent = parent; a.mask = reinterpret_cast<unsigned long long *>(mask); a.pos = pos_out;
+    a.words = words;
+    // (The tokens are less than 2^31, 256 to a workgroup: a launch has room for any 64 sequences.)
+    for (int b = 0; b < B;) {
+        unsigned blocks = 0;
+        PagedSeqs &s = a.seq;
+        for (s.n = 0; b < B && s.n < ZT_PAGED_MAXB; ++b) {
+            const int q_len = q_start[b + 1] - q_start[b];
+            if (q_len == 0) continue;
+            const int i = s.n++;
+            s.b[i] = b; s.q0[i] = q_start[b]; s.q_len[i] = q_len; s.n_rows[i] = pos ? pos[b] : 0;
+            s.first[i] = (int)blocks;
+            blocks += ((unsigned)q_len + kThreads - 1) / kThreads;
+        }
+        if (blocks && launch(st, "zt_tree_mask", blocks, a, stream)) return 1;
+    }
+    return 0;
 }
 
 int zt_paged_append(const float *q, const float *k_new, const float *v_new, float *q_out, float *k_pages, float *v_pages,

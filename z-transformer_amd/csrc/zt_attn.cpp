@@ -20,7 +20,9 @@
 #include <cstring>
 #include <functional>
 #include <initializer_list>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -38,6 +40,9 @@ extern const unsigned char zt_co_cal[], zt_co_cal_end[];
 extern const unsigned char zt_co_gemm[], zt_co_gemm_end[];
 extern const unsigned char zt_co_paged[], zt_co_paged_end[];
 extern const unsigned char zt_co_evict[], zt_co_evict_end[];
+extern const unsigned char zt_co_tree[], zt_co_tree_end[];
+extern const unsigned char zt_co_pages[], zt_co_pages_end[];
+extern const unsigned char zt_co_rotary[], zt_co_rotary_end[];
 int zt_noalloc_scratch_address(void **ptr);  // noalloc.hip
 }
 
@@ -52,7 +57,7 @@ struct DeviceState {
     bool ok = false;
     size_t lds_limit = 0;
     int cus = 0;
-    hipModule_t mods[8] = {};
+    hipModule_t mods[11] = {};
     float *scratch = nullptr;  // this device's address of noalloc.hip's scratch (null: unavailable)
     std::mutex mu;
     std::unordered_map<std::string, hipFunction_t> fns;
@@ -70,6 +75,9 @@ int module_of(const char *name) {
     if (strncmp(name, "zt_gem", 6) == 0) return 5;
     if (strncmp(name, "zt_pag", 6) == 0) return 6;
     if (strncmp(name, "zt_evi", 6) == 0) return 7;
+    if (strncmp(name, "zt_tre", 6) == 0) return 8;
+    if (strncmp(name, "zt_poo", 6) == 0) return 9;
+    if (strncmp(name, "zt_tur", 6) == 0) return 10;
     return 3;
 }
 
@@ -91,9 +99,9 @@ void load_device(DeviceState &st, int dev) {
     int lds = 0;
     if (hipDeviceGetAttribute(&lds, hipDeviceAttributeMaxSharedMemoryPerBlock, dev) != hipSuccess || lds <= 0)
         return;
-    const unsigned char *images[8] = {zt_co_fwd, zt_co_bwd, zt_co_dec,   zt_co_misc,
-                                      zt_co_cal, zt_co_gemm, zt_co_paged, zt_co_evict};
-    for (int i = 0; i < 8; ++i) {
+    const unsigned char *images[11] = {zt_co_fwd,   zt_co_bwd,   zt_co_dec,  zt_co_misc,  zt_co_cal,   zt_co_gemm,
+                                       zt_co_paged, zt_co_evict, zt_co_tree, zt_co_pages, zt_co_rotary};
+    for (int i = 0; i < 11; ++i) {
         if (hipModuleLoadData(&st.mods[i], images[i]) != hipSuccess) {
             fprintf(stderr, "zt_attn: the gfx950 code object %d would not load on device %d.\n", i, dev);
             return;
@@ -1782,6 +1790,8 @@ int zt_product_plan(int product, int M, int K, int N, char *name, int len) {
 int zt_matmul_plan(int M, int K, int N, char *name, int len) { return zt_product_plan(0, M, K, N, name, len); }
 
 #include "paged.inl"
+#include "pages.inl"
+#include "rotary.inl"
 
 int zt_attn_set_tuning(const char *name, int value) {
     for (int i = 0; name && i < kTuneCount; ++i) {

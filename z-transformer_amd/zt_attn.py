@@ -28,6 +28,9 @@ ABI_SYMBOLS = [
     "zt_attn_backward_train_ws", "zt_attn_forward_train_ws", "zt_attn_set_tuning", "zt_attn_get_tuning",
     "zt_calibrate_launch", "zt_attn_decode_noalloc", "zt_matmul_plan", "zt_product_plan",
     "zt_attn_paged_workspace", "zt_attn_paged", "zt_paged_append", "zt_paged_evict",
+    "zt_tree_mask", "zt_attn_paged_tree", "zt_paged_keep", "zt_paged_fork_workspace", "zt_paged_fork", "zt_paged_free",
+    "zt_paged_compact_workspace", "zt_paged_compact", "zt_paged_copy", "zt_rope_frequencies", "zt_rope_at_forward",
+    "zt_rope_at_backward", "zt_paged_append_at",
 ]
 HOLDER_SYMBOLS = [
     "zt_bytes_for", "zt_to_cint", "zt_forward_bounds", "zt_holder_init", "zt_holder_deinit",
@@ -98,6 +101,19 @@ def load_library(path):
         "zt_attn_paged": (I, [P] * 10 + [I] * 8 + [P, Z, P]),
         "zt_paged_append": (I, [P] * 11 + [I] * 8 + [D, P]),
         "zt_paged_evict": (I, [P] * 8 + [I] * 10 + [P]),
+        "zt_tree_mask": (I, [P] * 5 + [I] * 2 + [P]),
+        "zt_attn_paged_tree": (I, [P] * 9 + [I] * 8 + [P, Z, P]),
+        "zt_paged_keep": (I, [P] * 7 + [I] * 6 + [P]),
+        "zt_paged_fork_workspace": (Z, [P, P] + [I] * 3),
+        "zt_paged_fork": (I, [P] * 8 + [I] * 5 + [P, Z, P]),
+        "zt_paged_free": (I, [P] * 3 + [I] * 4 + [P]),
+        "zt_paged_compact_workspace": (Z, [I]),
+        "zt_paged_compact": (I, [P] * 6 + [I] * 4 + [P, Z, P]),
+        "zt_paged_copy": (I, [P] * 3 + [I] * 5 + [P]),
+        "zt_rope_frequencies": (I, [P, I, D, I, D, D, D, D]),
+        "zt_rope_at_forward": (I, [P] * 6 + [I] * 6 + [D, P]),
+        "zt_rope_at_backward": (I, [P] * 6 + [I] * 6 + [D, P]),
+        "zt_paged_append_at": (I, [P] * 12 + [I] * 10 + [D, P]),
         "zt_calibrate": (I, [P, Z, P, Z, P, P, P]),
         "zt_calibrate_launch": (I, [ctypes.c_uint, ctypes.c_uint, I, P, P]),
         "zt_rope_forward": (I, [P, P, I, I, I, D, I, P]),
@@ -398,6 +414,173 @@ def paged_evict(k_pages, v_pages, table, table_out, w_in, w_out, kept, n_rows, p
                                 _host_ints(n_rows, B),
                                 *_c_ints(B, n_pages, page_size, table_stride, w_in.shape[-1], n_kv_heads, dim, n_first,
                                          n_last, budget), _stream(stream)), "zt_paged_evict")
+
+
+def _masks(mask, tokens):
+    """Words of a token's mask; mask [.., words] int64 (the bits of the C side's uint64)."""
+    import torch
+    if mask.dtype != torch.int64 or not mask.is_cuda or not mask.is_contiguous() or mask.dim() != 2:
+        raise ValueError("masks must be contiguous int64 [tokens, words] on the GPU")
+    if mask.shape[0] < tokens:
+        raise ValueError(f"{mask.shape[0]} masks where there are {tokens} tokens")
+    return mask.shape[1]
+
+
+def _at_least(n, *ts):
+    for t in ts:
+        if t is not None and t.numel() < n:
+            raise ValueError(f"{t.numel()} values where {n} are needed")
+
+
+def tree_mask(parent, mask, q_start, pos_out=None, pos=None, stream=None):
+    """parent int32, mask int64 [.., words], pos_out int32: packed tokens; pos: a host sequence of B ints."""
+    B, N = len(q_start) - 1, int(q_start[-1])
+    _i32_cuda(*[t for t in (parent, pos_out) if t is not None])
+    _here(parent, mask, pos_out)
+    words = _masks(mask, N)
+    _at_least(N, parent, pos_out)
+    _check(lib().zt_tree_mask(_ptr(parent), _ptr(mask), _ptr(pos_out), _host_ints(q_start, B + 1),
+                              None if pos is None else _host_ints(pos, B), *_c_ints(B, words), _stream(stream)),
+           "zt_tree_mask")
+
+
+def attn_paged_tree(q, k_pages, v_pages, table, mask, out, q_start, n_rows, page_size, n_heads, n_kv_heads, dim, workspace,
+                    lse=None, stream=None):
+    """workspace: a tensor of attn_paged_workspace_bytes(...) bytes, or None where that is 0."""
+    _f32_cuda(q, k_pages, v_pages, out, *[t for t in (lse,) if t is not None])
+    _i32_cuda(table)
+    _here(q, k_pages, v_pages, table, mask, out, workspace, lse)
+    words = _masks(mask, int(q_start[-1]))
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    B, table_stride = table.shape
+    n_pages = _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages,
+                            [(q, n_heads * dim), (out, n_heads * dim), (lse, n_heads)], None, B)
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().zt_attn_paged_tree(*map(_ptr, (q, k_pages, v_pages, table, mask, out, lse)), _host_ints(q_start, B + 1),
+                                    _host_ints(n_rows, B),
+                                    *_c_ints(B, n_pages, page_size, table_stride, words, n_heads, n_kv_heads, dim),
+                                    _ptr(workspace), nbytes, _stream(stream)), "zt_attn_paged_tree")
+
+
+def paged_keep(k_pages, v_pages, table, path, count, q_start, n_rows, page_size, n_kv_heads, dim, stream=None):
+    """path int32 [.., packed tokens], count int32 [B]."""
+    _f32_cuda(k_pages, v_pages)
+    _i32_cuda(table, path, count)
+    _here(k_pages, v_pages, table, path, count)
+    B, table_stride = table.shape
+    n_pages = _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages, [(path, 1)], None, B)
+    _at_least(B, count)
+    _check(lib().zt_paged_keep(*map(_ptr, (k_pages, v_pages, table, path, count)), _host_ints(q_start, B + 1),
+                               _host_ints(n_rows, B), *_c_ints(B, n_pages, page_size, table_stride, n_kv_heads, dim),
+                               _stream(stream)), "zt_paged_keep")
+
+
+def paged_fork_workspace_bytes(n_rows, n_room, n_pages, page_size):
+    n = len(n_rows)
+    return lib().zt_paged_fork_workspace(_host_ints(n_rows, n), _host_ints(n_room, n), *_c_ints(n, n_pages, page_size))
+
+
+def paged_fork(table, refs, pairs, missing, src, dst, n_rows, n_room, page_size, workspace, stream=None):
+    """table [B, pages], refs [n_pages], pairs [n, 2], missing [1]: int32; src, dst, n_rows, n_room: host sequences of n."""
+    _i32_cuda(table, refs, pairs, missing)
+    _here(table, refs, pairs, missing, workspace)
+    if not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    (B, table_stride), n = table.shape, len(src)
+    _at_least(2 * n, pairs)
+    _at_least(1, missing)
+    _check(lib().zt_paged_fork(*map(_ptr, (table, refs, pairs, missing)), *[_host_ints(x, n) for x in (src, dst, n_rows, n_room)],
+                               *_c_ints(n, B, refs.numel(), page_size, table_stride), _ptr(workspace),
+                               workspace.numel() * workspace.element_size(), _stream(stream)), "zt_paged_fork")
+
+
+def paged_free(table, refs, n_keep, page_size, stream=None):
+    """n_keep: a host sequence of B ints."""
+    _i32_cuda(table, refs)
+    _here(table, refs)
+    B, table_stride = table.shape
+    _check(lib().zt_paged_free(_ptr(table), _ptr(refs), _host_ints(n_keep, B),
+                               *_c_ints(B, refs.numel(), page_size, table_stride), _stream(stream)), "zt_paged_free")
+
+
+def paged_compact_workspace_bytes(n_pages):
+    return lib().zt_paged_compact_workspace(*_c_ints(n_pages))
+
+
+def paged_compact(table, refs, table_out, refs_out, pairs, moved, workspace, stream=None):
+    """pairs [most, 2], moved [2] int32; table_out and refs_out are table and refs, or buffers of their own."""
+    _i32_cuda(table, refs, table_out, refs_out, pairs, moved)
+    _here(table, refs, table_out, refs_out, pairs, moved, workspace)
+    if table_out.shape != table.shape or refs_out.shape != refs.shape or pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise ValueError("table and table_out, and refs and refs_out, have one shape; pairs is [most, 2]")
+    if not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    _at_least(2, moved)
+    B, table_stride = table.shape
+    _check(lib().zt_paged_compact(*map(_ptr, (table, refs, table_out, refs_out, pairs, moved)),
+                                  *_c_ints(pairs.shape[0], B, refs.numel(), table_stride), _ptr(workspace),
+                                  workspace.numel() * workspace.element_size(), _stream(stream)), "zt_paged_compact")
+
+
+def paged_copy(k_pages, v_pages, pairs, page_size, n_kv_heads, dim, stream=None):
+    """pairs [n, 2] int32."""
+    _f32_cuda(k_pages, v_pages)
+    _i32_cuda(pairs)
+    _here(k_pages, v_pages, pairs)
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise ValueError("pairs is [n, 2]")
+    n_pages = _paged_shapes((0,), n_kv_heads, dim, page_size, k_pages, v_pages, [], None, 1)
+    _check(lib().zt_paged_copy(*map(_ptr, (k_pages, v_pages, pairs)),
+                               *_c_ints(pairs.shape[0], n_pages, page_size, n_kv_heads, dim), _stream(stream)), "zt_paged_copy")
+
+
+ZT_ROPE_PLAIN, ZT_ROPE_LINEAR, ZT_ROPE_BASE, ZT_ROPE_TURNS = range(4)
+
+
+def rope_frequencies(rot_dim, theta=500000.0, scaling=ZT_ROPE_PLAIN, factor=1.0, low=1.0, high=4.0, context=8192.0):
+    """The angle per position of each pair, a host array of rot_dim / 2 doubles."""
+    rot_dim, scaling = _c_ints(rot_dim, scaling)
+    freq = (ctypes.c_double * min(max(1, rot_dim // 2), 128))()  # (the C side refuses more)
+    _check(lib().zt_rope_frequencies(freq, rot_dim, theta, scaling, factor, low, high, context), "zt_rope_frequencies")
+    return freq
+
+
+def _host_freq(freq, rot_dim):
+    if len(freq) < rot_dim // 2:
+        raise ValueError(f"{len(freq)} frequencies for {rot_dim} rotated columns")
+    return (ctypes.c_double * len(freq))(*[float(f) for f in freq])
+
+
+def rope_at(q, k, q_out, k_out, pos, freq, n_heads, n_kv_heads, head_dim, rot_dim, interleaved=False, amplitude=1.0,
+            backward=False, stream=None):
+    """pos [rows] int32; freq: rope_frequencies(...), or any host sequence; q or k may be None with its heads 0."""
+    _f32_cuda(*[t for t in (q, k, q_out, k_out) if t is not None])
+    _i32_cuda(pos)
+    _here(q, k, q_out, k_out, pos)
+    rows = pos.numel()
+    _at_least(rows * n_heads * head_dim, q, q_out)
+    _at_least(rows * n_kv_heads * head_dim, k, k_out)
+    fn = lib().zt_rope_at_backward if backward else lib().zt_rope_at_forward
+    _check(fn(*map(_ptr, (q, k, q_out, k_out, pos)), _host_freq(freq, rot_dim),
+              *_c_ints(rows, n_heads, n_kv_heads, head_dim, rot_dim, interleaved), amplitude, _stream(stream)), "zt_rope_at")
+
+
+def paged_append_at(q, k_new, v_new, q_out, k_pages, v_pages, table, pos, freq, q_start, n_rows, page_size, n_heads,
+                    n_kv_heads, dim, rot_dim, interleaved=False, amplitude=1.0, w=None, stream=None):
+    """paged_append at positions of each token's own: pos int32, packed tokens."""
+    _f32_cuda(k_new, v_new, k_pages, v_pages, *[t for t in (q, q_out, w) if t is not None])
+    _i32_cuda(table, pos)
+    _here(q, k_new, v_new, q_out, k_pages, v_pages, table, pos, w)
+    B, table_stride = table.shape
+    n_pages = _paged_shapes(q_start, n_kv_heads, dim, page_size, k_pages, v_pages,
+                            [(q, n_heads * dim), (q_out, n_heads * dim), (k_new, n_kv_heads * dim),
+                             (v_new, n_kv_heads * dim), (pos, 1)], w, B)
+    _check(lib().zt_paged_append_at(*map(_ptr, (q, k_new, v_new, q_out, k_pages, v_pages, table, w, pos)),
+                                    _host_freq(freq, rot_dim), _host_ints(q_start, B + 1), _host_ints(n_rows, B),
+                                    *_c_ints(B, n_pages, page_size, table_stride, 0 if w is None else w.shape[-1], n_heads,
+                                             n_kv_heads, dim, rot_dim, interleaved), amplitude, _stream(stream)),
+           "zt_paged_append_at")
 
 
 def rmsnorm(x, w, y, rows, cols, eps=1e-5, stream=None):
