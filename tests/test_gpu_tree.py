@@ -460,7 +460,8 @@ class Pool:
 
 
 @pytest.mark.parametrize("B,stride,n_pages,page,lacks", [(6, 8, 20, 4, True), (200, 70, 4200, 16, True), (70, 300, 5000, 1, True),
-                                                         (3, 5, 8192, 1024, False), (150, 4, 4097, 8, False)])
+                                                         (3, 5, 8192, 1024, False), (150, 4, 4097, 8, False),
+                                                         (100, 500, 16385, 1, True), (200, 350, 20011, 2, True), (90, 40, 16384, 8, False)])
 def test_pages_in_use(gpu, zt, B, stride, n_pages, page, lacks):
     """Forks, growth, cuts, frees and compactions at random: tables and counts as treeref has them, the counts those of the
     tables; also calls that lack pages, and page tables that have been cut back into a shared page."""
@@ -520,16 +521,17 @@ def test_entries_that_name_no_page(gpu, zt):
     p.free([3, 100, 0, 0])
 
 
-def test_a_full_pool_and_an_empty_one(gpu, zt):
-    p = Pool(gpu, zt, 2, 9000, 8192, 1)
+@pytest.mark.parametrize("n_pages", [4096, 8192, 16384, 16385, 20480])
+def test_a_full_pool_and_an_empty_one(gpu, zt, n_pages):
+    p = Pool(gpu, zt, 2, n_pages + 100, n_pages, 1)
     p.compact(5, False)
-    assert p.fork([0], [0], [0], [8192])[1] == 0
+    assert p.fork([0], [0], [0], [n_pages])[1] == 0
     p.compact(5, False)
     assert p.fork([1], [1], [0], [1])[1] == 1
-    p.free([4100, 0])
-    assert p.fork([0], [1], [100], [100 + 4092])[1] == 0
-    p.free([0, 9000])
-    p.compact(8192, True)
+    p.free([n_pages // 2 + 4, 0])
+    assert p.fork([0], [1], [100], [100 + n_pages // 2 - 4])[1] == 0
+    p.free([0, n_pages + 100])
+    p.compact(n_pages, True)
 
 
 @pytest.mark.parametrize("page,Hkv,d", [(1, 2, 32), (8, 8, 128), (16, 3, 50), (64, 1, 34), (1024, 2, 256)])

@@ -136,12 +136,12 @@ def test_workspaces_follow_the_numbers(zt):
     def need(n_rows, n_room, n_pages=100, page=16):
         return L.zt_paged_fork_workspace(ints(n_rows), ints(n_room), len(n_rows), n_pages, page)
 
-    # A count per segment of 4096 pages, one per entry, two numbers per page that may be wanted.
+    # A count per segment of 1024 pages, one per entry, two numbers per page that may be wanted.
     assert need((5,), (5,)) == 4 * (1 + 1 + 2) and need((16,), (16,)) == 4 * 2 and need((5, 16), (40, 16)) == 4 * (1 + 2 + 6)
-    assert need((5,), (5,), n_pages=4097) == 4 * (2 + 1 + 2)
+    assert need((5,), (5,), n_pages=1025) == 4 * (2 + 1 + 2)
     assert need((5,), (4,)) == need((-1,), (4,)) == need((5,), (5,), page=3) == need((5,), (5,), n_pages=0) == 0
     assert need((0,), ((1 << 30) + 1,)) == 0
-    assert L.zt_paged_compact_workspace(0) == 0 and L.zt_paged_compact_workspace(4097) == 4 * (2 + 4097)
+    assert L.zt_paged_compact_workspace(0) == 0 and L.zt_paged_compact_workspace(4097) == 4 * (5 + 4097)
 
 
 @pytest.mark.parametrize("rot", [2, 4, 48, 128, 256])

@@ -179,7 +179,12 @@ struct PagedEvictArgs {
 };
 
 // Pages: refs[p] counts the table entries that name page p.
-#define ZT_PAGES_SEGMENT 4096  // pages that a workgroup counts
+#define ZT_PAGES_SEGMENT 1024   // pages that a workgroup counts
+#define ZT_PAGES_ONE 16384      // pages of a pool that one workgroup numbers by itself
+#define ZT_PAGES_ONE_SLOTS 4096 // columns that may need a page, of all sequences that it serves
+#define ZT_PAGES_MAXE 128       // entries of a launch that forks
+#define ZT_PAGES_COPY 2048      // 16-byte (8-byte) chunks that a workgroup copies at a time
+#define ZT_PAGES_MAXF 256       // sequences of a launch that frees
 
 // Sequences that go on from others, or grow: a launch's entries entry0 .. entry0 + n - 1 of `entries`.
 struct ForkArgs {
@@ -192,13 +197,13 @@ struct ForkArgs {
     int *rank;              // [slots] which of its entry's fresh pages a column takes, or -1
     int *list;              // the free pages in order, `slots` at most
     int n_pages, shift, table_stride, segments, entries, entry0, n, slots;
-    int src[ZT_PAGED_MAXB], dst[ZT_PAGED_MAXB], n_rows[ZT_PAGED_MAXB], n_room[ZT_PAGED_MAXB], slot0[ZT_PAGED_MAXB];
+    int src[ZT_PAGES_MAXE], dst[ZT_PAGES_MAXE], n_rows[ZT_PAGES_MAXE], n_room[ZT_PAGES_MAXE], slot0[ZT_PAGES_MAXE];
 };
 
 struct FreeArgs {
     int *table, *refs;
     int n_pages, table_stride, blocks;  // workgroups of a sequence
-    int b[ZT_PAGED_MAXB], from[ZT_PAGED_MAXB];
+    int b[ZT_PAGES_MAXF], from[ZT_PAGES_MAXF];
 };
 
 struct CompactArgs {

@@ -10,8 +10,9 @@
 
 DEVI bool is_page(int p, int n_pages) { return (unsigned)p < (unsigned)n_pages; }
 
-// Sum over the lanes below (exclusive) and over all 256 threads; both uniform calls of a whole workgroup.
-DEVI int block_scan(int x, int *total, int (&waves)[4]) {
+// Sum over the threads below (exclusive), and over all of a workgroup's; a uniform call of the whole workgroup.
+template <int NW>
+DEVI int block_scan(int x, int *total, int (&waves)[NW]) {
     const int lane = lane_id(), w = threadIdx.x >> 6;
     int s = x;
 #pragma unroll
@@ -24,7 +25,7 @@ DEVI int block_scan(int x, int *total, int (&waves)[4]) {
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NW; ++i) {
         before += i < w ? waves[i] : 0;
         all += waves[i];
     }
@@ -40,13 +41,41 @@ DEVI int block_sum(const int *counts, int n, int (&waves)[4]) {
     return total;
 }
 
+// The pages of a pool that one workgroup of 1024 threads numbers: thread t takes pages 1024 e + t.  flag(e) of them is
+// counted in the pages' order: of(e, .) pages before thread t's e-th one.
+struct OnePool {
+    static constexpr int E = ZT_PAGES_ONE / 1024;
+    int counts[E * 16];  // of each 64 pages, then before them
+};
+template <class Flag>
+DEVI int pool_number(OnePool &s, Flag flag, int (&before)[OnePool::E], int (&waves)[16]) {
+    constexpr int E = OnePool::E;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(flag(e));
+        before[e] = __popcll(m & ((1ull << lane) - 1));
+        if (lane == 0) s.counts[16 * e + w] = __popcll(m);
+    }
+    __syncthreads();
+    const int x = tid < 16 * E ? s.counts[tid] : 0;
+    int total;
+    const int at = block_scan(x, &total, waves);
+    if (tid < 16 * E) s.counts[tid] = at;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) before[e] += s.counts[16 * e + w];
+    return total;
+}
+
 // ---- Fork and growth --------------------------------------------------------------------
 //
 // Entry i: sequence dst goes on from src's first n_rows rows, with pages for n_room.  Of its table's columns those
 // below whole = n_rows / page are src's pages (one reference more each, where dst is another sequence); the columns
 // from there to want = ceil(n_room / page) are its own: kept where src is dst and nobody else refers to the page, else fresh ones.  A
 // fresh page for column `whole` of a partly filled one is asked to be copied: pairs[i].
-// Three launches: (1) the free pages of each segment of kSegment, and each entry's fresh columns, are counted; (2) the
+// Up to ZT_PAGES_ONE pages and ZT_PAGES_ONE_SLOTS columns a workgroup does it by itself (zt_pool_fork_one); else in
+// three launches: (1) the free pages of each segment of kSegment, and each entry's fresh columns, are counted; (2) the
 // free pages are numbered and listed, as many as could be wanted; (3) each entry takes those of its numbers. If there are too few, nothing is
 // changed but `missing`.
 constexpr int kSegment = ZT_PAGES_SEGMENT;
@@ -139,6 +168,105 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_fork(ForkArgs a) {
         for (int j = want + (int)threadIdx.x; j < a.table_stride; j += 256) to[j] = -1;
 }
 
+// The same by one workgroup, a wave to an entry.  The entries are read from the arguments, which are far, once, all at
+// the same time.
+extern "C" __global__ void __launch_bounds__(1024) zt_pool_fork_one(ForkArgs a) {
+    constexpr int E = OnePool::E;
+    struct Entry {
+        int src, dst, whole, want, part, slot0;
+    };
+    __shared__ Entry entry[ZT_PAGES_MAXE];
+    __shared__ int waves[16], base[ZT_PAGES_MAXE];
+    __shared__ int rank[ZT_PAGES_ONE_SLOTS], list[ZT_PAGES_ONE_SLOTS];
+    __shared__ OnePool pool;
+    const int tid = threadIdx.x, lane = tid & 63, page = 1 << a.shift;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // The thread's pages, loaded now, used below.
+    int mine[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine[e] = 1024 * e + tid < a.n_pages ? a.refs[1024 * e + tid] : 1;
+    if (tid < a.n) {
+        const int rows = a.n_rows[tid], room = a.n_room[tid];
+        entry[tid] = {a.src[tid], a.dst[tid], rows >> a.shift, (room + page - 1) >> a.shift, rows & (page - 1), a.slot0[tid]};
+    }
+    __syncthreads();
+    for (int i = w; i < a.n; i += 16) {
+        const Entry x = entry[i];
+        int fresh = 0;
+        if (x.src != x.dst) {
+            fresh = x.want - x.whole;
+        } else {
+            const int *row = a.table + (size_t)x.src * a.table_stride;
+            for (int j0 = x.whole; j0 < x.want; j0 += 64) {  // wave-uniform
+                const int j = j0 + lane;
+                bool take = false;
+                if (j < x.want) {
+                    const int p = row[j];
+                    take = !(is_page(p, a.n_pages) && a.refs[p] == 1);
+                }
+                const unsigned long long all = __builtin_amdgcn_ballot_w64(take);
+                if (j < x.want) rank[x.slot0 + j - x.whole] = take ? fresh + __popcll(all & ((1ull << lane) - 1)) : -1;
+                fresh += __popcll(all);
+            }
+        }
+        if (lane == 0) base[i] = fresh;
+    }
+    int before[E];
+    const int total = pool_number(pool, [&](int e) { return mine[e] == 0; }, before, waves);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (mine[e] == 0 && before[e] < a.slots) list[before[e]] = 1024 * e + tid;
+    // Every thread has read what it needs of the counts: they may change from here on.
+    const int x = tid < a.n ? base[tid] : 0;  // (written before the numbering's barriers)
+    int fresh;
+    const int first = block_scan(x, &fresh, waves);
+    if (tid < a.n) base[tid] = first;
+    if (tid == 0) *a.missing = max(0, fresh - total);
+    for (int i = tid; i < 2 * a.n; i += 1024) a.pairs[i] = -1;
+    __syncthreads();
+    if (fresh > total) return;  // workgroup-uniform
+    const auto put = [&](int i, const Entry &x, int j, int p) {  // column j of entry i, where its source has p
+        const bool self = x.src == x.dst, there = is_page(p, a.n_pages);
+        int *to = a.table + (size_t)x.dst * a.table_stride + j;
+        if (j >= x.want) {
+            if (!self) *to = -1;
+        } else if (j < x.whole) {
+            if (self) return;
+            *to = p;
+            if (there) atomicAdd(a.refs + p, 1);
+        } else {
+            const int r = self ? rank[x.slot0 + j - x.whole] : j - x.whole;
+            if (r < 0) return;
+            const int f = list[base[i] + r];
+            *to = f;
+            atomicAdd(a.refs + f, 1);
+            if (self && there) atomicSub(a.refs + p, 1);
+            if (j == x.whole && x.part) {
+                a.pairs[2 * i] = p;
+                a.pairs[2 * i + 1] = f;
+            }
+        }
+    };
+    // 64 columns of an entry at a time, and four such pieces: their reads do not wait for one another.
+    constexpr int U = 4;
+    const int pieces = (a.table_stride + 63) >> 6, items = a.n * pieces;
+    for (int item0 = w; item0 < items; item0 += 16 * U) {
+        int p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int item = min(item0 + 16 * u, items - 1), i = item / pieces, j = (item - i * pieces) * 64 + lane;
+            p[u] = j < a.table_stride ? a.table[(size_t)entry[i].src * a.table_stride + j] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int item = item0 + 16 * u;
+            if (item >= items) break;
+            const int i = item / pieces, j = (item - i * pieces) * 64 + lane;
+            if (j < a.table_stride) put(i, entry[i], j, p[u]);
+        }
+    }
+}
+
 // ---- Freeing ------------------------------------------------------------------------------
 //
 // Sequence b keeps its table's first from[i] pages; the entries behind them lose their reference and become -1.
@@ -155,7 +283,8 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_free(FreeArgs a) {
 // ---- Compaction ----------------------------------------------------------------------------
 //
 // With L pages in use: the k-th lowest free page below L takes what the k-th highest page in use, past L, holds (there
-// are as many of the one as of the other), for k < max_pairs.  Three launches: (1) the pages in use of each segment
+// are as many of the one as of the other), for k < max_pairs.  Up to ZT_PAGES_ONE pages a workgroup does it by itself
+// (zt_pool_compact_one); else in three launches: (1) the pages in use of each segment
 // are counted; (2) both kinds are numbered: pairs, and of each page what becomes of it; (3) tables and counts are written.
 constexpr int kStays = -1, kFilled = -2;  // else the number of the pair that it is the source of
 
@@ -217,13 +346,66 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_move(CompactArgs a) {
     }
 }
 
+// The same by one workgroup; the new numbers of all pages are kept in LDS.
+extern "C" __global__ void __launch_bounds__(1024) zt_pool_compact_one(CompactArgs a) {
+    constexpr int E = OnePool::E;
+    __shared__ int waves[16], holes[ZT_PAGES_ONE / 2], now[ZT_PAGES_ONE], above;
+    __shared__ OnePool pool;
+    const int tid = threadIdx.x;
+    int mine[E], before[E];  // before: pages in use below
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine[e] = 1024 * e + tid < a.n_pages ? a.refs[1024 * e + tid] : 0;
+    if (tid == 0) above = 0;
+    const int L = pool_number(pool, [&](int e) { return mine[e] != 0; }, before, waves);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int p = 1024 * e + tid;
+        // (A hole below L has a page in use past L to fill it: there are at most half as many as pages.)
+        if (p < L && mine[e] == 0 && p - before[e] < a.max_pairs) holes[p - before[e]] = p;
+        if (p == L && p < a.n_pages) above = L - before[e];  // pages in use from L on
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int p = 1024 * e + tid;
+        if (p >= a.n_pages) break;
+        const int k = L - 1 - before[e];  // of a page in use past L, from the highest down
+        const bool moves = mine[e] != 0 && p >= L && k < a.max_pairs;
+        const bool filled = mine[e] == 0 && p < L && p - before[e] < a.max_pairs;
+        int to = p;
+        if (moves) {
+            to = holes[k];
+            a.pairs[2 * (size_t)k] = p;
+            a.pairs[2 * (size_t)k + 1] = to;
+            a.refs_out[to] = mine[e];
+            a.refs_out[p] = 0;
+        } else if (!filled && a.refs_out != a.refs) {
+            a.refs_out[p] = mine[e];
+        }
+        now[p] = to;
+    }
+    __syncthreads();
+    const int m = min(above, a.max_pairs);
+    if (tid == 0) {
+        a.moved[0] = m;
+        a.moved[1] = above - m;
+    }
+    for (long long i = 2LL * m + tid; i < 2LL * a.max_pairs; i += 1024) a.pairs[i] = -1;
+    for (long long i = tid; i < a.entries; i += 1024) {
+        const int p = a.table[i];
+        a.table_out[i] = is_page(p, a.n_pages) ? now[p] : p;
+    }
+}
+
 // ---- Copies ---------------------------------------------------------------------------------
 //
-// Pages of K and V from pairs[2 i] to pairs[2 i + 1], a workgroup 256 x 4 chunks of N floats at a time.  A pair with a
-// number that is none of the pool's is passed over.  Bound: HBM.
+// Pages of K and V from pairs[2 i] to pairs[2 i + 1], a workgroup 256 x U chunks of N floats at a time.  A pair with a
+// number that is none of the pool's is passed over.  Bound: HBM: 600 pages
+// of 64 rows of 8 heads at d = 128, 123 us, 5.1 TB/s (a copy of 2 GiB 5.0; U = 4 128 us, stores past the caches 135).
 template <int N>
 DEVI void pool_copy(const CopyArgs &a) {
     typedef float vec __attribute__((ext_vector_type(N)));
+    constexpr int U = ZT_PAGES_COPY / 256;
     const long long items = 2LL * a.n_pairs * a.pieces;
     for (long long item = blockIdx.x; item < items; item += gridDim.x) {
         const int piece = (int)(item % a.pieces);
@@ -233,13 +415,13 @@ DEVI void pool_copy(const CopyArgs &a) {
         float *const base = rest & 1 ? a.v : a.k;
         const vec *x = reinterpret_cast<const vec *>(base + (size_t)from * a.page_floats);
         vec *y = reinterpret_cast<vec *>(base + (size_t)to * a.page_floats);
-        const long long n = a.page_floats / N, c0 = piece * 1024LL + threadIdx.x;
-        vec t[4];
+        const long long n = a.page_floats / N, c0 = piece * (long long)ZT_PAGES_COPY + threadIdx.x;
+        vec t[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
             if (c0 + 256 * u < n) t[u] = __builtin_nontemporal_load(x + c0 + 256 * u);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
             if (c0 + 256 * u < n) y[c0 + 256 * u] = t[u];
     }
 }

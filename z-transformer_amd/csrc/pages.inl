@@ -97,12 +97,18 @@ int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *sr
     while (1 << a.shift < page_size) ++a.shift;
     a.segments = page_segments(n_pages);
     a.entries = n; a.slots = (int)slots;
-    // Counts for all entries, a launch for each ZT_PAGED_MAXB; the list; and what they take, in launches alike.
+    // One workgroup does a small call: freeing, forking 5 entries of 22 columns and copying 19.6 us, with three launches
+    // 26.6, which is their way through the host.  With more columns it takes longer: 78 entries of 66 16.7 us, the three
+    // launches 3.8 + 3.0 + 5.1 (the same pass 30.5 / 27.2).
+    long long columns = 0;
+    for (int i = 0; i < n; ++i) columns += src[i] == dst[i] ? pages_of(n_room[i], page_size) - n_rows[i] / page_size : table_stride;
+    const bool one = n <= ZT_PAGES_MAXE && n_pages <= ZT_PAGES_ONE && slots <= ZT_PAGES_ONE_SLOTS && columns <= 2048;
+    // Counts for all entries, a launch for each ZT_PAGES_MAXE; the list; and what they take, in launches alike.
     for (const bool take : {false, true}) {
         long long slot = 0;
-        for (int e0 = 0; e0 < n; e0 += ZT_PAGED_MAXB) {
+        for (int e0 = 0; e0 < n; e0 += ZT_PAGES_MAXE) {
             a.entry0 = e0;
-            a.n = std::min(n - e0, ZT_PAGED_MAXB);
+            a.n = std::min(n - e0, ZT_PAGES_MAXE);
             a.pairs = pairs + 2 * (size_t)e0;
             for (int i = 0; i < a.n; ++i) {
                 a.src[i] = src[e0 + i]; a.dst[i] = dst[e0 + i];
@@ -110,6 +116,7 @@ int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *sr
                 a.slot0[i] = (int)slot;
                 slot += pages_of(a.n_room[i], page_size) - a.n_rows[i] / page_size;
             }
+            if (one) return launch(st, "zt_pool_fork_one", 1u, a, stream, 1024);
             const unsigned blocks = (unsigned)a.n + (!take && e0 == 0 ? (unsigned)a.segments : 0);
             if (launch(st, take ? "zt_pool_fork" : "zt_pool_count", blocks, a, stream)) return 1;
         }
@@ -141,7 +148,7 @@ int zt_paged_free(int *table, int *refs, const int *n_keep, int B, int n_pages, 
     a.table = table; a.refs = refs; a.n_pages = n_pages; a.table_stride = table_stride;
     for (int b = 0; b < B;) {
         int n = 0, least = table_stride;
-        for (; b < B && n < ZT_PAGED_MAXB; ++b) {
+        for (; b < B && n < ZT_PAGES_MAXF; ++b) {
             const int from = pages_of(n_keep[b], page_size);
             if (from >= table_stride) continue;
             a.b[n] = b;
@@ -187,6 +194,9 @@ int zt_paged_compact(const int *table, const int *refs, int *table_out, int *ref
     a.seg_used = static_cast<int *>(workspace); a.becomes = a.seg_used + a.segments;
     a.entries = (long long)B * table_stride;
     a.n_pages = n_pages; a.max_pairs = max_pairs;
+    // One workgroup does a pool that it numbers in one go and a table of few rounds: 130 pages and their copy 11.8 us, with
+    // three launches 17.7; 3437 pages 7.4 us, the three 7.7 + 10.7 + 4.9.
+    if (n_pages <= ZT_PAGES_ONE && a.entries <= 65536) return launch(st, "zt_pool_compact_one", 1u, a, stream, 1024);
     if (launch(st, "zt_pool_used", (unsigned)a.segments, a, stream)) return 1;
     if (launch(st, "zt_pool_pair", (unsigned)a.segments, a, stream)) return 1;
     const long long work = std::max<long long>(a.entries, n_pages);
@@ -214,7 +224,7 @@ int zt_paged_copy(float *k_pages, float *v_pages, const int *pairs, int n_pairs,
     CopyArgs a{};
     a.k = k_pages; a.v = v_pages; a.pairs = pairs; a.n_pairs = n_pairs; a.n_pages = n_pages;
     a.page_floats = (long long)page_size * n_kv_heads * dim;
-    a.pieces = (int)((a.page_floats / n + 1023) / 1024);
+    a.pieces = (int)((a.page_floats / n + ZT_PAGES_COPY - 1) / ZT_PAGES_COPY);
     const long long items = 2LL * n_pairs * a.pieces;
     return launch(st, n == 4 ? "zt_pool_copy_4" : "zt_pool_copy_2", (unsigned)std::min(items, 1LL << 20), a, stream);
 }
