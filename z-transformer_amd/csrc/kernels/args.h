@@ -252,7 +252,7 @@ struct TurnArgs {
     const float *q, *k;
     float *q_out, *k_out;
     const int *pos;            // [rows of the batch]
-    int rows, row0, H, Hkv, dim, rot;
+    int row0, rows, H, Hkv, dim, rot;
     int slices;                // parts that a row group's heads are cut into
     double amplitude, sine;    // of the cosines, and of the sines, negative for the way back
     double freq[ZT_MAX_DIM / 2];

@@ -73,15 +73,13 @@ namespace {
 template <class Args>
 int turn_launch(DeviceState *st, const char *name, Args &x, TurnArgs &a, long long rows, long long units,
                 hipStream_t stream) {
-    const int per = std::min(16, 256 / (a.rot / 2));
-    const long long most = 0xFFFFFFFFll / kThreads * per;
+    const long long most = 0xFFFFFFFFll / kThreads;
     const int row0 = a.row0;
     for (long long r = 0; r < rows; r += most) {
         a.row0 = (int)(row0 + r);
         a.rows = (int)std::min(most, rows - r);
-        const long long groups = ((long long)a.rows + per - 1) / per;
-        a.slices = (int)std::max(1LL, std::min(512 / groups, (std::min(a.rows, per) * units + kThreads - 1) / kThreads));
-        if (launch(st, name, (unsigned)(groups * a.slices), x, stream)) return 1;
+        a.slices = (int)std::max(1LL, std::min(1024LL / a.rows, (units + kThreads - 1) / kThreads));
+        if (launch(st, name, (unsigned)a.rows * (unsigned)a.slices, x, stream)) return 1;
     }
     return 0;
 }
