@@ -73,9 +73,9 @@ ZT_TREE(128)
 ZT_TREE(192)
 ZT_TREE(256)
 ZT_TREE_MANY(32, 4, 1) ZT_TREE_MANY(32, 4, 2) ZT_TREE_MANY(32, 8, 2)
-ZT_TREE_MANY(64, 4, 1) ZT_TREE_MANY(64, 4, 2) ZT_TREE_MANY(64, 8, 2)
-ZT_TREE_MANY(96, 4, 1) ZT_TREE_MANY(96, 4, 2) ZT_TREE_MANY(96, 8, 2)
-ZT_TREE_MANY(128, 4, 1) ZT_TREE_MANY(128, 4, 2) ZT_TREE_MANY(128, 8, 2)
+ZT_TREE_MANY(64, 4, 1) ZT_TREE_MANY(64, 4, 2) ZT_TREE_MANY(64, 8, 1) ZT_TREE_MANY(64, 8, 2)
+ZT_TREE_MANY(96, 4, 1) ZT_TREE_MANY(96, 4, 2) ZT_TREE_MANY(96, 8, 1) ZT_TREE_MANY(96, 8, 2)
+ZT_TREE_MANY(128, 4, 1) ZT_TREE_MANY(128, 4, 2) ZT_TREE_MANY(128, 8, 1) ZT_TREE_MANY(128, 8, 2)
 ZT_TREE_MANY(192, 4, 1) ZT_TREE_MANY(192, 8, 1)
 ZT_TREE_MANY(256, 8, 1)
 ZT_TREE_FEW(32, 2) ZT_TREE_FEW(64, 2) ZT_TREE_FEW(96, 2) ZT_TREE_FEW(128, 2)

@@ -483,7 +483,17 @@ static int paged_attend(const char *who, const float *q, const float *k_pages, c
     for (int ki = 0; ki < kPagedKinds; ++ki) {
         const PagedKind kind = (PagedKind)ki;
         const bool few = paged_few(kind);
-        const PagedShape shape = paged_shape(kind, dp);
+        PagedShape shape = paged_shape(kind, dp);
+        // Trees of 65 to 128 rows on a grid of at most one workgroup per CU take eight waves of 16 rows, two to a SIMD, and not
+        // four of 32 that nothing runs beside.  Measured on MI355X (us, four / eight): 26 tokens of 32 over 8 heads at d = 128 on 1000
+        // rows 29.6 / 25.5, 4103 (208 workgroups) 38.4 / 32.5, 30 of 24 over 8 heads at d = 96 on 4000 27.6 / 24.8, 4 sequences of 40
+        // of 12 over 4 at d = 64 on 2000 24.9 / 24.1; past it, 26 on 8000 52.6 / 57.0; 50 of 4 over 2 at d = 32 on 2000 20.3 / 21.5.
+        if (tree && kind == kMany128 && dp >= 64 && dp <= 128) {
+            long long wgs = 0;
+            for (int b = 0; b < B; ++b)
+                if (p.any(b) && p.kind(b) == kind) wgs += p.items(b);
+            if (wgs <= st->cus) shape = PagedShape{8, 1};
+        }
         a.scores = weights && (few || p.keep) ? reinterpret_cast<float *>(ws + space.scores) : nullptr;
         long long part0 = 0, score0 = 0;
         const auto fill = [&](int i, int b) {
