@@ -260,7 +260,7 @@ int zt_attn_paged_tree(const float *q, const float *k_pages, const float *v_page
 /* The rows that stay of the new ones: of each sequence's new tokens the one with number path[i] becomes new
  * row i, for i < count[b] (DEVICE ints; path packed as q's rows, path[i] >= i, as in any tree; others, and
  * numbers of no new token, move nothing).  The sequence's new n_rows is n_rows less its new tokens plus
- * count[b]; rows behind hold what they held, or parts of it.  n_rows and q_start (HOST) are those of the append.  The pages of the
+ * count[b]; rows behind those are left as they are.  n_rows and q_start (HOST) are those of the append.  The pages of the
  * new rows must not be shared.  Where a row's old or new page is none of the pool's, it is not moved. */
 int zt_paged_keep(float *k_pages, float *v_pages, const int *table, const int *path, const int *count, const int *q_start,
                   const int *n_rows, int B, int n_pages, int page_size, int table_stride, int n_kv_heads, int dim,
@@ -278,8 +278,9 @@ int zt_paged_keep(float *k_pages, float *v_pages, const int *table, const int *p
  * rest are free pages.  Where src[i] == dst[i] (growth), pages that are there stay, but a page from the
  * partly filled one on that another entry names as well is replaced, as every page that the sequence may write must be
  * its own.  pairs [n, 2] (DEVICE) receives the old and the new number of the page to copy, -1, -1 where there is
- * none.  Pages are taken from the lowest free number up, in the order of entries and columns.  If fewer are free than
- * needed, *missing (DEVICE) receives how many, pairs -1, and nothing else changes; else 0.  dst are all different, and none is another
+ * none; an old page may be free by then, and is to be copied before another call takes pages.  Pages are taken from the
+ * lowest free number up, in the order of entries and columns.  If fewer are free than needed, *missing (DEVICE) receives
+ * how many are short, pairs -1, and nothing else changes; else it receives 0.  dst are all different, and none is another
  * entry's src.  n <= B.  `workspace`: zt_paged_fork_workspace(...) bytes, 16-byte aligned. */
 size_t zt_paged_fork_workspace(const int *n_rows, const int *n_room, int n, int n_pages, int page_size);
 int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *src, const int *dst, const int *n_rows,

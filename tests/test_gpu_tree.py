@@ -461,7 +461,8 @@ class Pool:
 
 @pytest.mark.parametrize("B,stride,n_pages,page,lacks", [(6, 8, 20, 4, True), (200, 70, 4200, 16, True), (70, 300, 5000, 1, True),
                                                          (3, 5, 8192, 1024, False), (150, 4, 4097, 8, False),
-                                                         (100, 500, 16385, 1, True), (200, 350, 20011, 2, True), (90, 40, 16384, 8, False)])
+                                                         (100, 500, 16385, 1, True), (200, 350, 20011, 2, True), (90, 40, 16384, 8, False),
+                                                         (300, 5, 900, 8, False)])
 def test_pages_in_use(gpu, zt, B, stride, n_pages, page, lacks):
     """Forks, growth, cuts, frees and compactions at random: tables and counts as treeref has them, the counts those of the
     tables; also calls that lack pages, and page tables that have been cut back into a shared page."""

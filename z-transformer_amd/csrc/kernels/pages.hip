@@ -83,7 +83,7 @@ constexpr int kSegment = ZT_PAGES_SEGMENT;
 extern "C" __global__ void __launch_bounds__(256) zt_pool_count(ForkArgs a) {
     __shared__ int waves[4];
     if ((int)blockIdx.x >= a.n) {  // a segment
-        const int seg = (int)blockIdx.x - a.n, p0 = seg * kSegment, p1 = min(a.n_pages, p0 + kSegment);
+        const int seg = (int)blockIdx.x - a.n, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
         int x = 0, total;
         for (int p = p0 + (int)threadIdx.x; p < p1; p += 256) x += a.refs[p] == 0;
         block_scan(x, &total, waves);
@@ -115,7 +115,7 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_count(ForkArgs a) {
 
 extern "C" __global__ void __launch_bounds__(256) zt_pool_list(ForkArgs a) {
     __shared__ int waves[4];
-    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = min(a.n_pages, p0 + kSegment);
+    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
     int at = block_sum(a.seg_free, seg, waves);
     for (int q = p0; q < p1 && at < a.slots; q += 256) {  // workgroup-uniform
         const int p = q + (int)threadIdx.x;
@@ -271,7 +271,8 @@ extern "C" __global__ void __launch_bounds__(1024) zt_pool_fork_one(ForkArgs a) 
 //
 // Sequence b keeps its table's first from[i] pages; the entries behind them lose their reference and become -1.
 extern "C" __global__ void __launch_bounds__(256) zt_pool_free(FreeArgs a) {
-    const int i = (int)blockIdx.x / a.blocks, j = a.from[i] + ((int)blockIdx.x % a.blocks) * 256 + (int)threadIdx.x;
+    const int i = (int)blockIdx.x / a.blocks;
+    const long long j = a.from[i] + (long long)((int)blockIdx.x % a.blocks) * 256 + threadIdx.x;
     if (j >= a.table_stride) return;
     int *at = a.table + (size_t)a.b[i] * a.table_stride + j;
     const int p = *at;
@@ -292,7 +293,7 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_used(CompactArgs a) {
     __shared__ int waves[4];
     const long long step = 256LL * gridDim.x;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < 2LL * a.max_pairs; i += step) a.pairs[i] = -1;
-    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = min(a.n_pages, p0 + kSegment);
+    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
     int x = 0, total;
     for (int p = p0 + (int)threadIdx.x; p < p1; p += 256) x += a.refs[p] != 0;
     block_scan(x, &total, waves);
@@ -301,7 +302,7 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_used(CompactArgs a) {
 
 extern "C" __global__ void __launch_bounds__(256) zt_pool_pair(CompactArgs a) {
     __shared__ int waves[4];
-    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = min(a.n_pages, p0 + kSegment);
+    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
     int used = block_sum(a.seg_used, seg, waves);  // below the segment
     const int L = used + block_sum(a.seg_used + seg, a.segments - seg, waves);
     if (L == a.n_pages && seg == 0 && threadIdx.x == 0) a.moved[0] = a.moved[1] = 0;

@@ -156,10 +156,17 @@ int zt_paged_free(int *table, int *refs, const int *n_keep, int B, int n_pages, 
             least = std::min(least, from);
         }
         if (n == 0) break;
-        // (Pages are less than 2^31 / kThreads workgroups' threads: as many sequences as a launch has room for.)
-        a.blocks = (table_stride - least + kThreads - 1) / kThreads;
-        if (!grid_ok((unsigned long long)n * a.blocks)) return 1;
-        if (launch(st, "zt_pool_free", (unsigned)(n * a.blocks), a, stream)) return 1;
+        a.blocks = (int)(((long long)table_stride - least + kThreads - 1) / kThreads);
+        // As many sequences at a time as a launch has room for (one's table always has).
+        const int at_once = (int)std::min<long long>(n, 0xFFFFFFFFll / kThreads / a.blocks);
+        for (int i0 = 0; i0 < n; i0 += at_once) {
+            const int m = std::min(at_once, n - i0);
+            for (int i = 0; i0 && i < m; ++i) {
+                a.b[i] = a.b[i0 + i];
+                a.from[i] = a.from[i0 + i];
+            }
+            if (launch(st, "zt_pool_free", (unsigned)m * (unsigned)a.blocks, a, stream)) return 1;
+        }
     }
     return 0;
 }
