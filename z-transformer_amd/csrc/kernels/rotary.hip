@@ -12,7 +12,7 @@
 // head at a time, 16 bytes a load where widths allow, several such units in flight.  Bound: HBM: 8192 rows of 32 + 8
 // heads at d = 128 61 to 63 us, 5.4 TB/s (a copy of 2 GiB 5.0).  Measured on MI355X (us): with two rows to a workgroup 64,
 // with four 70; a quarter of each head turned 59.6, with 16 rows to a workgroup (16 angles each) 122; the new tokens of 48
-// sequences, 1952 of 16 + 4 heads at d = 256, and their masks, 23.5 with two units in flight, 31 with four.
+// sequences, 1936 of 16 + 4 heads at d = 256, and their masks, 23.5 with two units in flight, 31 with four.
 #include "common.h"
 #include "args.h"
 #include "paged.h"

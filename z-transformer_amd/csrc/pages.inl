@@ -97,8 +97,8 @@ int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *sr
     while (1 << a.shift < page_size) ++a.shift;
     a.segments = page_segments(n_pages);
     a.entries = n; a.slots = (int)slots;
-    // One workgroup does a small call: freeing, forking 5 entries of 22 columns and copying 19.6 us, with three launches
-    // 26.6, which is their way through the host.  With more columns it takes longer: 78 entries of 66 16.7 us, the three
+    // One workgroup does a small call: freeing, forking 8 entries of 21 columns and copying 19.6 us, with three launches
+    // 26.6, which is their way through the host.  With more columns it takes longer: 78 entries of 65 16.7 us, the three
     // launches 3.8 + 3.0 + 5.1 (the same pass 30.5 / 27.2).
     long long columns = 0;
     for (int i = 0; i < n; ++i) columns += src[i] == dst[i] ? pages_of(n_room[i], page_size) - n_rows[i] / page_size : table_stride;
@@ -201,8 +201,8 @@ int zt_paged_compact(const int *table, const int *refs, int *table_out, int *ref
     a.seg_used = static_cast<int *>(workspace); a.becomes = a.seg_used + a.segments;
     a.entries = (long long)B * table_stride;
     a.n_pages = n_pages; a.max_pairs = max_pairs;
-    // One workgroup does a pool that it numbers in one go and a table of few rounds: 130 pages and their copy 11.8 us, with
-    // three launches 17.7; 3437 pages 7.4 us, the three 7.7 + 10.7 + 4.9.
+    // One workgroup does a pool that it numbers in one go and a table of few rounds: 131 pages and their copy 11.8 us, with
+    // three launches 17.7; 3451 pages 7.4 us, the three 7.7 + 10.7 + 4.9.
     if (n_pages <= ZT_PAGES_ONE && a.entries <= 65536) return launch(st, "zt_pool_compact_one", 1u, a, stream, 1024);
     if (launch(st, "zt_pool_used", (unsigned)a.segments, a, stream)) return 1;
     if (launch(st, "zt_pool_pair", (unsigned)a.segments, a, stream)) return 1;
