@@ -197,6 +197,7 @@ struct ForkArgs {
     int *rank;              // [slots] which of its entry's fresh pages a column takes, or -1
     int *list;              // the free pages in order, `slots` at most
     int n_pages, shift, table_stride, segments, entries, entry0, n, slots;
+    int pieces;             // of 64 columns of an entry, at most (zt_pool_fork_one)
     int src[ZT_PAGES_MAXE], dst[ZT_PAGES_MAXE], n_rows[ZT_PAGES_MAXE], n_room[ZT_PAGES_MAXE], slot0[ZT_PAGES_MAXE];
 };
 

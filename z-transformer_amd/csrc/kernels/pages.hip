@@ -144,11 +144,10 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_fork(ForkArgs a) {
     __syncthreads();           // the pair's -1 before its pages
     const int *from = a.table + (size_t)src * a.table_stride;
     int *to = a.table + (size_t)dst * a.table_stride;
-    for (int j = threadIdx.x; j < want; j += 256) {
+    for (int j = (self ? whole : 0) + (int)threadIdx.x; j < want; j += 256) {
         const int p = from[j];
         const bool there = is_page(p, a.n_pages);
         if (j < whole) {
-            if (self) continue;
             to[j] = p;
             if (there) atomicAdd(a.refs + p, 1);
             continue;
@@ -247,22 +246,25 @@ extern "C" __global__ void __launch_bounds__(1024) zt_pool_fork_one(ForkArgs a) 
             }
         }
     };
-    // 64 columns of an entry at a time, and four such pieces: their reads do not wait for one another.
+    // 64 columns of an entry at a time, of one that grows only those that it may change, and four such pieces: their
+    // reads do not wait for one another.
     constexpr int U = 4;
-    const int pieces = (a.table_stride + 63) >> 6, items = a.n * pieces;
+    const int items = a.n * a.pieces;
     for (int item0 = w; item0 < items; item0 += 16 * U) {
-        int p[U];
+        int p[U], at[U];  // at: the column, or -1
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int item = min(item0 + 16 * u, items - 1), i = item / pieces, j = (item - i * pieces) * 64 + lane;
-            p[u] = j < a.table_stride ? a.table[(size_t)entry[i].src * a.table_stride + j] : -1;
+            const int item = min(item0 + 16 * u, items - 1), i = item / a.pieces;
+            const Entry x = entry[i];
+            const bool self = x.src == x.dst;
+            const int j = (self ? x.whole : 0) + (item - i * a.pieces) * 64 + lane;
+            at[u] = item0 + 16 * u < items && j < (self ? x.want : a.table_stride) ? j : -1;
+            p[u] = at[u] >= 0 ? a.table[(size_t)x.src * a.table_stride + j] : -1;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int item = item0 + 16 * u;
-            if (item >= items) break;
-            const int i = item / pieces, j = (item - i * pieces) * 64 + lane;
-            if (j < a.table_stride) put(i, entry[i], j, p[u]);
+            const int i = min(item0 + 16 * u, items - 1) / a.pieces;
+            if (at[u] >= 0) put(i, entry[i], at[u], p[u]);
         }
     }
 }

@@ -97,13 +97,16 @@ int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *sr
     while (1 << a.shift < page_size) ++a.shift;
     a.segments = page_segments(n_pages);
     a.entries = n; a.slots = (int)slots;
-    // One workgroup does a small call: freeing, forking 8 entries of 21 columns and copying 19.6 us, with three launches
-    // 26.6, which is their way through the host.  With more columns it takes longer: 78 entries of 65 16.7 us, the three
-    // launches 3.8 + 3.0 + 5.1 (the same pass 30.5 / 27.2).
-    long long columns = 0;
-    for (int i = 0; i < n; ++i) columns += src[i] == dst[i] ? pages_of(n_room[i], page_size) - n_rows[i] / page_size : table_stride;
-    const bool one = n <= ZT_PAGES_MAXE && n_pages <= ZT_PAGES_ONE && slots <= ZT_PAGES_ONE_SLOTS && columns <= 2048;
-    // Counts for all entries, a launch for each ZT_PAGES_MAXE; the list; and what they take, in launches alike.
+    // One workgroup does a small call, up to 64 pieces of 64 columns: freeing, forking 8 entries of 21 columns and copying
+    // 19.6 us, with three launches 26.6, which is their way through the host; growing 64 sequences in a pool of 16000 pages
+    // 11.2 us (in one of 30000, three launches, 12.1).  With more it takes longer: 78 entries of 65 columns 16.7 us, the
+    // three launches 3.8 + 3.0 + 5.1 (a pass 30.5 / 27.2).
+    int widest = 1;
+    for (int i = 0; i < n; ++i)
+        widest = std::max(widest, src[i] == dst[i] ? pages_of(n_room[i], page_size) - n_rows[i] / page_size : table_stride);
+    a.pieces = widest / 64 + (widest % 64 != 0);
+    const bool one = n <= ZT_PAGES_MAXE && n_pages <= ZT_PAGES_ONE && slots <= ZT_PAGES_ONE_SLOTS && (long long)n * a.pieces <= 64;
+    // Else counts for all entries, a launch for each ZT_PAGES_MAXE; the list; and what they take, in launches alike.
     for (const bool take : {false, true}) {
         long long slot = 0;
         for (int e0 = 0; e0 < n; e0 += ZT_PAGES_MAXE) {
