@@ -96,6 +96,34 @@ def test_a_line_is_a_chunk(gpu, zt, H, Hkv, d):
     assert np.array_equal(o.cpu().numpy(), out) and np.array_equal(l.cpu().numpy(), lse)
 
 
+def test_a_long_line(gpu, zt):
+    """A tree of 1500 tokens that is a line, as long as its cache and behind other rows: the chunk's outputs, bit for bit."""
+    H, Hkv, d, page, n_rows, q_len = 8, 2, 128, 16, [1500, 1703], [1500, 1500]
+    rng = np.random.default_rng(12)
+    c = Cache(gpu, rng, n_rows, page, Hkv, d)
+    q = gpu.randn(3000, H, d, device="cuda")
+    mask, parent = gpu.empty(3000, 24, device="cuda", dtype=gpu.int64), np.tile(np.arange(-1, 1499, dtype=np.int32), 2)
+    zt.tree_mask(dev(gpu, parent), mask, [0, 1500, 3000])
+    got, want = gpu.empty_like(q), gpu.empty_like(q)
+    ws = gpu.empty(zt.attn_paged_workspace_bytes([0, 1500, 3000], n_rows, H, Hkv, d) + 16, device="cuda", dtype=gpu.uint8)
+    zt.attn_paged_tree(q, c.k, c.v, c.table, mask, got, [0, 1500, 3000], n_rows, page, H, Hkv, d, ws)
+    zt.attn_paged(q, c.k, c.v, c.table, want, [0, 1500, 3000], n_rows, page, H, Hkv, d, ws)
+    assert gpu.equal(got, want)
+
+
+def test_no_tokens(gpu, zt):
+    """Sequences without new tokens: nothing is written."""
+    table, i32 = gpu.zeros(2, 4, device="cuda", dtype=gpu.int32), dict(device="cuda", dtype=gpu.int32)
+    k, v, q = (gpu.full((4, 8, 32), 7.0, device="cuda") for _ in range(3))
+    mask, pos = gpu.full((2, 1), 7, device="cuda", dtype=gpu.int64), gpu.full((2,), 7, **i32)
+    zt.tree_mask(pos, mask, [0, 0, 0], pos, [1, 2])
+    zt.attn_paged_tree(q, k, v, table, mask, q, [0, 0, 0], [5, 0], 8, 1, 1, 32, None)
+    zt.paged_append_at(q, k, v, q, k, v, table, pos, zt.rope_frequencies(32), [0, 0, 0], [5, 0], 8, 1, 1, 32, 32)
+    zt.paged_keep(k, v, table, pos, pos, [0, 0, 0], [5, 0], 8, 1, 32)
+    zt.paged_copy(k, v, gpu.empty(0, 2, **i32), 8, 1, 32)
+    assert all(bool((x == 7).all()) for x in (k, v, q, mask, pos))
+
+
 @pytest.mark.parametrize("wgs", [256, 32768])
 @pytest.mark.parametrize("H,Hkv,d,rows", pagedref.FEW_SHAPES)
 def test_forced_chunk_counts(gpu, zt, tune, H, Hkv, d, rows, wgs):
@@ -283,6 +311,18 @@ def test_many_rows_and_a_q_in_place_beside_a_k_that_is_not(gpu, zt):
         assert np.all(np.abs(y.cpu().numpy() - want) <= bound)
 
 
+def test_more_rows_than_a_launch_takes(gpu, zt):
+    """2^24 + 5 rows, of which a launch takes 2^24 - 1."""
+    rows = (1 << 24) + 5
+    x = gpu.randn(rows, 2, device="cuda")
+    pos = gpu.arange(rows, device="cuda", dtype=gpu.int32)
+    y = gpu.full_like(x, float("nan"))
+    zt.rope_at(x, None, y, None, pos, [0.37], 1, 0, 2, 2)
+    at = np.r_[0:3, 12345, rows - 9:rows]
+    want, bound = treeref.turn(x[at].cpu().numpy()[:, None], at, [0.37], 2, False)
+    assert np.all(np.abs(y[at].cpu().numpy()[:, None] - want) <= bound) and not bool(y.isnan().any())
+
+
 def test_whole_heads_are_the_plain_rope(gpu, zt):
     """Positions in order, whole heads, unscaled: zt_rope_qk_forward's rows, whose angles are t / theta^e where these are
     t theta^-e (a few steps of 64 bits apart)."""
@@ -462,7 +502,7 @@ class Pool:
 @pytest.mark.parametrize("B,stride,n_pages,page,lacks", [(6, 8, 20, 4, True), (200, 70, 4200, 16, True), (70, 300, 5000, 1, True),
                                                          (3, 5, 8192, 1024, False), (150, 4, 4097, 8, False),
                                                          (100, 500, 16385, 1, True), (200, 350, 20011, 2, True), (90, 40, 16384, 8, False),
-                                                         (300, 5, 900, 8, False)])
+                                                         (300, 5, 900, 8, False), (8, 600, 4300000, 1, False)])
 def test_pages_in_use(gpu, zt, B, stride, n_pages, page, lacks):
     """Forks, growth, cuts, frees and compactions at random: tables and counts as treeref has them, the counts those of the
     tables; also calls that lack pages, and page tables that have been cut back into a shared page."""
@@ -548,6 +588,51 @@ def test_copy(gpu, zt, page, Hkv, d):
         for of, to in ((3, 7), (0, 1), (0, 11)):
             y[to] = y[of]
     assert np.array_equal(kd.cpu().numpy(), k) and np.array_equal(vd.cpu().numpy(), v)
+
+
+def test_more_copies_than_a_grid(gpu, zt):
+    """600000 pairs, of which the last and a few others name pages."""
+    k, v = gpu.randn(64, 4, 32, device="cuda"), gpu.randn(64, 4, 32, device="cuda")
+    want = k.clone(), v.clone()
+    pairs = np.full((600000, 2), -1, np.int32)
+    for i, (of, to) in {0: (1, 2), 524287: (3, 4), 524288: (5, 6), 599999: (63, 0)}.items():
+        pairs[i] = of, to
+        for x in want:
+            x[to] = x[of]
+    zt.paged_copy(k, v, dev(gpu, pairs), 4, 1, 32)
+    assert gpu.equal(k, want[0]) and gpu.equal(v, want[1])
+
+
+def test_a_pool_past_32_bits(gpu, zt):
+    """2^31 values and more in K and in V: appends, attention, moves and copies at its end as at its beginning."""
+    H, Hkv, d, page, n, L = 8, 8, 128, 64, 150, 20
+    n_pages = (1 << 31) // (page * Hkv * d) + 40
+    rng = np.random.default_rng(3)
+    k, v = (gpu.empty(n_pages, page, Hkv * d, device="cuda") for _ in range(2))
+    head = gpu.randn(2, 3, page, Hkv * d, device="cuda")
+    table = gpu.tensor([[0, 1, 2], [n_pages - 5, n_pages - 3, n_pages - 1]], device="cuda", dtype=gpu.int32)
+    for b in range(2):
+        k[table[b].long()], v[table[b].long()] = head[0], head[1]
+    up = treeref.random_tree(rng, L)
+    parent = dev(gpu, np.tile(up, 2))
+    q_start, n_rows = [0, L, 2 * L], [n, n]
+    mask, pos = gpu.empty(2 * L, 1, device="cuda", dtype=gpu.int64), gpu.empty(2 * L, device="cuda", dtype=gpu.int32)
+    zt.tree_mask(parent, mask, q_start, pos, [n - L] * 2)
+    new = [gpu.randn(L, Hkv * d, device="cuda").repeat(2, 1) for _ in range(3)]
+    out = gpu.empty(2 * L, H * d, device="cuda")
+    zt.paged_append_at(new[0], new[1], new[2], new[0], k, v, table, pos, zt.rope_frequencies(d), q_start, n_rows, page, H, Hkv, d, d)
+    ws = gpu.empty(zt.attn_paged_workspace_bytes(q_start, n_rows, H, Hkv, d) + 16, device="cuda", dtype=gpu.uint8)
+    zt.attn_paged_tree(new[0], k, v, table, mask, out, q_start, n_rows, page, H, Hkv, d, ws)
+    line = max(treeref.lines(up), key=len)
+    path = np.zeros(2 * L, np.int32)
+    path[:len(line)] = path[L:L + len(line)] = line
+    zt.paged_keep(k, v, table, dev(gpu, path), dev(gpu, np.full(2, len(line), np.int32)), q_start, n_rows, page, Hkv, d)
+    assert gpu.equal(out[:L], out[L:]) and not bool(out.isnan().any())
+    for x in (k, v):
+        assert gpu.equal(x[table[0].long()], x[table[1].long()])
+    zt.paged_copy(k, v, gpu.tensor([[n_pages - 5, n_pages - 20], [0, n_pages - 7]], device="cuda", dtype=gpu.int32), page, Hkv, d)
+    for x in (k, v):
+        assert gpu.equal(x[n_pages - 20], x[0]) and gpu.equal(x[n_pages - 7], x[0])
 
 
 # ---- together -----------------------------------------------------------------------------------

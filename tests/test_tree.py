@@ -141,6 +141,8 @@ def test_workspaces_follow_the_numbers(zt):
     assert need((5,), (5,), n_pages=1025) == 4 * (2 + 1 + 2)
     assert need((5,), (4,)) == need((-1,), (4,)) == need((5,), (5,), page=3) == need((5,), (5,), n_pages=0) == 0
     assert need((0,), ((1 << 30) + 1,)) == 0
+    # Past 2^22 pages segments grow, so that there are 4096 or so.
+    assert need((16,), (16,), n_pages=(1 << 22) + 1024) == 4 * (2049 + 1) and need((16,), (16,), n_pages=2 ** 31 - 1, page=1) == 4 * (4096 + 1)
     assert L.zt_paged_compact_workspace(0) == 0 and L.zt_paged_compact_workspace(4097) == 4 * (5 + 4097)
 
 

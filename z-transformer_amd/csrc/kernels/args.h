@@ -179,7 +179,7 @@ struct PagedEvictArgs {
 };
 
 // Pages: refs[p] counts the table entries that name page p.
-#define ZT_PAGES_SEGMENT 1024   // pages that a workgroup counts
+#define ZT_PAGES_SEGMENT 1024   // pages that a workgroup counts, at least
 #define ZT_PAGES_ONE 16384      // pages of a pool that one workgroup numbers by itself
 #define ZT_PAGES_ONE_SLOTS 4096 // columns that may need a page, of all sequences that it serves
 #define ZT_PAGES_MAXE 128       // entries of a launch that forks
@@ -196,7 +196,7 @@ struct ForkArgs {
     int *entry_fresh;       // [entries] pages wanted
     int *rank;              // [slots] which of its entry's fresh pages a column takes, or -1
     int *list;              // the free pages in order, `slots` at most
-    int n_pages, shift, table_stride, segments, entries, entry0, n, slots;
+    int n_pages, shift, table_stride, segments, segment, entries, entry0, n, slots;  // segment: pages of one
     int pieces;             // of 64 columns of an entry, at most (zt_pool_fork_one)
     int src[ZT_PAGES_MAXE], dst[ZT_PAGES_MAXE], n_rows[ZT_PAGES_MAXE], n_room[ZT_PAGES_MAXE], slot0[ZT_PAGES_MAXE];
 };
@@ -213,7 +213,7 @@ struct CompactArgs {
     int *pairs, *moved;
     int *seg_used, *becomes;  // [segments], [n_pages]
     long long entries;        // of the table
-    int n_pages, segments, max_pairs;
+    int n_pages, segments, segment, max_pairs;
 };
 
 struct CopyArgs {

@@ -75,17 +75,15 @@ DEVI int pool_number(OnePool &s, Flag flag, int (&before)[OnePool::E], int (&wav
 // from there to want = ceil(n_room / page) are its own: kept where src is dst and nobody else refers to the page, else fresh ones.  A
 // fresh page for column `whole` of a partly filled one is asked to be copied: pairs[i].
 // Up to ZT_PAGES_ONE pages and ZT_PAGES_ONE_SLOTS columns a workgroup does it by itself (zt_pool_fork_one); else in
-// three launches: (1) the free pages of each segment of kSegment, and each entry's fresh columns, are counted; (2) the
+// three launches: (1) the free pages of each segment, and each entry's fresh columns, are counted; (2) the
 // free pages are numbered and listed, as many as could be wanted; (3) each entry takes those of its numbers. If there are too few, nothing is
 // changed but `missing`.
-constexpr int kSegment = ZT_PAGES_SEGMENT;
-
 extern "C" __global__ void __launch_bounds__(256) zt_pool_count(ForkArgs a) {
     __shared__ int waves[4];
     if ((int)blockIdx.x >= a.n) {  // a segment
-        const int seg = (int)blockIdx.x - a.n, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
+        const int seg = (int)blockIdx.x - a.n, p0 = seg * a.segment, len = min(a.segment, a.n_pages - p0);
         int x = 0, total;
-        for (int p = p0 + (int)threadIdx.x; p < p1; p += 256) x += a.refs[p] == 0;
+        for (int i = threadIdx.x; i < len; i += 256) x += a.refs[p0 + i] == 0;
         block_scan(x, &total, waves);
         if (threadIdx.x == 0) a.seg_free[seg] = total;
         return;
@@ -115,14 +113,14 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_count(ForkArgs a) {
 
 extern "C" __global__ void __launch_bounds__(256) zt_pool_list(ForkArgs a) {
     __shared__ int waves[4];
-    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
+    const int seg = blockIdx.x, p0 = seg * a.segment, len = min(a.segment, a.n_pages - p0);
     int at = block_sum(a.seg_free, seg, waves);
-    for (int q = p0; q < p1 && at < a.slots; q += 256) {  // workgroup-uniform
-        const int p = q + (int)threadIdx.x;
-        const bool free = p < p1 && a.refs[p] == 0;
+    for (int i0 = 0; i0 < len && at < a.slots; i0 += 256) {  // workgroup-uniform
+        const int i = i0 + (int)threadIdx.x;
+        const bool free = i < len && a.refs[p0 + i] == 0;
         int total;
         const int k = at + block_scan(free, &total, waves);
-        if (free && k < a.slots) a.list[k] = p;
+        if (free && k < a.slots) a.list[k] = p0 + i;
         at += total;
     }
 }
@@ -295,26 +293,26 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_used(CompactArgs a) {
     __shared__ int waves[4];
     const long long step = 256LL * gridDim.x;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < 2LL * a.max_pairs; i += step) a.pairs[i] = -1;
-    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
+    const int seg = blockIdx.x, p0 = seg * a.segment, len = min(a.segment, a.n_pages - p0);
     int x = 0, total;
-    for (int p = p0 + (int)threadIdx.x; p < p1; p += 256) x += a.refs[p] != 0;
+    for (int i = threadIdx.x; i < len; i += 256) x += a.refs[p0 + i] != 0;
     block_scan(x, &total, waves);
     if (threadIdx.x == 0) a.seg_used[seg] = total;
 }
 
 extern "C" __global__ void __launch_bounds__(256) zt_pool_pair(CompactArgs a) {
     __shared__ int waves[4];
-    const int seg = blockIdx.x, p0 = seg * kSegment, p1 = p0 + min(kSegment, a.n_pages - p0);
+    const int seg = blockIdx.x, p0 = seg * a.segment, len = min(a.segment, a.n_pages - p0);
     int used = block_sum(a.seg_used, seg, waves);  // below the segment
     const int L = used + block_sum(a.seg_used + seg, a.segments - seg, waves);
     if (L == a.n_pages && seg == 0 && threadIdx.x == 0) a.moved[0] = a.moved[1] = 0;
-    for (int q = p0; q < p1; q += 256) {  // workgroup-uniform
-        const int p = q + (int)threadIdx.x;
-        const bool live = p < p1 && a.refs[p] != 0;
+    for (int i0 = 0; i0 < len; i0 += 256) {  // workgroup-uniform
+        const int i = i0 + (int)threadIdx.x, p = i < len ? p0 + i : 0;
+        const bool live = i < len && a.refs[p] != 0;
         int total;
         const int before = used + block_scan(live, &total, waves);  // in use below p
         used += total;
-        if (p >= p1) continue;
+        if (i >= len) continue;
         int becomes = kStays;
         if (live && p >= L && L - 1 - before < a.max_pairs) {  // from the highest down
             becomes = L - 1 - before;

@@ -3,7 +3,13 @@
 
 static int pages_of(int rows, int page_size) { return (int)(((long long)rows + page_size - 1) / page_size); }
 
-static int page_segments(int n_pages) { return (int)(((long long)n_pages + ZT_PAGES_SEGMENT - 1) / ZT_PAGES_SEGMENT); }
+// Pages of a segment: few segments, as every workgroup adds up those before its own.
+static int page_segment(int n_pages) {
+    int s = ZT_PAGES_SEGMENT;
+    while (n_pages / s > 4096) s *= 2;
+    return s;
+}
+static int page_segments(int n_pages) { return pages_of(n_pages, page_segment(n_pages)); }
 
 // Columns of a fork's entries that may need a page, -1 where an entry's rows are not usable.
 static long long fork_slots(const int *n_rows, const int *n_room, int n, int page_size) {
@@ -96,6 +102,7 @@ int zt_paged_fork(int *table, int *refs, int *pairs, int *missing, const int *sr
     a.n_pages = n_pages; a.table_stride = table_stride;
     while (1 << a.shift < page_size) ++a.shift;
     a.segments = page_segments(n_pages);
+    a.segment = page_segment(n_pages);
     a.entries = n; a.slots = (int)slots;
     // One workgroup does a small call, up to 64 pieces of 64 columns: freeing, forking 8 entries of 21 columns and copying
     // 19.6 us, with three launches 26.6, which is their way through the host; growing 64 sequences in a pool of 16000 pages
@@ -201,6 +208,7 @@ int zt_paged_compact(const int *table, const int *refs, int *table_out, int *ref
     CompactArgs a{};
     a.table = table; a.refs = refs; a.table_out = table_out; a.refs_out = refs_out; a.pairs = pairs; a.moved = moved;
     a.segments = page_segments(n_pages);
+    a.segment = page_segment(n_pages);
     a.seg_used = static_cast<int *>(workspace); a.becomes = a.seg_used + a.segments;
     a.entries = (long long)B * table_stride;
     a.n_pages = n_pages; a.max_pairs = max_pairs;
