@@ -2,8 +2,9 @@
 // moving the rows that a tree of drafted tokens leaves.
 //
 // refs[p] counts the page-table entries that name page p; a page is free where it is 0.  What a call takes follows
-// from the tables and the counts alone, whatever the order its workgroups run in: free pages are taken from the lowest number up, so
-// the same state gives the same tables.  Counts change by atomic additions only, whose order does not matter.
+// from the tables and the counts alone, whatever the order its workgroups run in: free pages are taken from the lowest
+// number up, so the same state gives the same tables.  Counts change by atomic additions only, whose order does not
+// matter.
 #include "common.h"
 #include "args.h"
 #include "paged.h"
@@ -41,8 +42,8 @@ DEVI int block_sum(const int *counts, int n, int (&waves)[4]) {
     return total;
 }
 
-// The pages of a pool that one workgroup of 1024 threads numbers: thread t takes pages 1024 e + t.  flag(e) of them is
-// counted in the pages' order: of(e, .) pages before thread t's e-th one.
+// The pages of a pool that one workgroup of 1024 threads numbers: thread t takes pages 1024 e + t.  before[e]: how many
+// pages before the thread's e-th one have flag(e); returned: how many have it at all.
 struct OnePool {
     static constexpr int E = ZT_PAGES_ONE / 1024;
     int counts[E * 16];  // of each 64 pages, then before them
@@ -72,12 +73,12 @@ DEVI int pool_number(OnePool &s, Flag flag, int (&before)[OnePool::E], int (&wav
 //
 // Entry i: sequence dst goes on from src's first n_rows rows, with pages for n_room.  Of its table's columns those
 // below whole = n_rows / page are src's pages (one reference more each, where dst is another sequence); the columns
-// from there to want = ceil(n_room / page) are its own: kept where src is dst and nobody else refers to the page, else fresh ones.  A
-// fresh page for column `whole` of a partly filled one is asked to be copied: pairs[i].
-// Up to ZT_PAGES_ONE pages and ZT_PAGES_ONE_SLOTS columns a workgroup does it by itself (zt_pool_fork_one); else in
-// three launches: (1) the free pages of each segment, and each entry's fresh columns, are counted; (2) the
-// free pages are numbered and listed, as many as could be wanted; (3) each entry takes those of its numbers. If there are too few, nothing is
-// changed but `missing`.
+// from there to want = ceil(n_room / page) are its own: kept where src is dst and nobody else refers to the page, else
+// fresh ones.  A fresh page for column `whole` of a partly filled one is asked to be copied: pairs[i].
+// Three launches: (1) the free pages of each segment, and each entry's fresh columns, are counted; (2) the free pages
+// are numbered and listed, as many as could be wanted; (3) each entry takes those of its numbers.  If there are too
+// few, nothing is changed but `missing`.  Few columns in a pool of up to ZT_PAGES_ONE pages: zt_pool_fork_one.
+// Bound: a launch, and in it a chain of trips to memory (arguments, table, counts); an entry's pages are all in flight.
 extern "C" __global__ void __launch_bounds__(256) zt_pool_count(ForkArgs a) {
     __shared__ int waves[4];
     if ((int)blockIdx.x >= a.n) {  // a segment
