@@ -96,6 +96,34 @@ def test_a_line_is_a_chunk(gpu, zt, H, Hkv, d):
     assert np.array_equal(o.cpu().numpy(), out) and np.array_equal(l.cpu().numpy(), lse)
 
 
+@pytest.mark.parametrize("n,L", [(16, 16), (29, 29), (300, 17), (700, 26), (1021, 31)])
+@pytest.mark.parametrize("H,Hkv,d", [(8, 2, 64), (4, 1, 50), (8, 2, 96), (12, 3, 82), (32, 8, 128), (4, 1, 98)])
+def test_a_small_grid_of_65_to_128_rows(gpu, zt, H, Hkv, d, n, L):
+    """The shape that only trees have (five to eight blocks of 16 rows, one chunk or several), with a value past 2^40 and one
+    that is not finite in rows of the tree that some tokens do not see."""
+    rng = np.random.default_rng([H, d, n])
+    c = Cache(gpu, rng, [n], 16, Hkv, d, garbage=np.nan)
+    q = rng.standard_normal((L, H, d)).astype(np.float32)
+    up = treeref.random_tree(rng, L)
+    mask = treeref.masks([up], 1)[0]
+    check(run_tree(gpu, zt, c, q, mask, [0, L], H), reference(c, q, mask, [0, L], H), [0, L])
+    at = pagedref.places(c.table_h, 0, n, 16)[n - L + L // 2]
+    c.v_h[at, :, 1] = np.float32(2.0 ** 50)
+    c.k_h[at, :, 2] = np.float32(2.0 ** 41)
+    q[:, :, 2] = np.float32(2.0 ** -40)
+    c.k, c.v = dev(gpu, c.k_h), dev(gpu, c.v_h)
+    got, ref = run_tree(gpu, zt, c, q, mask, [0, L], H), reference(c, q, mask, [0, L], H)
+    check(got, ref, [0, L])
+    hit = np.array([L // 2 in line for line in treeref.lines(up)])
+    before = run_tree(gpu, zt, c, q, mask, [0, L], H)
+    c.v[at, :, 5] = float("nan")
+    c.k[at, :, 7] = float("inf")
+    after = run_tree(gpu, zt, c, q, mask, [0, L], H)
+    assert hit.any() and not hit.all()
+    assert np.array_equal(before[0][~hit], after[0][~hit]) and np.array_equal(before[1][~hit], after[1][~hit])
+    assert np.all(np.isnan(after[0][hit][..., 5]))
+
+
 def test_a_long_line(gpu, zt):
     """A tree of 1500 tokens that is a line, as long as its cache and behind other rows: the chunk's outputs, bit for bit."""
     H, Hkv, d, page, n_rows, q_len = 8, 2, 128, 16, [1500, 1703], [1500, 1500]
