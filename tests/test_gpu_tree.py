@@ -603,6 +603,40 @@ def test_a_full_pool_and_an_empty_one(gpu, zt, n_pages):
     p.compact(n_pages, True)
 
 
+def test_the_widest_tables(gpu, zt):
+    """Tables of 2^31 - 1 columns, the most that an int counts: a fork, a compaction and a free reach their last column and
+    leave what lies behind it."""
+    stride, behind = 2 ** 31 - 1, 4096
+    flat = gpu.full((2 * stride + behind,), 7, device="cuda", dtype=gpu.int32)
+    flat[:stride] = -1
+    table = flat[:2 * stride].view(2, stride)
+    flat[0], flat[1] = 3, 5
+    refs = gpu.tensor([0, 0, 0, 1, 0, 1, 1, 0], device="cuda", dtype=gpu.int32)
+    pairs, missing = gpu.full((1, 2), 9, device="cuda", dtype=gpu.int32), gpu.full((1,), 9, device="cuda", dtype=gpu.int32)
+
+    def holds(row0, row1):
+        """The rows begin so; all else in the tables is -1, behind them 7."""
+        for at, x in ((0, row0), (stride, row1)):
+            assert flat[at:at + len(x)].tolist() == x
+            for i in range(at + len(x), at + stride, 1 << 28):
+                assert bool((flat[i:min(i + (1 << 28), at + stride)] == -1).all()), i
+        assert bool((flat[2 * stride:] == 7).all())
+
+    ws = gpu.empty(zt.paged_fork_workspace_bytes([6], [9], 8, 4), device="cuda", dtype=gpu.uint8)
+    zt.paged_fork(table, refs, pairs, missing, [0], [1], [6], [9], 4, ws)
+    assert pairs.tolist() == [[5, 0]] and missing.tolist() == [0] and refs.tolist() == [1, 1, 0, 2, 0, 1, 1, 0]
+    holds([3, 5], [3, 0, 1])
+    flat[stride - 1] = 6  # the last column's page moves, and is given back
+    pairs, moved = gpu.full((8, 2), 9, device="cuda", dtype=gpu.int32), gpu.full((2,), 9, device="cuda", dtype=gpu.int32)
+    ws = gpu.empty(zt.paged_compact_workspace_bytes(8), device="cuda", dtype=gpu.uint8)
+    zt.paged_compact(table, refs, table, refs, pairs, moved, ws)
+    assert pairs.tolist() == [[6, 2], [5, 4]] + [[-1, -1]] * 6 and moved.tolist() == [2, 0]
+    assert int(flat[stride - 1]) == 2 and refs.tolist() == [1, 1, 1, 2, 1, 0, 0, 0]
+    zt.paged_free(table, refs, [8, 4], 4)
+    assert refs.tolist() == [0, 0, 0, 2, 1, 0, 0, 0]
+    holds([3, 4], [3])
+
+
 @pytest.mark.parametrize("page,Hkv,d", [(1, 2, 32), (8, 8, 128), (16, 3, 50), (64, 1, 34), (1024, 2, 256)])
 def test_copy(gpu, zt, page, Hkv, d):
     rng = np.random.default_rng([page, d])

@@ -162,8 +162,8 @@ extern "C" __global__ void __launch_bounds__(256) zt_pool_fork(ForkArgs a) {
             a.pairs[2 * i + 1] = f;
         }
     }
-    if (!self)  // behind its pages a new sequence has none
-        for (int j = want + (int)threadIdx.x; j < a.table_stride; j += 256) to[j] = -1;
+    if (!self)  // behind its pages a new sequence has none (64 bits: the step past a wide table's end is one past an int's)
+        for (long long j = want + (int)threadIdx.x; j < a.table_stride; j += 256) to[j] = -1;
 }
 
 // The same by one workgroup, a wave to an entry.  The entries are read from the arguments, which are far, once, all at
