@@ -575,6 +575,41 @@ def test_pages_in_use(gpu, zt, B, stride, n_pages, page, lacks):
     assert (lacked > 0) == lacks
 
 
+@pytest.mark.parametrize("B,stride,n_pages,most", [(40, 512, 1, 1), (64, 192, 16384, 16384), (1, 12289, 16384, 9000), (64, 1024, 16384, 500),
+                                                   (3, 6660, 1000, 1000), (3, 6661, 1000, 999), (5, 7, 4096, 9000), (5, 7, 4097, 4097),
+                                                   (5, 7, 4097, 4098), (2, 20000, 900, 70000)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_compaction_of_small_and_of_wide_tables(gpu, zt, B, stride, n_pages, most, in_place):
+    """Tables and pairs on both sides of what one workgroup is given; two thirds of the pool in use, some pages by several
+    entries, a call that leaves pages to move and one that finishes."""
+    rng = np.random.default_rng([B, stride, n_pages])
+    p = Pool(gpu, zt, B, stride, n_pages, 1)
+    live = rng.permutation(n_pages)[:max(1, min(2 * n_pages // 3, B * stride // 2))]
+    at = rng.permutation(B * stride)[:len(live) + len(live) // 3]
+    p.ref.table.reshape(-1)[at] = np.concatenate([live, live])[:len(at)]
+    p.ref.table[0, :3] = [n_pages, -5, 2 ** 31 - 1]
+    p.ref.refs[:] = p.ref.counted()
+    p.load()
+    for few in (7, most):
+        p.compact(min(few, most), in_place)
+        assert np.array_equal(p.ref.refs, p.ref.counted())
+
+
+@pytest.mark.parametrize("B,stride,n_pages,most,one", [(8, 128, 1000, 500, True), (64, 192, 1000, 500, True), (64, 1024, 1000, 500, False),
+                                                       (64, 1024, 16384, 500, False), (8, 128, 16384, 100000, False)])
+def test_who_compacts(gpu, zt, B, stride, n_pages, most, one):
+    """A single workgroup keeps its numbers to itself, three launches hand theirs on in the workspace: wide tables, and lists of
+    pairs far beyond a large pool, are not left to one."""
+    table, refs = gpu.full((B, stride), -1, device="cuda", dtype=gpu.int32), gpu.zeros(n_pages, device="cuda", dtype=gpu.int32)
+    pairs, moved = gpu.full((most, 2), 7, device="cuda", dtype=gpu.int32), gpu.full((2,), 7, device="cuda", dtype=gpu.int32)
+    table[0, 0], refs[n_pages - 1] = n_pages - 1, 1
+    ws = gpu.full((zt.paged_compact_workspace_bytes(n_pages) // 4,), -9, device="cuda", dtype=gpu.int32)
+    zt.paged_compact(table, refs, table, refs, pairs, moved, ws)
+    assert pairs[0].tolist() == [n_pages - 1, 0] and bool((pairs[1:] == -1).all()) and moved.tolist() == [1, 0]
+    assert int(table[0, 0]) == 0 and int(refs[0]) == 1 and int(refs.sum()) == 1
+    assert bool((ws == -9).all()) == one
+
+
 def test_entries_that_name_no_page(gpu, zt):
     """Numbers outside the pool in a table: shared as they are, not counted, replaced where a sequence grows, dropped where it is
     freed; compaction leaves them."""

@@ -212,9 +212,13 @@ int zt_paged_compact(const int *table, const int *refs, int *table_out, int *ref
     a.seg_used = static_cast<int *>(workspace); a.becomes = a.seg_used + a.segments;
     a.entries = (long long)B * table_stride;
     a.n_pages = n_pages; a.max_pairs = max_pairs;
-    // One workgroup does a pool that it numbers in one go and a table of few rounds: 131 pages and their copy 11.8 us, with
-    // three launches 17.7; 3451 pages 7.4 us, the three 7.7 + 10.7 + 4.9.
-    if (n_pages <= ZT_PAGES_ONE && a.entries <= 65536) return launch(st, "zt_pool_compact_one", 1u, a, stream, 1024);
+    // One workgroup does a pool that it numbers in one go and a table of few rounds, each a trip to memory.  Measured on MI355X
+    // (us, one workgroup / three launches): 96 entries and 131 pages 5.5 / 9.2, 19980 and 1000 8.8 / 10.3, 32768 and 1000 11.2 /
+    // 9.1; 8192 and 16384 9.3 / 10.1, 12288 10.0 / 10.1, 16384 10.8 / 10.1, 65536 (64 tables of 1024) 19.5 / 10.1.  Pairs beyond
+    // the pool's pages, which no call needs, are cleared by it or by a workgroup for each segment: 100000 with 1024
+    // entries and 1000 pages 13.3 / 29.1, 4000 13.9 / 14.8, 16384 16.0 / 11.7.
+    const bool one = n_pages <= ZT_PAGES_ONE && a.entries + n_pages / 2 <= 20480 && (max_pairs <= n_pages || n_pages <= 4096);
+    if (one) return launch(st, "zt_pool_compact_one", 1u, a, stream, 1024);
     if (launch(st, "zt_pool_used", (unsigned)a.segments, a, stream)) return 1;
     if (launch(st, "zt_pool_pair", (unsigned)a.segments, a, stream)) return 1;
     const long long work = std::max<long long>(a.entries, n_pages);
