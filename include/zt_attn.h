@@ -251,7 +251,11 @@ int zt_tree_mask(const int *parent, uint64_t *mask, int *pos_out, const int *q_s
 /* zt_attn_paged where a new token sees the rows before the new ones, as there, and of those
  * only the tokens of its mask, none behind itself (bits of later tokens are ignored): zt_tree_mask's, or any
  * other.  A token that sees nothing (no row before the new ones, and an empty mask) has out 0 and lse
- * -inf.  `workspace`: zt_attn_paged_workspace(..., 0) bytes for the same lengths.  All else as zt_attn_paged. */
+ * -inf.  `workspace`: zt_attn_paged_workspace(..., 0) bytes for the same lengths.  Limits, checks and what may overlap
+ * are zt_attn_paged's.  It accumulates no weights: of a row that zt_paged_append_at wrote with w, w stays 0, other rows
+ * get nothing, and zt_paged_evict would take the accepted rows first.  A cache that is evicted by w has, after
+ * zt_paged_keep, its accepted tokens attended once more as a chunk: zt_attn_paged of their q (packed, with the new n_rows)
+ * with w_in and w_out adds what they draw. */
 int zt_attn_paged_tree(const float *q, const float *k_pages, const float *v_pages, const int *table, const uint64_t *mask,
                        float *out, float *lse, const int *q_start, const int *n_rows, int B, int n_pages, int page_size,
                        int table_stride, int words, int n_heads, int n_kv_heads, int dim, void *workspace,
@@ -260,8 +264,9 @@ int zt_attn_paged_tree(const float *q, const float *k_pages, const float *v_page
 /* The rows that stay of the new ones: of each sequence's new tokens the one with number path[i] becomes new
  * row i, for i < count[b] (DEVICE ints; path packed as q's rows, path[i] >= i, as in any tree; others, and
  * numbers of no new token, move nothing).  The sequence's new n_rows is n_rows less its new tokens plus
- * count[b]; rows behind those are left as they are.  n_rows and q_start (HOST) are those of the append.  The pages of the
- * new rows must not be shared.  Where a row's old or new page is none of the pool's, it is not moved. */
+ * count[b]; rows behind those are left as they are, and so are accumulated weights.  n_rows and q_start (HOST) are those
+ * of the append.  The pages of the new rows must not be shared.  Where a row's old or new page is none of the pool's, it
+ * is not moved. */
 int zt_paged_keep(float *k_pages, float *v_pages, const int *table, const int *path, const int *count, const int *q_start,
                   const int *n_rows, int B, int n_pages, int page_size, int table_stride, int n_kv_heads, int dim,
                   hipStream_t stream);
@@ -278,7 +283,9 @@ int zt_paged_keep(float *k_pages, float *v_pages, const int *table, const int *p
  * rest are free pages.  Where src[i] == dst[i] (growth), pages that are there stay, but a page from the
  * partly filled one on that another entry names as well is replaced, as every page that the sequence may write must be
  * its own.  pairs [n, 2] (DEVICE) receives the old and the new number of the page to copy, -1, -1 where there is
- * none; an old page may be free by then, and is to be copied before another call takes pages.  Pages are taken from the
+ * none (the old number as the table has it, which zt_paged_copy passes over if it is none of the pool's); an old page may
+ * be free by then, and is to be copied before another call takes pages.  Accumulated weights are by sequence: a new
+ * one's are the caller's to copy.  Pages are taken from the
  * lowest free number up, in the order of entries and columns.  If fewer are free than needed, *missing (DEVICE) receives
  * how many are short, pairs -1, and nothing else changes; else it receives 0.  dst are all different, and none is another
  * entry's src.  n <= B.  `workspace`: zt_paged_fork_workspace(...) bytes, 16-byte aligned. */

@@ -828,6 +828,49 @@ def test_page_calls_in_a_graph(gpu, zt):
         assert all(gpu.equal(x, y) for x, y in zip(want, (p.table, p.refs, pairs, missing, k, v, t2, r2, cp, moved)))
 
 
+@pytest.mark.parametrize("H,Hkv,d", [(8, 2, 64), (6, 3, 50), (32, 8, 128)])
+def test_weights_beside_trees(gpu, zt, H, Hkv, d):
+    """A tree's step accumulates no weights: its rows have 0, the others keep theirs.  The accepted tokens attended once more, as
+    a chunk, add what they draw, those rows among them."""
+    n_rows, q_len, page, rot = [60, 200, 33, 9], [9, 40, 5, 9], 8, 24
+    rng = np.random.default_rng([H, d, 5])
+    c, B = Cache(gpu, rng, n_rows, page, Hkv, d, garbage=np.nan), len(n_rows)
+    q_start = np.cumsum([0] + q_len).tolist()
+    N = q_start[-1]
+    parents = [treeref.random_tree(rng, n, 0.8) for n in q_len]
+    mask, pos = gpu.empty(N, 1, device="cuda", dtype=gpu.int64), gpu.empty(N, device="cuda", dtype=gpu.int32)
+    zt.tree_mask(dev(gpu, np.concatenate(parents)), mask, q_start, pos, [n - L for n, L in zip(n_rows, q_len)])
+    q, kn, vn = (dev(gpu, rng.standard_normal((N, h, d)).astype(np.float32)) for h in (H, Hkv, Hkv))
+    w = rng.random((B, Hkv, max(n_rows) + 3), np.float32)
+    wd, out = dev(gpu, w), gpu.empty(N, H, d, device="cuda")
+    zt.paged_append_at(q, kn, vn, q, c.k, c.v, c.table, pos, zt.rope_frequencies(rot), q_start, n_rows, page, H, Hkv, d, rot, w=wd)
+    ws = gpu.empty(zt.attn_paged_workspace_bytes(q_start, n_rows, H, Hkv, d) + 16, device="cuda", dtype=gpu.uint8)
+    zt.attn_paged_tree(q, c.k, c.v, c.table, mask, out, q_start, n_rows, page, H, Hkv, d, ws)
+    lines = [max(treeref.lines(up), key=len) for up in parents]
+    path, count = np.zeros(N, np.int32), np.array([len(x) for x in lines], np.int32)
+    for t0, line in zip(q_start, lines):
+        path[t0:t0 + len(line)] = line
+    zt.paged_keep(c.k, c.v, c.table, dev(gpu, path), dev(gpu, count), q_start, n_rows, page, Hkv, d)
+    for b, (n, L) in enumerate(zip(n_rows, q_len)):
+        w[b, :, n - L:n] = 0
+    assert np.array_equal(wd.cpu().numpy(), w)
+    rows = [n - L + len(x) for n, L, x in zip(n_rows, q_len, lines)]
+    begin = np.cumsum([0] + [len(x) for x in lines]).tolist()
+    took = np.concatenate([t0 + np.array(line) for t0, line in zip(q_start, lines)])
+    q2 = q[dev(gpu, took)].contiguous()
+    out2 = gpu.empty_like(q2)
+    ws = gpu.empty(zt.attn_paged_workspace_bytes(begin, rows, H, Hkv, d, True), device="cuda", dtype=gpu.uint8)
+    zt.attn_paged(q2, c.k, c.v, c.table, out2, begin, rows, page, H, Hkv, d, ws, w_in=wd, w_out=wd)
+    k, v, got = c.k.cpu().numpy(), c.v.cpu().numpy(), wd.cpu().numpy()
+    ref, _, drawn, bound, w_bound = pagedref.attend(q2.cpu().numpy(), k, v, c.table_h, begin, rows, page, H, Hkv, d)
+    assert np.all(np.abs(out2.cpu().numpy() - ref) <= bound)
+    for b, n in enumerate(rows):
+        want = w[b, :, :n] + drawn[b, :, :n]
+        assert np.all(np.abs(got[b, :, :n] - want) <= w_bound[b, :, :n] + 2 * EPS * np.abs(want))
+        assert np.array_equal(got[b, :, n:], w[b, :, n:])
+        assert np.all(got[b, :, n - len(lines[b]):n] > 0)
+
+
 @pytest.mark.parametrize("H,Hkv,d,rot,inter", [(8, 2, 64, 64, False), (6, 3, 50, 24, True), (32, 8, 128, 64, False)])
 def test_drafting(gpu, zt, H, Hkv, d, rot, inter):
     """Sequences that share a prompt's pages answer by drafted trees: each step they get room, the tree goes into the cache and
