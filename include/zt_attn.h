@@ -322,7 +322,7 @@ int zt_paged_copy(float *k_pages, float *v_pages, const int *pairs, int n_pairs,
  *                   by factor, the highest stays;
  *   ZT_ROPE_TURNS   by the turns r = context f_i / 2 pi that a pair makes within the trained context: f_i where r >= high,
  *                   f_i / factor where r <= low, and between them (1 - s) f_i / factor + s f_i, s = (r - low) / (high - low).
- * Arguments that a scaling does not name are not read. */
+ * Arguments that a scaling does not name are not read; numbers whose base or frequencies are beyond 64 bits are refused. */
 enum { ZT_ROPE_PLAIN = 0, ZT_ROPE_LINEAR = 1, ZT_ROPE_BASE = 2, ZT_ROPE_TURNS = 3 };
 int zt_rope_frequencies(double *freq, int rot_dim, double theta, int scaling, double factor, double low, double high,
                         double context);

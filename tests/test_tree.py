@@ -172,6 +172,19 @@ def test_frequencies_refuse(zt, args):
         zt.rope_frequencies(*args)
 
 
+@pytest.mark.parametrize("args", [(4, 1.0, 2, 1e-200), (4, 5e5, 2, 1e300), (32, 1e4, 1, 1e-310), (32, 1e4, 1, 5e-324),
+                                  (128, 1e-320, 3, 5e-324, 1e300, 2e300, 1.0)])
+def test_frequencies_beyond_64_bits_are_refused(zt, capfd, args):
+    """Usable numbers by themselves, whose base or quotient is none; nothing is written."""
+    freq = (ctypes.c_double * 128)(*[-7.0] * 128)
+    rot, theta, scaling, factor, low, high, context = (list(args) + [1.0, 4.0, 8192.0][len(args) - 4:])[:7]
+    assert zt.lib().zt_rope_frequencies(freq, rot, theta, scaling, factor, low, high, context) == 1
+    assert "beyond 64 bits" in capfd.readouterr().err and set(freq) == {-7.0}
+    # As far as 64 bits go they are had.
+    assert zt.lib().zt_rope_frequencies(freq, 4, 5e5, 2, 1e100, 0.0, 0.0, 0.0) == 0 and 0 < freq[1] < 1e-100
+    assert zt.lib().zt_rope_frequencies(freq, 4, 1e4, 1, 1e-300, 0.0, 0.0, 0.0) == 0 and np.isfinite(freq[1]) and freq[0] == 1 / 1e-300
+
+
 def test_the_binding_does_not_wrap(zt):
     for call in (lambda: zt.paged_fork_workspace_bytes([1 << 32], [5], 8, 4), lambda: zt.paged_fork_workspace_bytes([5], [5], 1 << 32, 4),
                  lambda: zt.paged_compact_workspace_bytes((1 << 32) + 8), lambda: zt.rope_frequencies((1 << 32) + 32)):

@@ -21,6 +21,7 @@ int zt_rope_frequencies(double *freq, int rot_dim, double theta, int scaling, do
         return 1;
     }
     const double b = base ? theta * std::pow(factor, rot_dim / (rot_dim - 2.0)) : theta;
+    double got[kMaxDim / 2];
     for (int i = 0; i < rot_dim / 2; ++i) {
         const double f = std::pow(b, -2.0 * i / rot_dim);
         double by = scaling == ZT_ROPE_LINEAR ? 1.0 / factor : 1.0;
@@ -29,8 +30,13 @@ int zt_rope_frequencies(double *freq, int rot_dim, double theta, int scaling, do
             const double part = std::min(1.0, std::max(0.0, (r - low) / (high - low)));
             by = part + (1.0 - part) / factor;
         }
-        freq[i] = f * by;
+        got[i] = f * by;
+        if (!(b > 0.0) || !std::isfinite(b) || !std::isfinite(got[i])) {
+            fprintf(stderr, "zt_rope: frequency %d of theta %g, scaled by %g, is beyond 64 bits.\n", i, theta, factor);
+            return 1;
+        }
     }
+    std::copy(got, got + rot_dim / 2, freq);
     return 0;
 }
 
