@@ -13,6 +13,11 @@
 // heads at d = 128 61 to 63 us, 5.4 TB/s (a copy of 2 GiB 5.0).  Measured on MI355X (us): with two rows to a workgroup 64,
 // with four 70; a quarter of each head turned 59.6, with 16 rows to a workgroup (16 angles each) 122; the new tokens of 48
 // sequences, 1936 of 16 + 4 heads at d = 256, and their masks, 23.5 with two units in flight, 31 with four.
+//
+// The append beside zt_rope_paged_*, which turns whole heads, halves as pairs, at positions that the host counts up, with
+// zt_rope_forward's angles bit for bit, and several tokens to a workgroup where heads are narrow.  On the device (us, that one
+// / this one): 64 tokens, one a sequence, of 32 + 8 heads at d = 128 8.0 / 5.4, 1920 of 16 + 4 at d = 256 23.8 / 23.8, 8000 of
+// 32 + 8 at d = 128 68.6 / 68.0, 8000 of 4 + 2 at d = 32 10.6 / 15.9.
 #include "common.h"
 #include "args.h"
 #include "paged.h"

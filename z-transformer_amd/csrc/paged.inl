@@ -485,9 +485,13 @@ static int paged_attend(const char *who, const float *q, const float *k_pages, c
         const bool few = paged_few(kind);
         PagedShape shape = paged_shape(kind, dp);
         // Trees of 65 to 128 rows on a grid of at most one workgroup per CU take eight waves of 16 rows, two to a SIMD, and not
-        // four of 32 that nothing runs beside.  Measured on MI355X (us, four / eight): 26 tokens of 32 over 8 heads at d = 128 on 1000
-        // rows 29.6 / 25.5, 4103 (208 workgroups) 38.4 / 32.5, 30 of 24 over 8 heads at d = 96 on 4000 27.6 / 24.8, 4 sequences of 40
-        // of 12 over 4 at d = 64 on 2000 24.9 / 24.1; past it, 26 on 8000 52.6 / 57.0; 50 of 4 over 2 at d = 32 on 2000 20.3 / 21.5.
+        // four of 32 that nothing runs beside.  Measured on MI355X (us, four / eight): 26 tokens of 32 over 8 heads at d = 128
+        // on 1000 rows 31.0 / 24.9, 4103 (208 workgroups) 36.3 / 29.8, 30 of 24 over 8 heads at d = 96 on 4000 27.4 / 24.8, 4
+        // sequences of 40 of 12 over 4 at d = 64 on 2000 24.9 / 23.4; past it, 26 on 8000 50.5 / 56.2, two of them 75.5 / 76.0
+        // (but 24 sequences of 20 on 3192 to 8114 rows 482.6 / 454.8); 50 of 4 over 2 at d = 32 on 2000 20.3 / 21.5.
+        // Chunks stay with the kernels that they had: eight waves of 16 rows are not built for them (26 tokens on 4103 rows
+        // as a chunk 36.1).  The shape does not change the plan, whose workspace depends on no device and whose cuts are for
+        // two workgroups of four waves to a CU.
         if (tree && kind == kMany128 && dp >= 64 && dp <= 128) {
             long long wgs = 0;
             for (int b = 0; b < B; ++b)
